@@ -405,6 +405,59 @@ int jl_matvec_dev_prepared(jl_ctx *ctx, float *out_dev, const jl_weight *w, int 
 int jl_gemm_operand(jl_ctx *ctx, const jl_weight *w, int ntok, void **rows_f16, float **inv_scale);
 int jl_matmul_dev_prepared(jl_ctx *ctx, void *out_dev, int out_dtype, const jl_weight *w, int ntok, void *stream);
 
+/* ---- several sequences at once: packed prompts, a cache in pages (no seam in the reference, which decodes one sequence:
+ * its attention over a whole prompt is a Go loop of engine/model/forward.go) --------------------------------------------
+ * Attention of grouped query heads (query head h reads kv head h / (hq / n_kv)), causal within each sequence:
+ *   out[r][h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[r][h] . k_j - max),   j = 0 .. r's own position
+ * q, k and v are f16 or bf16 (one type), sums and softmax f32. out [total][hq][d] is f32, f16 or bf16; for an f32 result the softmax
+ * weights enter the product with V as two 16-bit values, for a 16-bit one as one (half a unit of that type at most on each).
+ * Served: d of 64 and 128, hq / n_kv up to 16.
+ *
+ * The sequences are described on the device, so that a captured graph can be replayed on other lengths: new rows of sequence s are rows
+ * starts[s] .. starts[s + 1] - 1 of q and out (int32 [n_seq + 1], ascending from 0; equal entries: no new rows). Rows at and behind
+ * starts[n_seq] are left as they were.
+ *
+ * scratch: jl_attn_scratch_bytes(ctx) bytes of the caller's device memory, in any state; a call uses it until its kernels are done, so
+ * calls that may overlap (streams, graphs replayed side by side) need one each. All memory is the context's device's, whatever device
+ * is current; the calls neither allocate nor wait. */
+size_t jl_attn_scratch_bytes(jl_ctx *ctx);
+/* Prompts: the positions of a sequence are its rows. k, v [total][n_kv][d] with strides in elements (multiples of 8: rows of a fused
+ * projection, or a [n_kv][max_len][d] cache); q likewise. */
+int jl_attn_prompt(jl_ctx *ctx, void *out_dev, int out_dtype, const void *q_dev, long long q_tok_stride, long long q_head_stride,
+                   const void *k_dev, const void *v_dev, long long kv_tok_stride, long long kv_head_stride, int dtype,
+                   const int32_t *starts_dev, int nseq, int total, int hq, int hkv, int d, float scale, void *scratch_dev,
+                   size_t scratch_bytes, void *stream);
+/* A cache in pages that sequences of different lengths share: k and v are [n_pages][n_kv][page_len][head_dim], position p of sequence s
+ * lies in page page_table[s * max_pages + p / page_len]. Pages hold 16 to 1024 positions, a power of two. Sequences may share pages
+ * (a common prefix). Entries of the table behind a sequence's length are not read, nor are positions behind it in its last page. */
+typedef struct jl_paged_kv {
+    uint32_t struct_size;
+    int32_t dtype;                       /* JL_DT_F16 or JL_DT_BF16 */
+    int32_t n_kv, head_dim, page_len;
+    int32_t n_pages;                     /* pages of the pool */
+    int32_t n_seq, max_pages;            /* rows and columns of the table */
+    void *k, *v;                         /* device */
+    const int32_t *page_table;           /* device [n_seq][max_pages] */
+} jl_paged_kv;
+/* lens[s] positions of sequence s are in the cache (int32, device), the last of them its new rows': new row i of n sits at position
+ * lens[s] - n + i and sees the positions up to its own. A row before position 0 sees nothing: its result is zero. A page number outside
+ * the pool, or a length beyond the table, is never followed: the results of the rows that read there are NaN, and so may be the
+ * sequence's other rows. max_new: the most new rows that any sequence has, as far as the host knows; it picks the kernel, not the
+ * result. */
+int jl_attn_paged(jl_ctx *ctx, void *out_dev, int out_dtype, const void *q_dev, long long q_tok_stride, long long q_head_stride,
+                  const jl_paged_kv *kv, const int32_t *starts_dev, const int32_t *lens_dev, int total, int max_new, int hq, float scale,
+                  void *scratch_dev, size_t scratch_bytes, void *stream);
+/* The cache's writer, in front of jl_attn_paged: rows of qkv [total][(hq + 2 n_kv) * head_dim] (f32, f16 or bf16) are new rows as above;
+ * q goes out rotated to its position as [total][hq][head_dim] of the cache's type, k (rotated) and v go to their position's page.
+ * cos / sin: f32 [max_pos][head_dim / 2], adjacent-pair rotation. A row at a position outside [0, max_pos) or the table is left out; k
+ * and v of a page number outside the pool are dropped. No two rows of a call may have the same place in the pool. head_dim % 4 == 0. */
+int jl_rope_append(jl_ctx *ctx, void *q_out_dev, const void *qkv_dev, int x_dtype, const jl_paged_kv *kv, const int32_t *starts_dev,
+                   const int32_t *lens_dev, int total, int hq, const float *cos_t, const float *sin_t, int max_pos, void *stream);
+/* Test-only, host: how a launch of `grid` CTAs divides the work; segs[n][6] = sequence, block of tok_item tokens, kv head, first unit,
+ * end unit, units of the item. Returns n. max_pages 0: no table. */
+int jl_test_attn_share(const int32_t *starts, const int32_t *lens, int nseq, int total, int hkv, int tok_item, int unit_shift, int min_units,
+                       int page_shift, int max_pages, int grid, int cta, int32_t *segs, int cap);
+
 /* ---- whole blocks in one submission: nn.LayerDevice (engine/nn/device.go:1096-1176) ------------
  * PrepLayer hands a block's weights to the device, Layers runs blocks [lo, hi) for the positions of one
  * step without the residual stream leaving the device, an optional Head continues the same submission

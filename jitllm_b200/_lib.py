@@ -79,8 +79,14 @@ class LayersDesc(C.Structure):
                 ("rank", C.c_int32), ("world", C.c_int32)]
 
 
+class PagedKVDesc(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("dtype", C.c_int32), ("n_kv", C.c_int32), ("head_dim", C.c_int32), ("page_len", C.c_int32),
+                ("n_pages", C.c_int32), ("n_seq", C.c_int32), ("max_pages", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p),
+                ("page_table", C.c_void_p)]
+
+
 # Every symbol include/jitllm_b200.h declares: (restype, argtypes).
-_VP, _I, _SZ, _U32 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint32
+_VP, _I, _SZ, _U32, _LL = C.c_void_p, C.c_int, C.c_size_t, C.c_uint32, C.c_longlong
 TUNE_OFF, TUNE_ON, TUNE_FORCE = 0, 1, 2
 MOE_ARM_EXACT, MOE_ARM_BLOCK_SCALED, MOE_ARM_BLOCK_SCALED_X3 = 0, 1, 2
 TUNE_TIMER = C.CFUNCTYPE(C.c_double, C.c_void_p, C.c_int, C.c_int)
@@ -150,6 +156,11 @@ SYMBOLS = {
     "jl_gemm_operand": (_I, [_VP, _VP, _I, C.POINTER(_VP), C.POINTER(_VP)]),
     "jl_matmul_dev_prepared": (_I, [_VP, _VP, _I, _VP, _I, _VP]),
     "jl_aux_add_rmsnorm_gemm": (_I, [_VP, _VP, _VP, C.c_float, _VP, _VP, _I, _I, _VP]),
+    "jl_attn_scratch_bytes": (_SZ, [_VP]),
+    "jl_attn_prompt": (_I, [_VP, _VP, _I, _VP, _LL, _LL, _VP, _VP, _LL, _LL, _I, _VP, _I, _I, _I, _I, _I, C.c_float, _VP, _SZ, _VP]),
+    "jl_attn_paged": (_I, [_VP, _VP, _I, _VP, _LL, _LL, C.POINTER(PagedKVDesc), _VP, _VP, _I, _I, _I, C.c_float, _VP, _SZ, _VP]),
+    "jl_rope_append": (_I, [_VP, _VP, _VP, _I, C.POINTER(PagedKVDesc), _VP, _VP, _I, _I, _VP, _VP, _I, _VP]),
+    "jl_test_attn_share": (_I, [_VP, _VP] + [_I] * 10 + [_VP, _I]),
     "jl_decode_operand": (_VP, [_VP, _VP, _I]),
     "jl_matvec_dev_prepared": (_I, [_VP, _VP, _VP, _I, _VP]),
 }

@@ -1,0 +1,313 @@
+// Several sequences at once: attention over packed prompts, attention of new tokens over a cache in pages, and the cache's writer.
+// The entry points, the join of partial results and the writer; the attention kernels are in attn_few.cu and attn_tc5.cu.
+#include "attn.cuh"
+
+#include <math.h>
+
+// ------------------------------------------------------------------ join of partial results
+// Block (c, y) joins rows of the item that CTA c began and the CTAs behind it continued: the softmax weights of the parts are
+// 2^(their maximum - the largest), the parts added in ascending order of positions by each of `WAYS` groups of warps and the groups
+// in order. Bound by the parts' bytes, which come from L2.
+template <int ROWS, int D, int WAYS>
+__global__ void __launch_bounds__(256) attn_merge_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+    constexpr int LANES = D / 4, RPB = 256 / LANES / WAYS;        // rows at a time: a row is LANES threads times WAYS groups
+    __shared__ float4 sums[WAYS > 1 ? 256 : 1];
+    __shared__ float sl[WAYS > 1 ? 256 : 1];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int c = blockIdx.x;
+    const AttnMeta own = a.meta[c];
+    if (!own.own) return;
+    const int way = threadIdx.x / LANES % WAYS, lane = threadIdx.x % LANES, r = blockIdx.y * RPB + threadIdx.x / (LANES * WAYS);
+    int end = c + 1;                                              // the CTA that holds the item's last part
+    while (end < ctas - 1 && !(a.meta[end].cont && a.meta[end].ends)) end++;
+    const size_t slot = attn_slot_floats(ROWS, D);
+    const bool live = r < own.ntok * a.g;
+    float M = -INFINITY;
+    if (live)
+        for (int i = c; i <= end; ++i) {
+            if (i > c && !a.meta[i].cont) continue;
+            M = fmaxf(M, __ldcg(a.part + ((size_t)i * 2 + (i == c)) * slot + ROWS * D + r));
+        }
+    const float mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int n = end - c + 1, lo = c + (int)((long long)n * way / WAYS), hi = c + (int)((long long)n * (way + 1) / WAYS);
+    if (live)
+        for (int i = lo; i < hi; ++i) {
+            if (i > c && !a.meta[i].cont) continue;
+            const float *p = a.part + ((size_t)i * 2 + (i == c)) * slot;
+            const float w = exp2f(__ldcg(p + ROWS * D + r) - mu), l = __ldcg(p + ROWS * D + ROWS + r);
+            if (l == 0.f) continue;                               // the part holds nothing of this row, perhaps not even numbers
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + (size_t)r * D) + lane);
+            L = fmaf(w, l, L);
+            acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+        }
+    if constexpr (WAYS > 1) {
+        sums[threadIdx.x] = acc;
+        sl[threadIdx.x] = L;
+        __syncthreads();
+        if (way) return;
+#pragma unroll
+        for (int i = 1; i < WAYS; ++i) {
+            const float4 v = sums[threadIdx.x + i * LANES];
+            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+            L += sl[threadIdx.x + i * LANES];
+        }
+    }
+    if (!live) return;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    attn_store4(a.out, a.out_dtype, ((size_t)(own.row + r / a.g) * a.hq + own.head * a.g + r % a.g) * D + 4 * lane,
+                make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+}
+
+template <int ROWS, int D, int WAYS>
+static cudaError_t merge_go(const AttnArgs &a, int ctas, cudaStream_t s) {
+    constexpr int RPB = 256 / (D / 4) / WAYS;
+    return attn_launch_pdl(attn_merge_kernel<ROWS, D, WAYS>, dim3(ctas, (ROWS + RPB - 1) / RPB), dim3(256), 0, s, a, ctas);
+}
+
+int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s) {
+    (void)rows;
+    const cudaError_t e = a.d == 128 ? merge_go<ATTN_FEW_ROWS, 128, 4>(a, ctas, s) : merge_go<ATTN_FEW_ROWS, 64, 4>(a, ctas, s);
+    JL_CUDA(ctx, e);
+    ctx->st.launches++;
+    return JL_OK;
+}
+
+// ------------------------------------------------------------------ the cache's writer
+// Row r of qkv is a new token of the sequence it lies in; four consecutive values of it (two pairs) to a thread. Bound by bytes:
+// qkv is read once, q_out and the pages written once.
+__device__ __forceinline__ float4 attn_load4(const void *x, int dtype, size_t at) {
+    if (dtype == JL_DT_F32) return __ldcs(reinterpret_cast<const float4 *>(static_cast<const float *>(x) + at));
+    const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(x) + at));
+    if (dtype == JL_DT_BF16)
+        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
+                           __uint_as_float(w.y & 0xFFFF0000u));
+    const float2 p = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), q = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+    return make_float4(p.x, p.y, q.x, q.y);
+}
+
+struct AppendArgs {
+    void *q_out, *k, *v;
+    const void *qkv;
+    const int *starts, *lens, *table;
+    const float *cos_t, *sin_t;
+    long long kv_tok, kv_head, kv_page;
+    int nseq, total, hq, hkv, d, page_shift, n_pages, max_pages, max_pos, x_dtype, dtype;
+};
+
+__global__ void __launch_bounds__(256) attn_append_kernel(const __grid_constant__ AppendArgs a) {
+    __shared__ int sh[2];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int row = blockIdx.x;
+    if (threadIdx.x == 0) {
+        int lo = 0, hi = a.nseq;                       // the last sequence that starts at or before the row: among equal starts the
+        while (lo < hi) {                              // one that has rows
+            const int mid = (lo + hi) >> 1;
+            if (a.starts[mid + 1] <= row) lo = mid + 1; else hi = mid;
+        }
+        int page = -1, pos = -1;
+        if (lo < a.nseq && row >= a.starts[lo]) {
+            const long long p = (long long)a.lens[lo] - a.starts[lo + 1] + row;
+            if (p >= 0 && p < a.max_pos && p < ((long long)a.max_pages << a.page_shift)) {
+                pos = (int)p;
+                page = a.table[(long long)lo * a.max_pages + (pos >> a.page_shift)];
+                if ((unsigned)page >= (unsigned)a.n_pages) page = -1;
+            }
+        }
+        sh[0] = pos; sh[1] = page;
+    }
+    __syncthreads();
+    const int pos = sh[0], page = sh[1];
+    if (pos < 0) return;
+    const int heads = a.hq + 2 * a.hkv, quads = a.d / 4;
+    const long long at = page * a.kv_page + (pos & ((1 << a.page_shift) - 1)) * a.kv_tok;
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < heads * quads; i += gridDim.y * 256) {
+        const int hd = i / quads, j = i - hd * quads;
+        float4 v = attn_load4(a.qkv, a.x_dtype, ((size_t)row * heads + hd) * a.d + 4 * j);
+        if (hd < a.hq + a.hkv) {
+            const float2 c = __ldg(reinterpret_cast<const float2 *>(a.cos_t + (size_t)pos * (a.d / 2)) + j);
+            const float2 s = __ldg(reinterpret_cast<const float2 *>(a.sin_t + (size_t)pos * (a.d / 2)) + j);
+            v = make_float4(v.x * c.x - v.y * s.x, v.x * s.x + v.y * c.x, v.z * c.y - v.w * s.y, v.z * s.y + v.w * c.y);
+        }
+        if (hd < a.hq) {
+            attn_store4(a.q_out, a.dtype, ((size_t)row * a.hq + hd) * a.d + 4 * j, v);
+        } else if (page >= 0) {
+            const bool isk = hd < a.hq + a.hkv;
+            attn_store4(isk ? a.k : a.v, a.dtype, (size_t)(at + (long long)(hd - a.hq - (isk ? 0 : a.hkv)) * a.kv_head + 4 * j), v);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ C ABI
+namespace {
+// The caller's current device comes back however the call ends.
+struct DeviceGuard {
+    int was;
+    bool ok;
+    explicit DeviceGuard(int device) : was(-1), ok(false) {
+        if (cudaGetDevice(&was) != cudaSuccess) { cudaGetLastError(); was = -1; }
+        ok = was == device || cudaSetDevice(device) == cudaSuccess;
+        if (!ok) cudaGetLastError();
+    }
+    ~DeviceGuard() { if (was >= 0) cudaSetDevice(was); }
+};
+bool off16(const void *p) { return ((uintptr_t)p & 15u) != 0; }
+bool is16(int dtype) { return dtype == JL_DT_F16 || dtype == JL_DT_BF16; }
+
+// What both attention calls ask of their arguments; JL_OK, or the status with its reason.
+int check_common(jl_ctx *ctx, const char *name, const void *out, int out_dtype, const void *q, const void *k, const void *v, int dtype,
+                 long long q_tok, long long q_head, const void *starts, int nseq, int total, int hq, int hkv, int d, float scale,
+                 const void *scratch, size_t scratch_bytes) {
+    if (!out || !q || !k || !v || !starts || !scratch) return jl_set_err(ctx, JL_EINVAL, "%s: a pointer is NULL", name);
+    if (!is16(dtype)) return jl_set_err(ctx, JL_EINVAL, "%s: q, k and v are f16 or bf16", name);
+    if (out_dtype != JL_DT_F32 && !is16(out_dtype)) return jl_set_err(ctx, JL_EINVAL, "%s: out is f32, f16 or bf16", name);
+    if (nseq < 1 || total < 1 || hq < 1 || hkv < 1) return jl_set_err(ctx, JL_EINVAL, "%s: sizes below one", name);
+    if (hq % hkv || hq / hkv > 16) return jl_set_err(ctx, JL_ENOTSUP, "%s: %d query heads over %d kv heads (a multiple, up to 16)", name, hq, hkv);
+    if (d != 64 && d != 128) return jl_set_err(ctx, JL_ENOTSUP, "%s: head size %d (64 and 128 are served)", name, d);
+    if (!(scale > 0.f) || !(scale < INFINITY)) return jl_set_err(ctx, JL_EINVAL, "%s: the scale must be positive and finite", name);
+    if (total > (1 << 26) || hq > 1024 || nseq > (1 << 20)) return jl_set_err(ctx, JL_ENOTSUP, "%s: too many rows, heads or sequences", name);
+    if (off16(out) || off16(q) || off16(k) || off16(v) || off16(scratch) || ((uintptr_t)starts & 3))
+        return jl_set_err(ctx, JL_EINVAL, "%s: pointers must be 16-byte aligned (4 for the sequences' tables)", name);
+    if (q_tok < 0 || q_head < 0 || q_tok % 8 || q_head % 8 || q_tok >= (1ll << 31) || q_head >= (1ll << 31))
+        return jl_set_err(ctx, JL_EINVAL, "%s: strides of q must be multiples of 8 elements", name);
+    if (scratch_bytes < jl_attn_scratch_bytes(ctx)) return jl_set_err(ctx, JL_EINVAL, "%s: scratch of %zu bytes, jl_attn_scratch_bytes is %zu", name, scratch_bytes, jl_attn_scratch_bytes(ctx));
+    return JL_OK;
+}
+
+// A cache in pages: JL_OK, or the status with its reason. *shift: log2 of the page length.
+int check_pages(jl_ctx *ctx, const char *name, const jl_paged_kv *kv, jl_paged_kv *out, int *shift) {
+    if (!kv || kv->struct_size < sizeof(jl_paged_kv)) return jl_set_err(ctx, JL_EINVAL, "%s: a jl_paged_kv with its struct_size set", name);
+    *out = *kv;
+    if (!kv->k || !kv->v || !kv->page_table) return jl_set_err(ctx, JL_EINVAL, "%s: a pointer of the cache is NULL", name);
+    if (!is16(kv->dtype)) return jl_set_err(ctx, JL_EINVAL, "%s: the cache is f16 or bf16", name);
+    if (kv->n_kv < 1 || kv->n_pages < 1 || kv->n_seq < 1 || kv->max_pages < 1) return jl_set_err(ctx, JL_EINVAL, "%s: sizes below one", name);
+    int s = 0;
+    while (s < 11 && (1 << s) < kv->page_len) s++;
+    if (kv->page_len < 16 || kv->page_len > 1024 || (1 << s) != kv->page_len)
+        return jl_set_err(ctx, JL_ENOTSUP, "%s: pages of %d positions (powers of two from 16 to 1024 are served)", name, kv->page_len);
+    if (((long long)kv->max_pages << s) > (1ll << 30)) return jl_set_err(ctx, JL_ENOTSUP, "%s: more than 2^30 positions to a sequence", name);
+    if (off16(kv->k) || off16(kv->v) || ((uintptr_t)kv->page_table & 3)) return jl_set_err(ctx, JL_EINVAL, "%s: the pages must be 16-byte aligned", name);
+    *shift = s;
+    return JL_OK;
+}
+}  // namespace
+
+JL_EXPORT size_t jl_attn_scratch_bytes(jl_ctx *ctx) {
+    if (!ctx) return 0;
+    const int few = ctx->sm_count * ATTN_FEW_CTAS;
+    const size_t b = attn_meta_bytes(few) + (size_t)few * 2 * attn_slot_floats(ATTN_FEW_ROWS, 128) * sizeof(float);
+    return b;
+}
+
+JL_EXPORT int jl_attn_prompt(jl_ctx *ctx, void *out, int out_dtype, const void *q, long long q_tok_stride, long long q_head_stride,
+                             const void *k, const void *v, long long kv_tok_stride, long long kv_head_stride, int dtype,
+                             const int32_t *starts_dev, int nseq, int total, int hq, int hkv, int d, float scale, void *scratch,
+                             size_t scratch_bytes, void *stream) {
+    if (!ctx) return JL_EINVAL;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    int rc = check_common(ctx, "jl_attn_prompt", out, out_dtype, q, k, v, dtype, q_tok_stride, q_head_stride, starts_dev, nseq, total, hq,
+                          hkv, d, scale, scratch, scratch_bytes);
+    if (rc != JL_OK) return rc;
+    if (kv_tok_stride < 0 || kv_head_stride < 0 || kv_tok_stride % 8 || kv_head_stride % 8 || kv_tok_stride >= (1ll << 31) ||
+        kv_head_stride >= (1ll << 38))
+        return jl_set_err(ctx, JL_EINVAL, "jl_attn_prompt: strides of k and v must be multiples of 8 elements");
+    if (ctx->unhealthy) return jl_set_err(ctx, JL_ECUDA, "context is unhealthy after an earlier CUDA error");
+    DeviceGuard dg(ctx->device);
+    if (!dg.ok) return jl_set_err(ctx, JL_ECUDA, "jl_attn_prompt: the device cannot be made current");
+    AttnArgs a = {};
+    a.out = out; a.q = q; a.k = k; a.v = v; a.starts = starts_dev;
+    a.q_tok = q_tok_stride; a.q_head = q_head_stride; a.kv_tok = kv_tok_stride; a.kv_head = kv_head_stride;
+    a.nseq = nseq; a.total = total; a.hq = hq; a.hkv = hkv; a.g = hq / hkv; a.d = d;
+    a.out_dtype = out_dtype; a.scale_log2 = scale * 1.4426950408889634f; a.status = ctx->dev_status;
+    a.meta = static_cast<AttnMeta *>(scratch);
+    a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + attn_meta_bytes(ctx->sm_count * ATTN_FEW_CTAS));
+    rc = attn_launch_few(ctx, a, dtype, (cudaStream_t)stream);
+    if (rc == JL_OK) ctx->st.served++;
+    return rc;
+}
+
+JL_EXPORT int jl_attn_paged(jl_ctx *ctx, void *out, int out_dtype, const void *q, long long q_tok_stride, long long q_head_stride,
+                            const jl_paged_kv *kv, const int32_t *starts_dev, const int32_t *lens_dev, int total, int max_new, int hq,
+                            float scale, void *scratch, size_t scratch_bytes, void *stream) {
+    if (!ctx) return JL_EINVAL;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    jl_paged_kv c;
+    int shift = 0, rc = check_pages(ctx, "jl_attn_paged", kv, &c, &shift);
+    if (rc == JL_OK)
+        rc = check_common(ctx, "jl_attn_paged", out, out_dtype, q, c.k, c.v, c.dtype, q_tok_stride, q_head_stride, starts_dev, c.n_seq, total,
+                          hq, c.n_kv, c.head_dim, scale, scratch, scratch_bytes);
+    if (rc != JL_OK) return rc;
+    if (!lens_dev || ((uintptr_t)lens_dev & 3)) return jl_set_err(ctx, JL_EINVAL, "jl_attn_paged: the sequences' lengths are missing or misaligned");
+    if (max_new < 1) return jl_set_err(ctx, JL_EINVAL, "jl_attn_paged: max_new below one");
+    if (ctx->unhealthy) return jl_set_err(ctx, JL_ECUDA, "context is unhealthy after an earlier CUDA error");
+    DeviceGuard dg(ctx->device);
+    if (!dg.ok) return jl_set_err(ctx, JL_ECUDA, "jl_attn_paged: the device cannot be made current");
+    AttnArgs a = {};
+    a.out = out; a.q = q; a.k = c.k; a.v = c.v; a.starts = starts_dev; a.lens = lens_dev; a.table = c.page_table;
+    a.q_tok = q_tok_stride; a.q_head = q_head_stride;
+    a.kv_tok = c.head_dim; a.kv_head = (long long)c.page_len * c.head_dim; a.kv_page = a.kv_head * c.n_kv;
+    a.nseq = c.n_seq; a.total = total; a.hq = hq; a.hkv = c.n_kv; a.g = hq / c.n_kv; a.d = c.head_dim;
+    a.page_shift = shift; a.n_pages = c.n_pages; a.max_pages = c.max_pages;
+    a.out_dtype = out_dtype; a.scale_log2 = scale * 1.4426950408889634f; a.status = ctx->dev_status;
+    a.meta = static_cast<AttnMeta *>(scratch);
+    a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + attn_meta_bytes(ctx->sm_count * ATTN_FEW_CTAS));
+    rc = attn_launch_few(ctx, a, c.dtype, (cudaStream_t)stream);
+    if (rc == JL_OK) ctx->st.served++;
+    return rc;
+}
+
+JL_EXPORT int jl_rope_append(jl_ctx *ctx, void *q_out, const void *qkv, int x_dtype, const jl_paged_kv *kv, const int32_t *starts_dev,
+                             const int32_t *lens_dev, int total, int hq, const float *cos_t, const float *sin_t, int max_pos, void *stream) {
+    if (!ctx) return JL_EINVAL;
+    std::lock_guard<std::mutex> lk(ctx->mu);
+    jl_paged_kv c;
+    int shift = 0, rc = check_pages(ctx, "jl_rope_append", kv, &c, &shift);
+    if (rc != JL_OK) return rc;
+    if (!q_out || !qkv || !starts_dev || !lens_dev || !cos_t || !sin_t) return jl_set_err(ctx, JL_EINVAL, "jl_rope_append: a pointer is NULL");
+    if (x_dtype != JL_DT_F32 && !is16(x_dtype)) return jl_set_err(ctx, JL_EINVAL, "jl_rope_append: qkv is f32, f16 or bf16");
+    if (total < 1 || hq < 1 || max_pos < 1) return jl_set_err(ctx, JL_EINVAL, "jl_rope_append: sizes below one");
+    if (c.head_dim < 4 || c.head_dim > 1024 || c.head_dim % 4) return jl_set_err(ctx, JL_ENOTSUP, "jl_rope_append: head size %d (a multiple of 4)", c.head_dim);
+    if (total > (1 << 26) || hq > 1024 || c.n_kv > 1024) return jl_set_err(ctx, JL_ENOTSUP, "jl_rope_append: too many rows or heads");
+    if (off16(q_out) || off16(qkv) || off16(cos_t) || off16(sin_t) || ((uintptr_t)starts_dev & 3) || ((uintptr_t)lens_dev & 3))
+        return jl_set_err(ctx, JL_EINVAL, "jl_rope_append: pointers must be 16-byte aligned (4 for the sequences' tables)");
+    if (ctx->unhealthy) return jl_set_err(ctx, JL_ECUDA, "context is unhealthy after an earlier CUDA error");
+    DeviceGuard dg(ctx->device);
+    if (!dg.ok) return jl_set_err(ctx, JL_ECUDA, "jl_rope_append: the device cannot be made current");
+    AppendArgs a = {};
+    a.q_out = q_out; a.k = c.k; a.v = c.v; a.qkv = qkv; a.starts = starts_dev; a.lens = lens_dev; a.table = c.page_table;
+    a.cos_t = cos_t; a.sin_t = sin_t;
+    a.kv_tok = c.head_dim; a.kv_head = (long long)c.page_len * c.head_dim; a.kv_page = a.kv_head * c.n_kv;
+    a.nseq = c.n_seq; a.total = total; a.hq = hq; a.hkv = c.n_kv; a.d = c.head_dim; a.page_shift = shift; a.n_pages = c.n_pages;
+    a.max_pages = c.max_pages; a.max_pos = max_pos; a.x_dtype = x_dtype; a.dtype = c.dtype;
+    const cudaError_t e = attn_launch_pdl(attn_append_kernel, dim3(total, 1), dim3(256), 0, (cudaStream_t)stream, a);
+    JL_CUDA(ctx, e);
+    ctx->st.launches++;
+    ctx->st.served++;
+    return JL_OK;
+}
+
+// The division of the work as attn_share and AttnWalk make it, on the host: the segments of CTA `cta` as (sequence, block, head,
+// first unit, end unit, units of the item). Test-only.
+JL_EXPORT int jl_test_attn_share(const int32_t *starts, const int32_t *lens, int nseq, int total, int hkv, int tok_item, int unit_shift,
+                                 int min_units, int page_shift, int max_pages, int grid, int cta, int32_t *segs, int cap) {
+    if (!starts || !segs || nseq < 1 || hkv < 1 || tok_item < 1 || unit_shift < 1 || grid < 1 || cta < 0 || cta >= grid) return JL_EINVAL;
+    AttnArgs a = {};
+    a.starts = starts; a.lens = lens; a.nseq = nseq; a.total = total; a.hkv = hkv; a.tok_item = tok_item;
+    a.table = max_pages > 0 ? starts : nullptr;       // only its presence matters here
+    a.page_shift = page_shift; a.max_pages = max_pages;
+    AttnCut first, last;
+    attn_share_host(a, cta, grid, unit_shift, min_units, first, last);
+    AttnWalk w;
+    w.begin(first, last);
+    AttnSeg g;
+    int n = 0;
+    while (w.next(a, unit_shift, g)) {
+        if (n == cap) return -100;
+        int32_t *o = segs + 6 * n++;
+        o[0] = g.seq; o[1] = g.blk; o[2] = g.head; o[3] = g.u0; o[4] = g.u1; o[5] = g.units;
+    }
+    return n;
+}

@@ -1,0 +1,270 @@
+// Attention of several sequences at once: what the kernels of attn_few.cu (few query rows) and attn_tc5.cu (chunks and prompts)
+// share -- the sequences as the device sees them, the division of the work over the CTAs, and the record of a partial result.
+#pragma once
+
+#include "jl_internal.cuh"
+
+// One call. Positions of a sequence are numbered from its first cached one; its new rows are the last `n` of them.
+struct AttnMeta;
+struct AttnArgs {
+    void *out;
+    const void *q, *k, *v;
+    const int *starts;           // [nseq + 1]
+    const int *lens;             // [nseq]; NULL: a sequence is its new rows (packed prompts)
+    const int *table;            // [nseq][max_pages]; NULL: position p of sequence s is row starts[s] + p of k and v
+    AttnMeta *meta;              // scratch: one of each CTA, then
+    float *part;                 // its two partial results
+    int *status;                 // [0] code of a wait that ran out, [1] the limit in microseconds
+    long long q_tok, q_head;     // strides in elements; the innermost is 1
+    long long kv_tok, kv_head, kv_page;
+    int nseq, total, hq, hkv, g, d;
+    int page_shift, n_pages, max_pages;
+    int tok_item;                // tokens of one item
+    int out_dtype;
+    float scale_log2;            // scale * log2(e): softmax is taken to the base 2
+};
+
+struct AttnSeq { int row, n, len, pos0; };   // first row, new rows, positions readable, position of the first new row
+
+__host__ __device__ static inline AttnSeq attn_seq(const AttnArgs &a, int s) {
+    AttnSeq q;
+    int lo = a.starts[s], hi = a.starts[s + 1];
+    lo = lo < 0 ? 0 : (lo > a.total ? a.total : lo);
+    hi = hi < lo ? lo : (hi > a.total ? a.total : hi);
+    q.row = lo;
+    q.n = hi - lo;
+    int len = a.lens ? a.lens[s] : q.n;
+    if (len < 0) len = 0;
+    q.pos0 = len - q.n;                           // below zero where a sequence is shorter than its new rows: those see nothing
+    if (a.table) {
+        const long long cap = (long long)a.max_pages << a.page_shift;
+        if (len > cap) len = (int)cap;
+    }
+    q.len = len;
+    return q;
+}
+// Positions that the item of tokens [t0, t1) of a sequence walks: those of its last token.
+__host__ __device__ static inline int attn_limit(const AttnSeq &q, int t1) {
+    const int l = q.pos0 + t1;
+    return l < 0 ? 0 : (l > q.len ? q.len : l);
+}
+
+// The work is a line of items -- (sequence, block of tok_item tokens, kv head), heads innermost -- and item i is as long on it as
+// the positions that it walks plus ATTN_ITEM_COST * unit for its start and end. The line is cut into equal shares, one to a CTA,
+// the cuts rounded to whole units of positions inside an item; an item that a cut divides leaves a partial result in each CTA,
+// and attn_merge_kernel joins them in ascending order of positions. A few long sequences thus fill the GPU as well as many short
+// ones, whatever the lengths, which only the device knows; results depend on the cuts in their rounding and on nothing else.
+#define ATTN_ITEM_COST 1         // units
+#define ATTN_SNAP 2              // units: cuts nearer than this to an item's end move onto it, if the shares are long
+
+struct AttnCut { int seq, blk, head, unit; };     // before `unit` of item (seq, blk, head); seq == nseq: the line's end
+
+__host__ __device__ static inline long long attn_item_weight(const AttnSeq &q, int blk, int T, int cost) {
+    const int t1 = (blk + 1) * T < q.n ? (blk + 1) * T : q.n;
+    return (long long)cost + (q.pos0 > 0 ? q.pos0 : 0) + t1;
+}
+// Sum of the weights of blocks [0, i) of a sequence, i <= ceil(n / T); for one head.
+__host__ __device__ static inline long long attn_blocks_weight(const AttnSeq &q, int i, int T, int cost) {
+    if (i <= 0) return 0;
+    const long long base = (long long)i * (cost + (q.pos0 > 0 ? q.pos0 : 0));
+    const long long whole = (long long)T * i * (i + 1) / 2;
+    const long long over = (long long)i * T - q.n;           // of the last block, if it is the ragged one
+    return base + whole - (over > 0 ? over : 0);
+}
+__host__ __device__ static inline int attn_blocks(const AttnSeq &q, int T) { return (q.n + T - 1) / T; }
+
+// Where a cut at `x` (0 <= x < weight of the sequence times the heads) falls inside sequence s.
+__host__ __device__ static inline AttnCut attn_cut_in(const AttnArgs &a, int s, const AttnSeq &q, long long x, int unit_shift, int snap) {
+    const int T = a.tok_item, cost = ATTN_ITEM_COST << unit_shift;
+    int lo = 0, hi = attn_blocks(q, T) - 1;                  // the last block whose blocks in front weigh no more than x
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (attn_blocks_weight(q, mid, T, cost) * a.hkv <= x) lo = mid; else hi = mid - 1;
+    }
+    x -= attn_blocks_weight(q, lo, T, cost) * a.hkv;
+    const long long w = attn_item_weight(q, lo, T, cost);
+    AttnCut c;
+    c.seq = s; c.blk = lo; c.head = (int)(x / w);
+    x -= c.head * w;
+    const int t1 = (lo + 1) * T < q.n ? (lo + 1) * T : q.n;
+    const int units = (attn_limit(q, t1) + (1 << unit_shift) - 1) >> unit_shift;
+    long long u = (x - cost + (1 << (unit_shift - 1))) >> unit_shift;
+    u = u < 0 ? 0 : (u > units ? units : u);
+    if (u <= snap || units - u <= snap) u = 2 * u <= units ? 0 : units;      // a cut this near an item's end would leave a sliver
+    c.unit = (int)u;
+    return c;
+}
+
+// What each CTA left in scratch. A CTA has at most two partial results: slot 0 continues an item that a CTA in front began,
+// slot 1 begins an item that the next one continues.
+struct AttnMeta {
+    int cont, ends;              // slot 0 holds a part; the item of slot 0 ends in this CTA
+    int own;                     // slot 1 holds the first part of an item
+    int row, ntok, head;         // of that item: its first row, its tokens, its kv head
+};
+__host__ __device__ static inline size_t attn_meta_bytes(int ctas) { return ((size_t)ctas * sizeof(AttnMeta) + 255) & ~(size_t)255; }
+
+// A segment: units [u0, u1) of an item of `units`.
+struct AttnSeg { int seq, blk, head, u0, u1, units; AttnSeq q; };
+
+// Walks a CTA's share. first / last are its two cuts.
+struct AttnWalk {
+    AttnCut at, end;
+    AttnSeq q;
+    bool fresh;
+    __host__ __device__ void begin(const AttnCut &first, const AttnCut &last) { at = first; end = last; fresh = true; }
+    // The next segment that has work, or false.
+    __host__ __device__ bool next(const AttnArgs &a, int unit_shift, AttnSeg &g) {
+        for (;;) {
+            if (at.seq >= a.nseq) return false;
+            if (fresh) { q = attn_seq(a, at.seq); fresh = false; }
+            const int nblk = attn_blocks(q, a.tok_item);
+            if (at.blk >= nblk) {                            // past the sequence's last item, or a sequence without rows
+                if (at.seq >= end.seq) return false;
+                at.seq++; at.blk = at.head = at.unit = 0; fresh = true;
+                continue;
+            }
+            const bool last = at.seq == end.seq && at.blk == end.blk && at.head == end.head;
+            const int t1 = (at.blk + 1) * a.tok_item < q.n ? (at.blk + 1) * a.tok_item : q.n;
+            g.units = (attn_limit(q, t1) + (1 << unit_shift) - 1) >> unit_shift;
+            g.seq = at.seq; g.blk = at.blk; g.head = at.head; g.q = q;
+            g.u0 = at.unit;
+            g.u1 = last ? end.unit : g.units;
+            const bool some = g.u0 < g.u1 || (g.units == 0 && !last);
+            if (last) at.seq = a.nseq;                       // nothing after it
+            else {
+                at.unit = 0;
+                if (++at.head == a.hkv) { at.head = 0; at.blk++; }
+            }
+            if (some) return true;
+        }
+    }
+};
+
+__host__ __device__ static inline long long attn_seq_weight(const AttnArgs &a, const AttnSeq &q, int unit_shift) {
+    return attn_blocks_weight(q, attn_blocks(q, a.tok_item), a.tok_item, ATTN_ITEM_COST << unit_shift) * a.hkv;
+}
+// The shares of a line of `total`: how many there are (each min_units units at least), where share `cta` lies, and how near an item's
+// end a cut snaps onto it. False: the CTA has no share.
+__host__ __device__ static inline bool attn_cuts(long long total, int cta, int grid, int unit_shift, int min_units, long long &b0,
+                                                 long long &b1, int &snap) {
+    long long ctas = total / ((long long)min_units << unit_shift);
+    ctas = ctas < 1 ? 1 : (ctas > grid ? grid : ctas);
+    if (total == 0 || cta >= ctas) return false;
+    const long long share = total / ctas, rest = total % ctas;        // total * cta may pass 63 bits
+    b0 = share * cta + rest * cta / ctas;
+    b1 = share * (cta + 1) + rest * (cta + 1) / ctas;
+    const long long quarter = share >> (unit_shift + 2);
+    snap = quarter < ATTN_SNAP ? (int)quarter : ATTN_SNAP;
+    return true;
+}
+static inline void attn_share_host(const AttnArgs &a, int cta, int grid, int unit_shift, int min_units, AttnCut &first, AttnCut &last) {
+    long long total = 0, b0, b1, base = 0;
+    int snap;
+    for (int s = 0; s < a.nseq; ++s) total += attn_seq_weight(a, attn_seq(a, s), unit_shift);
+    first = last = AttnCut{a.nseq, 0, 0, 0};
+    if (!attn_cuts(total, cta, grid, unit_shift, min_units, b0, b1, snap)) return;
+    for (int s = 0; s < a.nseq; ++s) {
+        const AttnSeq q = attn_seq(a, s);
+        const long long w = attn_seq_weight(a, q, unit_shift);
+        if (b0 >= base && b0 < base + w) first = attn_cut_in(a, s, q, b0 - base, unit_shift, snap);
+        if (b1 >= base && b1 < base + w) last = attn_cut_in(a, s, q, b1 - base, unit_shift, snap);
+        base += w;
+    }
+}
+
+#ifdef __CUDACC__
+// The two cuts of CTA `cta` of `grid`, found by each warp; every lane returns them.
+__device__ static inline void attn_share(const AttnArgs &a, int cta, int grid, int unit_shift, int min_units,
+                                         AttnCut &first, AttnCut &last) {
+    const int lane = threadIdx.x & 31;
+    long long total = 0;
+    for (int s0 = 0; s0 < a.nseq; s0 += 32) {
+        long long w = s0 + lane < a.nseq ? attn_seq_weight(a, attn_seq(a, s0 + lane), unit_shift) : 0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        total += w;
+    }
+    first.seq = last.seq = a.nseq;
+    first.blk = first.head = first.unit = last.blk = last.head = last.unit = 0;
+    long long b0, b1;
+    int snap;
+    if (!attn_cuts(total, cta, grid, unit_shift, min_units, b0, b1, snap)) return;
+    long long base = 0;
+    for (int s0 = 0; s0 < a.nseq; s0 += 32) {
+        AttnSeq q = {0, 0, 0, 0};
+        long long w = 0;
+        if (s0 + lane < a.nseq) {
+            q = attn_seq(a, s0 + lane);
+            w = attn_seq_weight(a, q, unit_shift);
+        }
+        long long upto = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const long long from = base + upto - w;
+        base += __shfl_sync(0xffffffffu, upto, 31);
+        const unsigned m0 = __ballot_sync(0xffffffffu, b0 >= from && b0 < from + w);
+        const unsigned m1 = __ballot_sync(0xffffffffu, b1 >= from && b1 < from + w);
+        AttnCut c = {a.nseq, 0, 0, 0}, e = {a.nseq, 0, 0, 0};
+        if ((m0 >> lane) & 1) c = attn_cut_in(a, s0 + lane, q, b0 - from, unit_shift, snap);
+        if ((m1 >> lane) & 1) e = attn_cut_in(a, s0 + lane, q, b1 - from, unit_shift, snap);
+        if (m0) {
+            const int l = __ffs(m0) - 1;
+            first.seq = __shfl_sync(0xffffffffu, c.seq, l); first.blk = __shfl_sync(0xffffffffu, c.blk, l);
+            first.head = __shfl_sync(0xffffffffu, c.head, l); first.unit = __shfl_sync(0xffffffffu, c.unit, l);
+        }
+        if (m1) {
+            const int l = __ffs(m1) - 1;
+            last.seq = __shfl_sync(0xffffffffu, e.seq, l); last.blk = __shfl_sync(0xffffffffu, e.blk, l);
+            last.head = __shfl_sync(0xffffffffu, e.head, l); last.unit = __shfl_sync(0xffffffffu, e.unit, l);
+        }
+        if (base > b1) break;
+    }
+}
+
+// Two results as out_dtype, from row-major element offset `at` (even).
+__device__ __forceinline__ void attn_store2(void *out, int dtype, size_t at, float x, float y) {
+    if (dtype == JL_DT_F32) *reinterpret_cast<float2 *>(static_cast<float *>(out) + at) = make_float2(x, y);
+    else if (dtype == JL_DT_BF16) *reinterpret_cast<__nv_bfloat162 *>(static_cast<__nv_bfloat16 *>(out) + at) = __floats2bfloat162_rn(x, y);
+    else *reinterpret_cast<__half2 *>(static_cast<__half *>(out) + at) = __floats2half2_rn(x, y);
+}
+__device__ __forceinline__ void attn_store4(void *out, int dtype, size_t at, float4 v) {
+    if (dtype == JL_DT_F32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) = v;
+        return;
+    }
+    uint2 w;
+    if (dtype == JL_DT_BF16) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+        w = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    } else {
+        const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+        w = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(out) + at) = w;
+}
+#endif
+
+// A partial result in scratch: [rows][d] weighted sums of V, then [rows] maxima (base 2, scaled), then [rows] sums, all f32.
+__host__ __device__ static inline size_t attn_slot_floats(int rows, int d) { return (size_t)rows * (d + 2); }
+#define ATTN_FEW_ROWS 16
+#define ATTN_FEW_CTAS 3          // to an SM
+#define ATTN_TC_ROWS 256
+
+// Launched so that the next kernel of the stream may be put in place while this one drains.
+template <typename... P, typename... Args>
+static cudaError_t attn_launch_pdl(void (*kern)(P...), dim3 grid, dim3 block, int smem, cudaStream_t s, Args... args) {
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = s; cfg.attrs = at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
+}
+
+// attn_few.cu, attn.cu
+int attn_launch_few(jl_ctx *ctx, const AttnArgs &a, int dtype, cudaStream_t s);
+int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s);

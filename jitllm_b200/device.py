@@ -14,7 +14,7 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from ._lib import Choice, LayersBlock, LayersDesc, MoeDesc, Opts, Packed, Stats
+from ._lib import Choice, LayersBlock, LayersDesc, MoeDesc, Opts, Packed, PagedKVDesc, Stats
 
 
 class DeviceError(RuntimeError):
@@ -157,6 +157,30 @@ class Layers:
         self.handle, self._peers = 0, []
 
 
+class PagedKV:
+    """A key/value cache in pages that sequences of different lengths share: jl_paged_kv over torch tensors of the device.
+
+    k, v: [n_pages][n_kv][page_len][head_dim], f16 or bf16. table: int32 [n_seq][max_pages]; position p of sequence s lies in page
+    table[s][p // page_len]. The tensors stay the caller's: their contents may change between calls (a captured graph sees the change)."""
+
+    def __init__(self, k, v, table):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v must be alike: [n_pages][n_kv][page_len][head_dim]")
+        if table.dim() != 2 or not str(table.dtype).endswith("int32"):
+            raise ValueError("the page table must be int32 [n_seq][max_pages]")
+        if not (k.device == v.device == table.device) or k.device.type != "cuda":
+            raise ValueError("the cache and its table must lie on one GPU")
+        code = _dtype_code(k)
+        if code == _lib.DT_F32:
+            raise ValueError("the cache is f16 or bf16")
+        self.k, self.v, self.table = k, v, table
+        self.n_pages, self.n_kv, self.page_len, self.head_dim = k.shape
+        self.n_seq, self.max_pages = table.shape
+        self.desc = PagedKVDesc(struct_size=C.sizeof(PagedKVDesc), dtype=code, n_kv=self.n_kv, head_dim=self.head_dim,
+                                page_len=self.page_len, n_pages=self.n_pages, n_seq=self.n_seq, max_pages=self.max_pages, k=_ptr(k),
+                                v=_ptr(v), page_table=_ptr(table))
+
+
 class Device:
     """One B200, behind the reference's `nn.Device` surface."""
 
@@ -176,6 +200,7 @@ class Device:
             raise DeviceError(rc, "jl_open failed: no B200 (sm_100) visible as device %d; "
                                   "this path has no CPU fallback" % device)
         self.last_status = _lib.OK
+        self.ordinal = device
 
     # -- lifetime -----------------------------------------------------------
     def Close(self) -> None:
@@ -354,6 +379,98 @@ class Device:
     def MoeDev(self, out, h, logits, ntok: int, desc: MoeDesc, sel_out=None, wt_out=None, stream: int = 0) -> None:
         self._check(self.lib.jl_moe_dev(self.ctx, _ptr(out), _ptr(h), _dtype_code(h), _ptr(logits), ntok,
                                         C.byref(desc), _ptr(sel_out), _ptr(wt_out), stream))
+
+    # -- several sequences at once --------------------------------------------------
+    def AttnScratchBytes(self) -> int:
+        """Bytes of device memory that AttnPrompt and AttnPaged need as `scratch` (in any state; one for calls that may overlap)."""
+        return self.lib.jl_attn_scratch_bytes(self.ctx)
+
+    def AttnPrompt(self, out, q, k, v, starts, scratch, scale: float | None = None, stream: int = 0) -> None:
+        """Causal attention over packed prompts: sequence s is rows starts[s] .. starts[s + 1] - 1 (int32 device tensor [n_seq + 1]).
+        q [total][hq][d], k and v [total][hkv][d], f16 or bf16, views with any token and head stride; query head h reads kv head
+        h // (hq // hkv). out [total][hq][d], f32, f16 or bf16; rows behind the last sequence are left as they were. scale: None
+        for 1 / sqrt(d)."""
+        total, hq, d = self._heads("q", q)
+        if k.shape != v.shape or self._heads("k", k)[::2] != (total, d) or self._heads("v", v)[::2] != (total, d):
+            raise ValueError("q, k and v must be [total][heads][d] with one total and one d, k and v of one shape")
+        if self._strides(k) != self._strides(v):
+            raise ValueError("k and v must have the same strides")
+        if not q.dtype == k.dtype == v.dtype:
+            raise ValueError("q, k and v must be of one type")
+        self._seqs("starts", starts)
+        self._out(out, (total, hq, d))
+        self._on_device(out, q, k, v, starts, scratch)
+        if starts.numel() < 2 or total == 0:
+            return
+        self._check(self.lib.jl_attn_prompt(self.ctx, _ptr(out), _dtype_code(out), q.data_ptr(), *self._strides(q), k.data_ptr(),
+                                            v.data_ptr(), *self._strides(k), _dtype_code(q), _ptr(starts), starts.numel() - 1,
+                                            total, hq, k.shape[1], d, d ** -0.5 if scale is None else scale, _ptr(scratch),
+                                            _nbytes(scratch), stream))
+
+    def AttnPaged(self, out, q, kv: PagedKV, starts, lens, scratch, max_new: int | None = None, scale: float | None = None,
+                  stream: int = 0) -> None:
+        """Attention of each sequence's new rows over its pages, causal: new row i of the n that sequence s has sits at position
+        lens[s] - n + i (its key and value are in the cache already: RopeAppend). starts int32 [n_seq + 1] and lens int32 [n_seq] are
+        device tensors; q, out, scratch and scale as in AttnPrompt. max_new: the most new rows of any sequence, as far as the caller
+        knows; it picks the kernel, not the result (None: all rows may be one sequence's)."""
+        total, hq, d = self._heads("q", q)
+        if d != kv.head_dim or q.dtype != kv.k.dtype:
+            raise ValueError("q must have the cache's head size and type")
+        self._seqs("starts", starts, kv.n_seq + 1)
+        self._seqs("lens", lens, kv.n_seq)
+        self._out(out, (total, hq, d))
+        self._on_device(out, q, kv.k, starts, lens, scratch)
+        if kv.n_seq == 0 or total == 0:
+            return
+        self._check(self.lib.jl_attn_paged(self.ctx, _ptr(out), _dtype_code(out), q.data_ptr(), *self._strides(q), C.byref(kv.desc),
+                                           _ptr(starts), _ptr(lens), total, total if max_new is None else max_new, hq,
+                                           d ** -0.5 if scale is None else scale, _ptr(scratch), _nbytes(scratch), stream))
+
+    def RopeAppend(self, q_out, qkv, kv: PagedKV, starts, lens, cos, sin, stream: int = 0) -> None:
+        """The cache's writer: rows of qkv [total][(hq + 2 n_kv) * d] (f32, f16 or bf16) are the sequences' new rows, at the positions
+        that AttnPaged gives them. q_out [total][hq][d] of the cache's type gets q rotated; k (rotated) and v go to their pages.
+        cos, sin: f32 [positions][d / 2], adjacent-pair rotation. Rows at positions outside the tables are left out."""
+        total, hq, d = self._heads("q_out", q_out)
+        if d != kv.head_dim or q_out.dtype != kv.k.dtype or not q_out.is_contiguous():
+            raise ValueError("q_out must be contiguous and have the cache's head size and type")
+        if tuple(qkv.shape) != (total, (hq + 2 * kv.n_kv) * d):
+            raise ValueError("qkv must be [total][(hq + 2 n_kv) * d]")
+        for name, tab in (("cos", cos), ("sin", sin)):
+            if tab.dim() != 2 or tab.shape != cos.shape or tab.shape[1] * 2 != d or _dtype_code(tab) != _lib.DT_F32:
+                raise ValueError(f"{name} must be f32 [positions][d / 2]")
+        self._seqs("starts", starts, kv.n_seq + 1)
+        self._seqs("lens", lens, kv.n_seq)
+        self._on_device(q_out, qkv, kv.k, starts, lens, cos, sin)
+        if kv.n_seq == 0 or total == 0:
+            return
+        self._check(self.lib.jl_rope_append(self.ctx, _ptr(q_out), _ptr(qkv), _dtype_code(qkv), C.byref(kv.desc), _ptr(starts), _ptr(lens),
+                                            total, hq, _ptr(cos), _ptr(sin), cos.shape[0], stream))
+
+    @staticmethod
+    def _heads(name, t):
+        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+            raise ValueError(f"{name} must be [total][heads][d], contiguous in d")
+        return tuple(t.shape)
+
+    @staticmethod
+    def _strides(t):
+        """Token and head stride; those of a dimension of one are never used, whatever they say."""
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2], t.stride(1) if t.shape[1] > 1 else t.shape[2]
+
+    @staticmethod
+    def _out(out, shape):
+        if tuple(out.shape) != shape or not out.is_contiguous():
+            raise ValueError("out must be contiguous [total][hq][d]")
+
+    @staticmethod
+    def _seqs(name, t, n=None):
+        if t.dim() != 1 or not str(t.dtype).endswith("int32") or (n is not None and t.numel() != n):
+            raise ValueError(f"{name} must be a one-dimensional int32 tensor" + (f" of {n}" if n is not None else ""))
+
+    def _on_device(self, *tensors):
+        for t in tensors:
+            if t.device.type != "cuda" or t.device.index != self.ordinal:
+                raise ValueError(f"a tensor lies on {t.device}, this Device is GPU {self.ordinal}")
 
     def _check(self, rc: int) -> None:
         self.last_status = rc
