@@ -68,8 +68,8 @@ static cudaError_t merge_go(const AttnArgs &a, int ctas, cudaStream_t s) {
 }
 
 int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s) {
-    (void)rows;
-    const cudaError_t e = a.d == 128 ? merge_go<ATTN_FEW_ROWS, 128, 4>(a, ctas, s) : merge_go<ATTN_FEW_ROWS, 64, 4>(a, ctas, s);
+    const cudaError_t e = rows == ATTN_FEW_ROWS ? (a.d == 128 ? merge_go<ATTN_FEW_ROWS, 128, 4>(a, ctas, s) : merge_go<ATTN_FEW_ROWS, 64, 4>(a, ctas, s))
+                                                : (a.d == 128 ? merge_go<ATTN_TC_ROWS, 128, 1>(a, ctas, s) : merge_go<ATTN_TC_ROWS, 64, 1>(a, ctas, s));
     JL_CUDA(ctx, e);
     ctx->st.launches++;
     return JL_OK;
@@ -177,6 +177,15 @@ int check_common(jl_ctx *ctx, const char *name, const void *out, int out_dtype, 
     return JL_OK;
 }
 
+// Sequences of up to max_new new rows: one block of sixteen query rows to a kv head, or the tensor core's 256.
+int attn_launch(jl_ctx *ctx, const AttnArgs &a, int dtype, int max_new, cudaStream_t s) {
+    if ((long long)max_new * a.g > ATTN_FEW_ROWS) {
+        const int rc = attn_launch_tc5(ctx, a, dtype, s);
+        if (rc != JL_DECLINED) return rc;
+    }
+    return attn_launch_few(ctx, a, dtype, s);
+}
+
 // A cache in pages: JL_OK, or the status with its reason. *shift: log2 of the page length.
 int check_pages(jl_ctx *ctx, const char *name, const jl_paged_kv *kv, jl_paged_kv *out, int *shift) {
     if (!kv || kv->struct_size < sizeof(jl_paged_kv)) return jl_set_err(ctx, JL_EINVAL, "%s: a jl_paged_kv with its struct_size set", name);
@@ -198,8 +207,8 @@ int check_pages(jl_ctx *ctx, const char *name, const jl_paged_kv *kv, jl_paged_k
 JL_EXPORT size_t jl_attn_scratch_bytes(jl_ctx *ctx) {
     if (!ctx) return 0;
     const int few = ctx->sm_count * ATTN_FEW_CTAS;
-    const size_t b = attn_meta_bytes(few) + (size_t)few * 2 * attn_slot_floats(ATTN_FEW_ROWS, 128) * sizeof(float);
-    return b;
+    const size_t f = (size_t)few * 2 * attn_slot_floats(ATTN_FEW_ROWS, 128), t = (size_t)ctx->sm_count * 2 * attn_slot_floats(ATTN_TC_ROWS, 128);
+    return attn_meta_bytes(few) + (f > t ? f : t) * sizeof(float);
 }
 
 JL_EXPORT int jl_attn_prompt(jl_ctx *ctx, void *out, int out_dtype, const void *q, long long q_tok_stride, long long q_head_stride,
@@ -224,7 +233,7 @@ JL_EXPORT int jl_attn_prompt(jl_ctx *ctx, void *out, int out_dtype, const void *
     a.out_dtype = out_dtype; a.scale_log2 = scale * 1.4426950408889634f; a.status = ctx->dev_status;
     a.meta = static_cast<AttnMeta *>(scratch);
     a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + attn_meta_bytes(ctx->sm_count * ATTN_FEW_CTAS));
-    rc = attn_launch_few(ctx, a, dtype, (cudaStream_t)stream);
+    rc = attn_launch(ctx, a, dtype, total, (cudaStream_t)stream);
     if (rc == JL_OK) ctx->st.served++;
     return rc;
 }
@@ -254,7 +263,7 @@ JL_EXPORT int jl_attn_paged(jl_ctx *ctx, void *out, int out_dtype, const void *q
     a.out_dtype = out_dtype; a.scale_log2 = scale * 1.4426950408889634f; a.status = ctx->dev_status;
     a.meta = static_cast<AttnMeta *>(scratch);
     a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + attn_meta_bytes(ctx->sm_count * ATTN_FEW_CTAS));
-    rc = attn_launch_few(ctx, a, c.dtype, (cudaStream_t)stream);
+    rc = attn_launch(ctx, a, c.dtype, max_new, (cudaStream_t)stream);
     if (rc == JL_OK) ctx->st.served++;
     return rc;
 }

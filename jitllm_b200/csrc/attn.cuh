@@ -24,7 +24,8 @@ struct AttnArgs {
     float scale_log2;            // scale * log2(e): softmax is taken to the base 2
 };
 
-struct AttnSeq { int row, n, len, pos0; };   // first row, new rows, positions readable, position of the first new row
+// first row, new rows, positions readable, position of the first new row; longer than its table?
+struct AttnSeq { int row, n, len, pos0, over; };
 
 __host__ __device__ static inline AttnSeq attn_seq(const AttnArgs &a, int s) {
     AttnSeq q;
@@ -36,9 +37,10 @@ __host__ __device__ static inline AttnSeq attn_seq(const AttnArgs &a, int s) {
     int len = a.lens ? a.lens[s] : q.n;
     if (len < 0) len = 0;
     q.pos0 = len - q.n;                           // below zero where a sequence is shorter than its new rows: those see nothing
+    q.over = 0;
     if (a.table) {
         const long long cap = (long long)a.max_pages << a.page_shift;
-        if (len > cap) len = (int)cap;
+        if (len > cap) { len = (int)cap; q.over = 1; }
     }
     q.len = len;
     return q;
@@ -192,7 +194,7 @@ __device__ static inline void attn_share(const AttnArgs &a, int cta, int grid, i
     if (!attn_cuts(total, cta, grid, unit_shift, min_units, b0, b1, snap)) return;
     long long base = 0;
     for (int s0 = 0; s0 < a.nseq; s0 += 32) {
-        AttnSeq q = {0, 0, 0, 0};
+        AttnSeq q = {0, 0, 0, 0, 0};
         long long w = 0;
         if (s0 + lane < a.nseq) {
             q = attn_seq(a, s0 + lane);
@@ -265,6 +267,7 @@ static cudaError_t attn_launch_pdl(void (*kern)(P...), dim3 grid, dim3 block, in
     return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
 }
 
-// attn_few.cu, attn.cu
+// attn_few.cu, attn_tc5.cu, attn.cu
 int attn_launch_few(jl_ctx *ctx, const AttnArgs &a, int dtype, cudaStream_t s);
+int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &a, int dtype, cudaStream_t s);    // JL_DECLINED: no tensor map for these strides
 int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s);

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
                 const float4 v = *reinterpret_cast<const float4 *>(&red[w][r][4 * c]);
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
-            if (bad) L = __int_as_float(0x7fffffff);                // a page outside the pool: NaN
+            if (bad || sg.q.over) L = __int_as_float(0x7fffffff);   // a page outside the pool, positions outside the table: NaN
             if (whole) {
                 const int tk = r / a.g;
                 if (tk < ntok) {

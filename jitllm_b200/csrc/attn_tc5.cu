@@ -1,0 +1,577 @@
+// Attention for many query rows (chunks of new tokens, prompts) on tcgen05.
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale log2(e) q.k_j - m),  m a maximum of the exponents so far
+//
+// An item is 256 query rows of one kv head in two tiles of 128: (new token, query head of the group), token-major, so that grouped
+// heads share the tile's keys and a causal edge is 128 / g tokens wide. Per 128 positions a tile takes two 128 x 128 x d products
+// (tcgen05.mma, kind::f16: S = Q K^T out of shared memory, O += P V with P out of TMEM) and 128 x 128 exponentials: 1024 clocks each at
+// d = 128, so the two tiles alternate -- the tensor core works on one while the other's softmax runs.
+//
+// Roles of a CTA (one to an SM): two softmax warpgroups, one a tile (a thread owns a row: S comes to its registers, P goes back over
+// S's columns, 16 bits), an MMA warp, a TMA producer, and a warp that looks over the V tiles at a sequence's edge. K and V tiles of 128
+// positions come through one ring by TMA (a box to a page and 64 columns), Q once an item.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since it was last (P is then at most 2^8: no overflow, the
+// same relative rounding, and the sum of P carries the same factor); by the softmax warpgroup itself, which S's arrival tells that
+// the product before it is complete.
+#include "attn.cuh"
+#include "tc5.cuh"
+
+#define TA_UNIT_SHIFT 7
+#define TA_KV 128                        // positions of a unit
+#define TA_WARPS 12                      // 0-3, 4-7 softmax of tile 0, 1; 8 MMA; 9 producer; 10 edges; 11 only fills its warpgroup
+// Registers: launched with 168 a thread (384 threads: 64512); the softmax warpgroups, whose rows of S live in registers, go up by 40 a
+// thread (256 threads: 10240), the third goes down by 80 (128 threads: 10240).
+#define TA_REGS_SOFTMAX 208
+#define TA_REGS_OTHER 88
+#define TA_STATUS_CODE 7
+
+template <int D> struct TaSmem {
+    static constexpr int NH = D / 64;                         // 64-column halves: 128 bytes of a row, the swizzle's width
+    static constexpr int HALF = 128 * 128;                    // bytes of 128 rows of one
+    static constexpr int TILE = NH * HALF;
+    static constexpr int STAGES = D == 128 ? 5 : 10;
+    static constexpr int Q = 0, KV = 2 * TILE, BARS = KV + STAGES * TILE;
+    // barriers: kv_full[STAGES], kv_empty[STAGES], q_full, q_empty, s_full[2], p_full[2], o_full[2], drain, v_ok[OKS], e_full[OKS]
+    static constexpr int OKS = D == 128 ? 4 : 8;              // more than the V tiles that the ring can hold
+    static constexpr int NBARS = 2 * STAGES + 9 + 2 * OKS;
+    static constexpr int MISC = BARS + NBARS * 8;             // tmem address, abort flag and limit, seg_bad[4], seg_odd[4], cuts
+    static constexpr int TOTAL = MISC + 128 + 1024;           // 1024: the tiles start on a swizzle atom
+};
+
+// D[tmem] (+)= A[tmem] * B[smem desc].
+__device__ __forceinline__ void ta_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void ta_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+        "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void ta_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void ta_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ta_tma_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void ta_tma_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+                 : "memory");
+}
+// V tile as the B operand, N (the head's columns) contiguous: 64-column halves 16 KB apart, groups of 8 positions 1 KB apart.
+__device__ __forceinline__ uint64_t ta_desc_mn(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr >> 4) & 0x3FFF);
+    d |= (uint64_t)((128 * 128) >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__device__ __forceinline__ float ta_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF16> __device__ __forceinline__ uint32_t ta_pack(float x, float y) {
+    if constexpr (BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __half2 h = __floats2half2_rn(x, y);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+template <bool BF16> __device__ __forceinline__ float2 ta_unpack(uint32_t w) {
+    if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    else return __half22float2(*reinterpret_cast<const __half2 *>(&w));
+}
+// A packed pair with what is infinite or NaN in it set to zero.
+template <bool BF16> __device__ __forceinline__ uint32_t ta_finite(uint32_t w) {
+    constexpr uint32_t E = BF16 ? 0x7F80u : 0x7C00u;
+    if ((w & E) == E) w &= 0xFFFF0000u;
+    if ((w & (E << 16)) == (E << 16)) w &= 0x0000FFFFu;
+    return w;
+}
+
+// What the roles need of a segment.
+struct TaSeg {
+    int tok0, ntok;              // of the item
+    int e[2];                    // units of the segment that each tile walks
+    int edge;                    // units from this one on hold positions that some row of the item does not see, or the sequence's end
+};
+__device__ __forceinline__ TaSeg ta_seg(const AttnArgs &a, const AttnSeg &g) {
+    TaSeg t;
+    const int tq = a.tok_item >> 1;
+    t.tok0 = g.blk * a.tok_item;
+    t.ntok = min(a.tok_item, g.q.n - t.tok0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int first = t.tok0 + i * tq;
+        const int units = first < g.q.n ? (attn_limit(g.q, min(first + tq, g.q.n)) + TA_KV - 1) >> TA_UNIT_SHIFT : 0;
+        t.e[i] = max(0, min(units, g.u1) - g.u0);
+    }
+    t.edge = min(attn_limit(g.q, t.tok0 + 1), g.q.len) >> TA_UNIT_SHIFT;
+    return t;
+}
+
+template <int D, bool BF16, bool HILO>
+__global__ void __launch_bounds__(TA_WARPS * 32, 1)
+attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                const __grid_constant__ CUtensorMap vmap, int box_rows, int min_units) {
+    using L = TaSmem<D>;
+    extern __shared__ uint8_t raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
+    const uint32_t sbase = smem_u32(smem), bars = sbase + L::BARS;
+    const uint32_t kv_full = bars, kv_empty = bars + 8 * L::STAGES, q_full = bars + 16 * L::STAGES, q_empty = q_full + 8, s_full = q_full + 16,
+                   p_full = q_full + 32, o_full = q_full + 48, drain = q_full + 64, v_ok = q_full + 72, e_full = v_ok + 8 * L::OKS;
+    volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem + L::MISC);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::MISC + 4);        // [0] flag, [1] limit
+    volatile int *seg_bad = reinterpret_cast<volatile int *>(smem + L::MISC + 16), *seg_odd = seg_bad + 4;
+    const int warp = tc5_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int tq = a.tok_item >> 1;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::STAGES; ++s) { mbar_init(kv_full + 8 * s, 1); mbar_init(kv_empty + 8 * s, 1); }
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_full + 8 * i, 4);                   // one arrival a softmax warp
+            mbar_init(o_full + 8 * i, 1);
+        }
+        for (int i = 0; i < 2 * L::OKS; ++i) mbar_init(v_ok + 8 * i, 1);       // and e_full
+        mbar_init(drain, 1);
+        for (int i = 0; i < 4; ++i) seg_bad[i] = seg_odd[i] = 0;
+        abort_flag[0] = 0;
+        abort_flag[1] = a.status[1];
+        mbar_init_fence();
+    }
+    if (warp == 8) tc5_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), 512);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    AttnCut first, last;
+    attn_share(a, blockIdx.x, gridDim.x, TA_UNIT_SHIFT, min_units, first, last);
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    const uint32_t tmem = *tmem_slot;                       // S of the tiles at columns 0, 128; O at 256, 384
+    AttnWalk walk;
+    walk.begin(first, last);
+    AttnSeg g;
+    bool ok = true;
+#define TA_REGS(how, n) asm volatile("setmaxnreg." how ".sync.aligned.u32 %0;" ::"n"(n))
+
+    if (warp == 9) {
+        TA_REGS("dec", TA_REGS_OTHER);
+        // ------------------------------------------------ producer
+        uint32_t it = 0, segs = 0, edges = 0;               // tiles issued, segments with work, edge tiles of V
+        while (ok && walk.next(a, TA_UNIT_SHIFT, g)) {
+            const TaSeg t = ta_seg(a, g);
+            const int E = max(t.e[0], t.e[1]);
+            if (E == 0) continue;
+            if (segs) ok = __all_sync(0xffffffffu, tc5_wait(q_empty, (segs - 1) & 1, abort_flag));
+            if (!ok) break;
+            if (lane == 0) {
+                seg_bad[segs & 3] = g.q.over;
+                const int tiles = t.ntok > tq ? 2 : 1;      // of Q; boxes of g heads x tq tokens x 64 columns
+                mbar_arrive_expect_tx(q_full, tiles * L::NH * a.g * tq * 128);
+                for (int i = 0; i < tiles; ++i)
+                    for (int h = 0; h < L::NH; ++h)
+                        ta_tma_3d(sbase + L::Q + i * L::TILE + h * L::HALF, &qmap, h * 64, g.head * a.g, g.q.row + t.tok0 + i * tq, q_full);
+            }
+            __syncwarp();
+            // lane b * NH + h fetches box b (box_rows positions) of 64-column half h
+            const int box = lane / L::NH, half = lane % L::NH, nbox = TA_KV / box_rows;
+            auto page_of = [&](int u) -> int {
+                const int p = u * TA_KV + box * box_rows;
+                if (!a.table || box >= nbox || u >= g.u1 || p >= g.q.len) return 0;
+                return __ldg(a.table + (long long)g.seq * a.max_pages + (p >> a.page_shift));
+            };
+            int page = page_of(g.u0);
+            for (int u = g.u0; u < g.u0 + E && ok; ++u) {
+                const int p = u * TA_KV + box * box_rows;
+                const int boxes = min(nbox, (g.q.len - u * TA_KV + box_rows - 1) / box_rows);
+                const bool mine = box < boxes;
+                int y, z = page;
+                if (a.table) {
+                    y = p & ((1 << a.page_shift) - 1);
+                    if (mine && (unsigned)page >= (unsigned)a.n_pages) { z = a.n_pages; seg_bad[segs & 3] = 1; }   // out of the map: zeros
+                } else {
+                    y = g.q.row + p;
+                }
+                page = page_of(u + 1);
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv, ++it) {
+                    const uint32_t s = it % L::STAGES;
+                    if (it >= (uint32_t)L::STAGES)
+                        ok = __all_sync(0xffffffffu, tc5_wait(kv_empty + 8 * s, (it / L::STAGES + 1) & 1, abort_flag));
+                    if (!ok) break;
+                    // an edge tile of V lands on a barrier of its own, which the edge warp waits for: it sees no other tile, and a
+                    // stage's barrier would look to it as if a fill that it has not seen were the one it wants
+                    uint32_t full = kv_full + 8 * s;
+                    if (kv && u >= t.edge) {
+                        if (lane == 0) mbar_arrive(full);
+                        full = e_full + 8 * (edges++ % L::OKS);
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(full, boxes * L::NH * box_rows * 128);
+                    __syncwarp();
+                    if (mine)
+                        ta_tma_4d(sbase + L::KV + s * L::TILE + half * L::HALF + box * box_rows * 128, kv ? &vmap : &kmap, half * 64, y, g.head, z,
+                                  full);
+                }
+            }
+            segs++;
+        }
+        // a copy must not outlive its CTA: after a failed wait elsewhere those in flight are waited for here
+        if (*abort_flag) {
+            const uint64_t limit = tc5_limit_ns(abort_flag);
+            if (segs) mbar_wait_ns(q_full, (segs - 1) & 1, limit);
+            for (uint32_t i = it > (uint32_t)L::STAGES ? it - L::STAGES : 0; i < it; ++i)
+                mbar_wait_ns(kv_full + 8 * (i % L::STAGES), (i / L::STAGES) & 1, limit);
+            for (uint32_t i = edges > (uint32_t)L::OKS ? edges - L::OKS : 0; i < edges; ++i)
+                mbar_wait_ns(e_full + 8 * (i % L::OKS), (i / L::OKS) & 1, limit);
+        }
+    } else if (warp == 8) {
+        TA_REGS("dec", TA_REGS_OTHER);
+        // ------------------------------------------------ MMA
+        constexpr uint32_t type = BF16 ? (1u << 7) | (1u << 10) : 0u;
+        constexpr uint32_t id_s = tc5_idesc(128, 128) | type, id_o = tc5_idesc(128, D) | type | (1u << 16);   // V: N contiguous
+        const bool leader = tc5_elect();
+        uint32_t it = 0, segs = 0, done[2] = {0, 0}, edges = 0;      // tiles of the ring consumed, segments, P tiles consumed, edge tiles
+        while (ok && walk.next(a, TA_UNIT_SHIFT, g)) {
+            const TaSeg t = ta_seg(a, g);
+            const int E = max(t.e[0], t.e[1]);
+            if (E == 0) continue;
+            ok = __all_sync(0xffffffffu, tc5_wait(q_full, segs & 1, abort_flag)) &&
+                 __all_sync(0xffffffffu, tc5_wait(kv_full + 8 * (it % L::STAGES), (it / L::STAGES) & 1, abort_flag));
+            if (!ok) break;
+            tc5_fence_after();
+            auto scores = [&](int i, uint32_t stage) {               // S of tile i = Q K^T
+                const uint32_t q = sbase + L::Q + i * L::TILE, k = sbase + L::KV + stage * L::TILE;
+#pragma unroll
+                for (int x = 0; x < D / 16; ++x)
+                    tc5_mma_f16(tmem + i * 128, tc5_smem_desc(q + (x / 4) * L::HALF) + 2 * (x % 4), tc5_smem_desc(k + (x / 4) * L::HALF) + 2 * (x % 4),
+                                id_s, x != 0);
+                tc5_commit(s_full + 8 * i);
+            };
+            if (leader) {
+                for (int i = 0; i < 2; ++i)
+                    if (t.e[i] > 0) scores(i, it % L::STAGES);
+                tc5_commit(kv_empty + 8 * (it % L::STAGES));
+                if (E == 1) tc5_commit(q_empty);
+            }
+            it++;                                                    // now at V of unit 0
+            for (int j = 0; j < E && ok; ++j, it += 2) {
+                const uint32_t sv = it % L::STAGES, sk = (it + 1) % L::STAGES;
+                if (g.u0 + j >= t.edge) {
+                    ok = __all_sync(0xffffffffu, tc5_wait(v_ok + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag));
+                    edges++;
+                } else {
+                    ok = __all_sync(0xffffffffu, tc5_wait(kv_full + 8 * sv, (it / L::STAGES) & 1, abort_flag));
+                }
+                if (ok && j + 1 < E) ok = __all_sync(0xffffffffu, tc5_wait(kv_full + 8 * sk, ((it + 1) / L::STAGES) & 1, abort_flag));
+                for (int i = 0; i < 2 && ok; ++i) {
+                    if (j >= t.e[i]) continue;
+                    ok = __all_sync(0xffffffffu, tc5_wait(p_full + 8 * i, done[i] & 1, abort_flag));
+                    if (!ok) break;
+                    done[i]++;
+                    tc5_fence_after();
+                    if (leader) {
+                        const uint32_t v = sbase + L::KV + sv * L::TILE;
+#pragma unroll
+                        for (int x = 0; x < TA_KV / 16; ++x)
+                            ta_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * x, ta_desc_mn(v + x * 2048), id_o, j != 0 || x != 0);
+                        if constexpr (HILO) {
+#pragma unroll
+                            for (int x = 0; x < TA_KV / 16; ++x)
+                                ta_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + 64 + 8 * x, ta_desc_mn(v + x * 2048), id_o, 1);
+                        }
+                        if (j + 1 < t.e[i]) scores(i, sk);
+                        else tc5_commit(o_full + 8 * i);
+                    }
+                }
+                if (ok && leader) {
+                    tc5_commit(kv_empty + 8 * sv);
+                    if (j + 1 < E) tc5_commit(kv_empty + 8 * sk);
+                    if (j + 2 == E) tc5_commit(q_empty);
+                }
+            }
+            it--;                                                    // the last round counted a K tile that was not there
+            segs++;
+        }
+        if (leader) tc5_commit(drain);                               // nothing of the tensor core's is left when TMEM is given back
+        __syncwarp();
+        if (!mbar_wait_ns(drain, 0, tc5_limit_ns(abort_flag))) *abort_flag = 1;
+    } else if (warp == 10) {
+        TA_REGS("dec", TA_REGS_OTHER);
+        // ------------------------------------------------ edges
+        // V tiles at the edge of what the item's rows see. Positions behind the sequence's end become zeros (another sequence's rows,
+        // or what was in the stage before), and so does what is infinite or NaN: its weight is zero for the rows that do not see it,
+        // and 0 * inf is not. The rows that do see it get it back at the end (seg_odd).
+        uint32_t it = 0, segs = 0, edges = 0;
+        while (ok && walk.next(a, TA_UNIT_SHIFT, g)) {
+            const TaSeg t = ta_seg(a, g);
+            const int E = max(t.e[0], t.e[1]);
+            if (E == 0) continue;
+            if (lane == 0) seg_odd[segs & 3] = 0;
+            __syncwarp();
+            for (int j = 0; j < E && ok; ++j, it += 2) {
+                if (g.u0 + j < t.edge) continue;
+                const uint32_t s = (it + 1) % L::STAGES;
+                ok = __all_sync(0xffffffffu, tc5_wait(e_full + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag));
+                if (!ok) break;
+                const int rows = g.q.len - (g.u0 + j) * TA_KV;       // of the sequence
+                const uint32_t v = sbase + L::KV + s * L::TILE;
+                bool odd = false;
+#pragma unroll 2
+                for (int x = lane; x < L::NH * 128 * 8; x += 32) {   // 16-byte pieces, eight to a row of a half
+                    const uint32_t at = v + x * 16;
+                    uint32_t w[4] = {0, 0, 0, 0};
+                    bool write = true;
+                    if (((x >> 3) & 127) < rows) {
+                        uint32_t f[4];
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+                        write = false;
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            f[y] = ta_finite<BF16>(w[y]);
+                            write = write || f[y] != w[y];
+                            w[y] = f[y];
+                        }
+                        odd = odd || write;
+                    }
+                    if (write) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                }
+                if (odd) seg_odd[segs & 3] = 1;
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(v_ok + 8 * (edges % L::OKS));
+                edges++;
+            }
+            segs++;
+        }
+    } else if (warp == 11) {
+        TA_REGS("dec", TA_REGS_OTHER);
+    } else {
+        TA_REGS("inc", TA_REGS_SOFTMAX);
+        // ------------------------------------------------ softmax: warpgroup i owns tile i, a thread one of its rows
+        const int i = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // 32 lanes a warp, in bits 16 and up of a TMEM address
+        const uint32_t S = tmem + i * 128 + lanes, O = tmem + 256 + i * 128 + lanes;
+        const float c = a.scale_log2;
+        uint32_t tiles = 0, parts = 0, segs = 0;
+        AttnMeta meta = {0, 0, 0, 0, 0, 0};
+        while (ok && walk.next(a, TA_UNIT_SHIFT, g)) {
+            const TaSeg t = ta_seg(a, g);
+            const int tok = i * tq + r / a.g;                        // of the item
+            const bool live = r < tq * a.g && tok < t.ntok;
+            const int seen = attn_limit(g.q, t.tok0 + min(tok, t.ntok - 1) + 1);
+            const int all_seen = attn_limit(g.q, t.tok0 + i * tq + 1);      // by the tile's first token: below it nothing is masked
+            float m = -INFINITY, l = 0.f;                            // m: the maximum that O and l are scaled to (of S, unscaled)
+            const int E = t.e[i];
+            for (int j = 0; j < E; ++j, ++tiles) {
+                ok = tc5_wait(s_full + 8 * i, tiles & 1, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc5_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) tc5_ld32(S + 32 * x, s[x]);
+                tc5_wait_ld();
+                const int p0 = (g.u0 + j) * TA_KV;
+                if (p0 + TA_KV > all_seen) {
+                    const int n = seen - p0;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int y = 0; y < 32; ++y)
+                            if (32 * x + y >= n) s[x][y] = 0xFF800000u;
+                }
+                float mx[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    mx[x] = __uint_as_float(s[x][0]);
+#pragma unroll
+                    for (int y = 1; y < 32; ++y) mx[x] = fmaxf(mx[x], __uint_as_float(s[x][y]));
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool grow = top > m && (top - m) * c > 8.f;    // from -inf too
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float next = fmaxf(m, top);
+                    const float f = next == -INFINITY ? 1.f : ta_exp2((m - next) * c);
+                    m = next;
+                    l *= f;
+                    if (j > 0) {
+#pragma unroll
+                        for (int x = 0; x < D / 32; ++x) {
+                            uint32_t o[32];
+                            tc5_ld32(O + 32 * x, o);
+                            tc5_wait_ld();
+#pragma unroll
+                            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                            ta_st32(O + 32 * x, o);
+                        }
+                    }
+                }
+                const float mc = m == -INFINITY ? 0.f : -m * c;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t hi[16], lo[16];
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) {
+                        float u, w;
+                        tc5_fma2(u, w, __uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1]), c, mc);
+                        u = ta_exp2(u);
+                        w = ta_exp2(w);
+                        sum[y & 1] += u;
+                        sum[2 + (y & 1)] += w;
+                        hi[y] = ta_pack<BF16>(u, w);
+                        if constexpr (HILO) {
+                            const float2 b = ta_unpack<BF16>(hi[y]);
+                            lo[y] = ta_pack<BF16>(u - b.x, w - b.y);
+                        }
+                    }
+                    ta_st16(S + 16 * x, hi);
+                    if constexpr (HILO) ta_st16(S + 64 + 16 * x, lo);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                ta_wait_st();
+                tc5_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + 8 * i);
+            }
+            if (!ok) break;
+            const bool work = max(t.e[0], t.e[1]) > 0;
+            const bool whole = g.u0 == 0 && g.u1 == g.units;
+            bool odd = false;
+            if (E > 0) {
+                ok = __all_sync(0xffffffffu, tc5_wait(o_full + 8 * i, parts & 1, abort_flag));
+                if (!ok) break;
+                parts++;
+                tc5_fence_after();
+                if (seg_bad[segs & 3]) l = __int_as_float(0x7fffffff);
+                odd = seg_odd[segs & 3];
+            }
+            const int row = i * tq * a.g + r;                        // of the item
+            float *slot = nullptr;
+            if (!whole) {
+                const int which = g.u0 > 0 ? 0 : 1;
+                slot = a.part + ((size_t)blockIdx.x * 2 + which) * attn_slot_floats(ATTN_TC_ROWS, D);
+                if (which == 0) { meta.cont = 1; meta.ends = g.u1 == g.units; }
+                else { meta.own = 1; meta.row = g.q.row + t.tok0; meta.ntok = t.ntok; meta.head = g.head; }
+                if (live) {
+                    slot[ATTN_TC_ROWS * D + row] = m * c;
+                    slot[ATTN_TC_ROWS * D + ATTN_TC_ROWS + row] = l;
+                }
+            }
+            const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+            const size_t at = ((size_t)(g.q.row + t.tok0 + tok) * a.hq + g.head * a.g + r % a.g) * D;
+#pragma unroll 1
+            for (int x = 0; x < D / 32; ++x) {
+                uint32_t o[32];
+                if (E > 0) {
+                    tc5_ld32(O + 32 * x, o);
+                    tc5_wait_ld();
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 32; ++y) o[y] = 0u;
+                }
+                if (odd && live) {
+                    for (int p = max(g.u0, t.edge) * TA_KV; p < min(seen, (g.u0 + E) * TA_KV); ++p) {
+                        long long o0 = a.table ? 0 : (long long)(g.q.row + p) * a.kv_tok + g.head * a.kv_head;
+                        if (a.table) {
+                            const int page = __ldg(a.table + (long long)g.seq * a.max_pages + (p >> a.page_shift));
+                            if ((unsigned)page >= (unsigned)a.n_pages) continue;
+                            o0 = page * a.kv_page + g.head * a.kv_head + (p & ((1 << a.page_shift) - 1)) * a.kv_tok;
+                        }
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) {
+                            const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.v) + o0 + 32 * x) + y);
+                            if (ta_finite<BF16>(w) == w) continue;
+                            const float2 f = ta_unpack<BF16>(w);
+                            if (!isfinite(f.x)) o[2 * y] = __float_as_uint(__uint_as_float(o[2 * y]) + f.x);
+                            if (!isfinite(f.y)) o[2 * y + 1] = __float_as_uint(__uint_as_float(o[2 * y + 1]) + f.y);
+                        }
+                    }
+                }
+                if (!live) continue;
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                    const float4 v = make_float4(__uint_as_float(o[4 * y]) * inv, __uint_as_float(o[4 * y + 1]) * inv,
+                                                 __uint_as_float(o[4 * y + 2]) * inv, __uint_as_float(o[4 * y + 3]) * inv);
+                    if (whole) attn_store4(a.out, a.out_dtype, at + 32 * x + 4 * y, v);
+                    else if (E > 0) *reinterpret_cast<float4 *>(slot + (size_t)row * D + 32 * x + 4 * y) = v;
+                }
+            }
+            if (work) segs++;
+        }
+        if (threadIdx.x == 0) a.meta[blockIdx.x] = meta;
+    }
+    tc5_fence_before();
+    __syncthreads();
+    tc5_fence_after();
+    if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, TA_STATUS_CODE);
+    if (warp == 8) tc5_dealloc(tmem, 512);
+}
+
+static bool ta_map(CUtensorMap *map, const void *base, bool bf16, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
+    jl_encode_tiled_fn enc = jl_get_encode_tiled();
+    if (!enc) return false;
+    const cuuint32_t one[4] = {1, 1, 1, 1};
+    return enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, const_cast<void *>(base), dims, strides, box, one,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool BF16, bool HILO>
+static int ta_go(jl_ctx *ctx, const AttnArgs &a, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, int box_rows, cudaStream_t s) {
+    auto kern = attn_tc5_kernel<D, BF16, HILO>;
+    const int smem = TaSmem<D>::TOTAL, grid = ctx->sm_count;
+    JL_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const cudaError_t e = attn_launch_pdl(kern, dim3(grid), dim3(TA_WARPS * 32), smem, s, a, q, k, v, box_rows, 2);
+    JL_CUDA(ctx, e);
+    ctx->st.launches++;
+    return attn_launch_merge(ctx, a, ATTN_TC_ROWS, grid, s);
+}
+
+int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &args, int dtype, cudaStream_t s) {
+    AttnArgs a = args;
+    const int tq = 128 / a.g;
+    a.tok_item = 2 * tq;
+    const bool bf16 = dtype == JL_DT_BF16, hilo = a.out_dtype == JL_DT_F32;
+    CUtensorMap q, k, v;
+    const cuuint64_t d = a.d;
+    const cuuint64_t qd[3] = {d, (cuuint64_t)a.hq, (cuuint64_t)a.total}, qs[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_tok * 2};
+    const cuuint32_t qb[3] = {64, (cuuint32_t)a.g, (cuuint32_t)tq};
+    const int box_rows = a.table ? (a.page_shift < TA_UNIT_SHIFT ? 1 << a.page_shift : TA_KV) : TA_KV;
+    const cuuint64_t rows = a.table ? (cuuint64_t)1 << a.page_shift : (cuuint64_t)a.total, pages = a.table ? (cuuint64_t)a.n_pages : 1;
+    const cuuint64_t kd[4] = {d, rows, (cuuint64_t)a.hkv, pages};
+    const cuuint64_t ks[3] = {(cuuint64_t)a.kv_tok * 2, (cuuint64_t)a.kv_head * 2, a.table ? (cuuint64_t)a.kv_page * 2 : (cuuint64_t)a.kv_tok * 2};
+    const cuuint32_t kb[4] = {64, (cuuint32_t)box_rows, 1, 1};
+    if (!ta_map(&q, a.q, bf16, 3, qd, qs, qb) || !ta_map(&k, a.k, bf16, 4, kd, ks, kb) || !ta_map(&v, a.v, bf16, 4, kd, ks, kb))
+        return JL_DECLINED;
+#define TA_GO(D) (bf16 ? (hilo ? ta_go<D, true, true>(ctx, a, q, k, v, box_rows, s) : ta_go<D, true, false>(ctx, a, q, k, v, box_rows, s)) \
+                       : (hilo ? ta_go<D, false, true>(ctx, a, q, k, v, box_rows, s) : ta_go<D, false, false>(ctx, a, q, k, v, box_rows, s)))
+    return a.d == 128 ? TA_GO(128) : TA_GO(64);
+#undef TA_GO
+}
