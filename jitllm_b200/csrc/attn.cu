@@ -2,73 +2,103 @@
 // The entry points, the join of partial results and the writer; the attention kernels are in attn_few.cu and attn_tc5.cu.
 #include "attn.cuh"
 
+#include <limits.h>
 #include <math.h>
 
 // ------------------------------------------------------------------ join of partial results
 // Block (c, y) joins rows of the item that CTA c began and the CTAs behind it continued: the softmax weights of the parts are
-// 2^(their maximum - the largest), the parts added in ascending order of positions by each of `WAYS` groups of warps and the groups
-// in order. Bound by the parts' bytes, which come from L2.
+// 2^(their maximum - the largest), the parts added in ascending order of positions. Bound by the parts' bytes, which come from L2, and,
+// where a long sequence has few rows, by the loads' latency: WAYS warps share a row then, each a run of the parts, the runs added in
+// order (131,071 positions of two kv heads, 222 parts to a row: 150 us with one warp and one part at a time, 4 with eight).
 template <int ROWS, int D, int WAYS>
 __global__ void __launch_bounds__(256) attn_merge_kernel(const __grid_constant__ AttnArgs a, int ctas) {
-    constexpr int LANES = D / 4, RPB = 256 / LANES / WAYS;        // rows at a time: a row is LANES threads times WAYS groups
-    __shared__ float4 sums[WAYS > 1 ? 256 : 1];
-    __shared__ float sl[WAYS > 1 ? 256 : 1];
+    constexpr int RPB = 8 / WAYS, V = D / 32;                     // rows of a block; values of a lane
+    __shared__ float sums[8][D + 1];                              // a warp's weighted sums, and its sum of weights
+    __shared__ float tops[8];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int c = blockIdx.x;
+    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % WAYS;
     const AttnMeta own = a.meta[c];
     if (!own.own) return;
-    const int way = threadIdx.x / LANES % WAYS, lane = threadIdx.x % LANES, r = blockIdx.y * RPB + threadIdx.x / (LANES * WAYS);
+    const int r = blockIdx.y * RPB + warp / WAYS;
+    if (blockIdx.y * RPB >= own.ntok * a.g) return;
     int end = c + 1;                                              // the CTA that holds the item's last part
-    while (end < ctas - 1 && !(a.meta[end].cont && a.meta[end].ends)) end++;
+    for (;; end += 32) {
+        const int i = min(end + lane, ctas - 1);
+        const unsigned m = __ballot_sync(0xffffffffu, i == ctas - 1 || (a.meta[i].cont && a.meta[i].ends));
+        if (m) { end = min(end + __ffs(m) - 1, ctas - 1); break; }
+    }
     const size_t slot = attn_slot_floats(ROWS, D);
     const bool live = r < own.ntok * a.g;
+    const int n = end - c + 1, lo = c + n * way / WAYS, hi = c + n * (way + 1) / WAYS;
+    // part i of the row: its maximum (none: no weight)
+    auto top_of = [&](int i) { return i > c && !a.meta[i].cont ? -INFINITY : __ldcg(a.part + ((size_t)i * 2 + (i == c)) * slot + ROWS * D + r); };
     float M = -INFINITY;
     if (live)
-        for (int i = c; i <= end; ++i) {
-            if (i > c && !a.meta[i].cont) continue;
-            M = fmaxf(M, __ldcg(a.part + ((size_t)i * 2 + (i == c)) * slot + ROWS * D + r));
-        }
+        for (int i = lo + lane; i < hi; i += 32) M = fmaxf(M, top_of(i));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if constexpr (WAYS > 1) {
+        if (lane == 0) tops[warp] = M;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAYS; ++i) M = fmaxf(M, tops[warp - way + i]);
+    }
     const float mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int n = end - c + 1, lo = c + (int)((long long)n * way / WAYS), hi = c + (int)((long long)n * (way + 1) / WAYS);
+    float L = 0.f, acc[V];
+#pragma unroll
+    for (int x = 0; x < V; ++x) acc[x] = 0.f;
     if (live)
-        for (int i = lo; i < hi; ++i) {
-            if (i > c && !a.meta[i].cont) continue;
-            const float *p = a.part + ((size_t)i * 2 + (i == c)) * slot;
-            const float w = exp2f(__ldcg(p + ROWS * D + r) - mu), l = __ldcg(p + ROWS * D + ROWS + r);
-            if (l == 0.f) continue;                               // the part holds nothing of this row, perhaps not even numbers
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + (size_t)r * D) + lane);
-            L = fmaf(w, l, L);
-            acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
+        for (int i0 = lo; i0 < hi; i0 += 32) {
+            float w = 0.f, l = 0.f;                               // of part i0 + lane
+            if (i0 + lane < hi) {
+                w = exp2f(top_of(i0 + lane) - mu);
+                l = i0 + lane > c && !a.meta[i0 + lane].cont ? 0.f : __ldcg(a.part + ((size_t)(i0 + lane) * 2 + (i0 + lane == c)) * slot + ROWS * D + ROWS + r);
+            }
+            const int cnt = min(32, hi - i0);
+#pragma unroll 8
+            for (int k = 0; k < cnt; ++k) {
+                const float wk = __shfl_sync(0xffffffffu, w, k), lk = __shfl_sync(0xffffffffu, l, k);
+                if (lk == 0.f) continue;                          // the part holds nothing of this row, perhaps not even numbers
+                const float *p = a.part + ((size_t)(i0 + k) * 2 + (i0 + k == c)) * slot + (size_t)r * D + V * lane;
+                L = fmaf(wk, lk, L);
+                if constexpr (V == 4) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(p));
+                    acc[0] = fmaf(wk, v.x, acc[0]); acc[1] = fmaf(wk, v.y, acc[1]); acc[2] = fmaf(wk, v.z, acc[2]); acc[3] = fmaf(wk, v.w, acc[3]);
+                } else {
+                    const float2 v = __ldcg(reinterpret_cast<const float2 *>(p));
+                    acc[0] = fmaf(wk, v.x, acc[0]); acc[1] = fmaf(wk, v.y, acc[1]);
+                }
+            }
         }
     if constexpr (WAYS > 1) {
-        sums[threadIdx.x] = acc;
-        sl[threadIdx.x] = L;
+#pragma unroll
+        for (int x = 0; x < V; ++x) sums[warp][V * lane + x] = acc[x];
+        if (lane == 0) sums[warp][D] = L;
         __syncthreads();
         if (way) return;
 #pragma unroll
         for (int i = 1; i < WAYS; ++i) {
-            const float4 v = sums[threadIdx.x + i * LANES];
-            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-            L += sl[threadIdx.x + i * LANES];
+#pragma unroll
+            for (int x = 0; x < V; ++x) acc[x] += sums[warp + i][V * lane + x];
+            L += sums[warp + i][D];
         }
     }
     if (!live) return;
     const float inv = L == 0.f ? 0.f : 1.f / L;
-    attn_store4(a.out, a.out_dtype, ((size_t)(own.row + r / a.g) * a.hq + own.head * a.g + r % a.g) * D + 4 * lane,
-                make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    const size_t at = ((size_t)(own.row + r / a.g) * a.hq + own.head * a.g + r % a.g) * D + V * lane;
+    if constexpr (V == 4) attn_store4(a.out, a.out_dtype, at, make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv));
+    else attn_store2(a.out, a.out_dtype, at, acc[0] * inv, acc[1] * inv);
 }
 
 template <int ROWS, int D, int WAYS>
 static cudaError_t merge_go(const AttnArgs &a, int ctas, cudaStream_t s) {
-    constexpr int RPB = 256 / (D / 4) / WAYS;
+    constexpr int RPB = 8 / WAYS;
     return attn_launch_pdl(attn_merge_kernel<ROWS, D, WAYS>, dim3(ctas, (ROWS + RPB - 1) / RPB), dim3(256), 0, s, a, ctas);
 }
 
 int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s) {
-    const cudaError_t e = rows == ATTN_FEW_ROWS ? (a.d == 128 ? merge_go<ATTN_FEW_ROWS, 128, 4>(a, ctas, s) : merge_go<ATTN_FEW_ROWS, 64, 4>(a, ctas, s))
+    const cudaError_t e = rows == ATTN_FEW_ROWS ? (a.d == 128 ? merge_go<ATTN_FEW_ROWS, 128, 8>(a, ctas, s) : merge_go<ATTN_FEW_ROWS, 64, 8>(a, ctas, s))
                                                 : (a.d == 128 ? merge_go<ATTN_TC_ROWS, 128, 1>(a, ctas, s) : merge_go<ATTN_TC_ROWS, 64, 1>(a, ctas, s));
     JL_CUDA(ctx, e);
     ctx->st.launches++;
@@ -177,13 +207,22 @@ int check_common(jl_ctx *ctx, const char *name, const void *out, int out_dtype, 
     return JL_OK;
 }
 
-// Sequences of up to max_new new rows: one block of sixteen query rows to a kv head, or the tensor core's 256.
-int attn_launch(jl_ctx *ctx, const AttnArgs &a, int dtype, int max_new, cudaStream_t s) {
-    if ((long long)max_new * a.g > ATTN_FEW_ROWS) {
-        const int rc = attn_launch_tc5(ctx, a, dtype, s);
-        if (rc != JL_DECLINED) return rc;
+// Sequences of up to max_new new rows: those of at most sixteen query rows to a kv head go to the kernel that takes sixteen, the others
+// to the tensor core's 256. A launch that finds no sequence of its own costs about 4 us: there are two only where `mixed` says that both
+// kinds are likely.
+int attn_launch(jl_ctx *ctx, AttnArgs a, int dtype, long long max_new, bool mixed, cudaStream_t s) {
+    a.row_lo = 0;
+    a.row_hi = INT_MAX;
+    if (max_new * a.g <= ATTN_FEW_ROWS) return attn_launch_few(ctx, a, dtype, s);
+    if (mixed) {
+        a.row_hi = ATTN_FEW_ROWS;
+        const int rc = attn_launch_few(ctx, a, dtype, s);
+        if (rc != JL_OK) return rc;
+        a.row_lo = a.row_hi;
+        a.row_hi = INT_MAX;
     }
-    return attn_launch_few(ctx, a, dtype, s);
+    const int rc = attn_launch_tc5(ctx, a, dtype, s);
+    return rc == JL_DECLINED ? attn_launch_few(ctx, a, dtype, s) : rc;
 }
 
 // A cache in pages: JL_OK, or the status with its reason. *shift: log2 of the page length.
@@ -233,7 +272,7 @@ JL_EXPORT int jl_attn_prompt(jl_ctx *ctx, void *out, int out_dtype, const void *
     a.out_dtype = out_dtype; a.scale_log2 = scale * 1.4426950408889634f; a.status = ctx->dev_status;
     a.meta = static_cast<AttnMeta *>(scratch);
     a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + attn_meta_bytes(ctx->sm_count * ATTN_FEW_CTAS));
-    rc = attn_launch(ctx, a, dtype, total, (cudaStream_t)stream);
+    rc = attn_launch(ctx, a, dtype, total, false, (cudaStream_t)stream);
     if (rc == JL_OK) ctx->st.served++;
     return rc;
 }
@@ -263,7 +302,7 @@ JL_EXPORT int jl_attn_paged(jl_ctx *ctx, void *out, int out_dtype, const void *q
     a.out_dtype = out_dtype; a.scale_log2 = scale * 1.4426950408889634f; a.status = ctx->dev_status;
     a.meta = static_cast<AttnMeta *>(scratch);
     a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + attn_meta_bytes(ctx->sm_count * ATTN_FEW_CTAS));
-    rc = attn_launch(ctx, a, c.dtype, max_new, (cudaStream_t)stream);
+    rc = attn_launch(ctx, a, c.dtype, max_new, c.n_seq > 1 && total < (long long)max_new * c.n_seq, (cudaStream_t)stream);
     if (rc == JL_OK) ctx->st.served++;
     return rc;
 }
@@ -307,6 +346,7 @@ JL_EXPORT int jl_test_attn_share(const int32_t *starts, const int32_t *lens, int
     a.starts = starts; a.lens = lens; a.nseq = nseq; a.total = total; a.hkv = hkv; a.tok_item = tok_item;
     a.table = max_pages > 0 ? starts : nullptr;       // only its presence matters here
     a.page_shift = page_shift; a.max_pages = max_pages;
+    a.g = 1; a.row_hi = INT_MAX;
     AttnCut first, last;
     attn_share_host(a, cta, grid, unit_shift, min_units, first, last);
     AttnWalk w;

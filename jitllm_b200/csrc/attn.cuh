@@ -19,6 +19,7 @@ struct AttnArgs {
     long long kv_tok, kv_head, kv_page;
     int nseq, total, hq, hkv, g, d;
     int page_shift, n_pages, max_pages;
+    int row_lo, row_hi;          // the launch takes the sequences with row_lo < new rows * g <= row_hi
     int tok_item;                // tokens of one item
     int out_dtype;
     float scale_log2;            // scale * log2(e): softmax is taken to the base 2
@@ -43,6 +44,8 @@ __host__ __device__ static inline AttnSeq attn_seq(const AttnArgs &a, int s) {
         if (len > cap) { len = (int)cap; q.over = 1; }
     }
     q.len = len;
+    const long long rows = (long long)q.n * a.g;
+    if (rows <= a.row_lo || rows > a.row_hi) q.n = 0;
     return q;
 }
 // Positions that the item of tokens [t0, t1) of a sequence walks: those of its last token.

@@ -19,25 +19,13 @@
 
 #define TA_UNIT_SHIFT 7
 #define TA_KV 128                        // positions of a unit
-#define TA_WARPS 12                      // 0-3, 4-7 softmax of tile 0, 1; 8 MMA; 9 producer; 10 edges; 11 only fills its warpgroup
+#define TA_WARPS 12                      // 0-3, 4-7 softmax of tile 0, 1; 8 MMA; 9 producer; 10 edges; 11 the walk
 // Registers: launched with 168 a thread (384 threads: 64512); the softmax warpgroups, whose rows of S live in registers, go up by 40 a
 // thread (256 threads: 10240), the third goes down by 80 (128 threads: 10240).
 #define TA_REGS_SOFTMAX 208
 #define TA_REGS_OTHER 88
 #define TA_STATUS_CODE 7
 
-template <int D> struct TaSmem {
-    static constexpr int NH = D / 64;                         // 64-column halves: 128 bytes of a row, the swizzle's width
-    static constexpr int HALF = 128 * 128;                    // bytes of 128 rows of one
-    static constexpr int TILE = NH * HALF;
-    static constexpr int STAGES = D == 128 ? 5 : 10;
-    static constexpr int Q = 0, KV = 2 * TILE, BARS = KV + STAGES * TILE;
-    // barriers: kv_full[STAGES], kv_empty[STAGES], q_full, q_empty, s_full[2], p_full[2], o_full[2], drain, v_ok[OKS], e_full[OKS]
-    static constexpr int OKS = D == 128 ? 4 : 8;              // more than the V tiles that the ring can hold
-    static constexpr int NBARS = 2 * STAGES + 9 + 2 * OKS;
-    static constexpr int MISC = BARS + NBARS * 8;             // tmem address, abort flag and limit, seg_bad[4], seg_odd[4], cuts
-    static constexpr int TOTAL = MISC + 128 + 1024;           // 1024: the tiles start on a swizzle atom
-};
 
 // D[tmem] (+)= A[tmem] * B[smem desc].
 __device__ __forceinline__ void ta_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -87,6 +75,21 @@ __device__ __forceinline__ uint64_t ta_desc_mn(uint32_t smem_addr) {
     d |= (uint64_t)2 << 61;
     return d;
 }
+__device__ __forceinline__ float ta_max3(float x, float y, float z) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+    return m;
+}
+// d += x on both halves.
+__device__ __forceinline__ void ta_add2(float (&d)[2], float x, float y) {
+    asm("{\n\t.reg .b64 rd, rx;\n\t"
+        "mov.b64 rd, {%0, %1};\n\t"
+        "mov.b64 rx, {%2, %3};\n\t"
+        "add.rn.f32x2 rd, rd, rx;\n\t"
+        "mov.b64 {%0, %1}, rd;\n\t}"
+        : "+f"(d[0]), "+f"(d[1])
+        : "f"(x), "f"(y));
+}
 __device__ __forceinline__ float ta_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -113,25 +116,76 @@ template <bool BF16> __device__ __forceinline__ uint32_t ta_finite(uint32_t w) {
     return w;
 }
 
-// What the roles need of a segment.
-struct TaSeg {
-    int tok0, ntok;              // of the item
+// What the roles need of a segment. One warp walks the CTA's share and hands the segments out through a ring in shared memory: a row of S
+// fills most of a softmax thread's registers, and a walk of its own would spill the rest.
+struct __align__(16) TaSeg {
+    int seq, head;               // seq < 0: the share's end
+    int u0, u1, whole;           // units; is this all of the item?
+    int ends;                    // the item ends here
+    int tok0, ntok;              // of the item, in the sequence
     int e[2];                    // units of the segment that each tile walks
     int edge;                    // units from this one on hold positions that some row of the item does not see, or the sequence's end
+    int row, n, len, pos0, over; // of the sequence
 };
-__device__ __forceinline__ TaSeg ta_seg(const AttnArgs &a, const AttnSeg &g) {
-    TaSeg t;
-    const int tq = a.tok_item >> 1;
-    t.tok0 = g.blk * a.tok_item;
-    t.ntok = min(a.tok_item, g.q.n - t.tok0);
+#define TA_SEGS 4
+#define TA_SEG_USERS 11          // warps that read it
+__device__ __forceinline__ void ta_seg(const AttnArgs &a, const AttnSeg &g, volatile TaSeg *t) {
+    const int tq = a.tok_item >> 1, tok0 = g.blk * a.tok_item;
+    t->seq = g.seq; t->head = g.head; t->u0 = g.u0; t->u1 = g.u1;
+    t->whole = g.u0 == 0 && g.u1 == g.units;
+    t->ends = g.u1 == g.units;
+    t->tok0 = tok0;
+    t->ntok = min(a.tok_item, g.q.n - tok0);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int first = t.tok0 + i * tq;
+        const int first = tok0 + i * tq;
         const int units = first < g.q.n ? (attn_limit(g.q, min(first + tq, g.q.n)) + TA_KV - 1) >> TA_UNIT_SHIFT : 0;
-        t.e[i] = max(0, min(units, g.u1) - g.u0);
+        t->e[i] = max(0, min(units, g.u1) - g.u0);
     }
-    t.edge = min(attn_limit(g.q, t.tok0 + 1), g.q.len) >> TA_UNIT_SHIFT;
-    return t;
+    t->edge = min(attn_limit(g.q, tok0 + 1), g.q.len) >> TA_UNIT_SHIFT;
+    t->row = g.q.row; t->n = g.q.n; t->len = g.q.len; t->pos0 = g.q.pos0; t->over = g.q.over;
+}
+__device__ __forceinline__ int ta_seen(const volatile TaSeg *t, int tok1) {          // attn_limit
+    return max(0, min(t->pos0 + tok1, t->len));
+}
+
+template <int D> struct TaSmem {
+    static constexpr int NH = D / 64;                         // 64-column halves: 128 bytes of a row, the swizzle's width
+    static constexpr int HALF = 128 * 128;                    // bytes of 128 rows of one
+    static constexpr int TILE = NH * HALF;
+    static constexpr int STAGES = D == 128 ? 4 : 8;
+    static constexpr int Q = 0, KV = 2 * TILE, OUT = KV + STAGES * TILE, BARS = OUT + 8 * 4096;      // OUT: a softmax warp's 32 rows of 128 bytes
+    // barriers: kv_full[STAGES], kv_empty[STAGES], q_full, q_empty, s_full[2], p_full[2], o_full[2], drain, v_ok[OKS], e_full[OKS], g_full[TA_SEGS], g_empty[TA_SEGS]
+    static constexpr int OKS = D == 128 ? 4 : 8;              // more than the V tiles that the ring can hold
+    static constexpr int NBARS = 2 * STAGES + 9 + 2 * OKS + 2 * TA_SEGS;
+    static constexpr int SEGS = (BARS + NBARS * 8 + 15) & ~15;
+    static constexpr int MISC = SEGS + TA_SEGS * (int)sizeof(TaSeg);      // tmem address, abort flag and limit, seg_bad[4], seg_odd[4]
+    static constexpr int TOTAL = MISC + 64 + 1024;           // 1024: the tiles start on a swizzle atom
+};
+
+// Columns c0 .. c0 + 31 of a row's sum get back what the edge warp took out of positions [p0, p1), which the row sees.
+template <bool BF16>
+__device__ __forceinline__ void ta_odd(const AttnArgs &a, int seq, int head, int row, int p0, int p1, int c0, uint32_t (&o)[32]) {
+#pragma unroll 1
+    for (int p = p0; p < p1; ++p) {
+        long long at;
+        if (a.table) {
+            const int page = __ldg(a.table + (long long)seq * a.max_pages + (p >> a.page_shift));
+            if ((unsigned)page >= (unsigned)a.n_pages) continue;
+            at = page * a.kv_page + head * a.kv_head + (p & ((1 << a.page_shift) - 1)) * a.kv_tok;
+        } else {
+            at = (long long)(row + p) * a.kv_tok + head * a.kv_head;
+        }
+        const uint32_t *v = reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.v) + at + c0);
+#pragma unroll
+        for (int y = 0; y < 16; ++y) {
+            const uint32_t w = __ldg(v + y);
+            if (ta_finite<BF16>(w) == w) continue;
+            const float2 f = ta_unpack<BF16>(w);
+            if (!isfinite(f.x)) o[2 * y] = __float_as_uint(__uint_as_float(o[2 * y]) + f.x);
+            if (!isfinite(f.y)) o[2 * y + 1] = __float_as_uint(__uint_as_float(o[2 * y + 1]) + f.y);
+        }
+    }
 }
 
 template <int D, bool BF16, bool HILO>
@@ -143,7 +197,8 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sbase = smem_u32(smem), bars = sbase + L::BARS;
     const uint32_t kv_full = bars, kv_empty = bars + 8 * L::STAGES, q_full = bars + 16 * L::STAGES, q_empty = q_full + 8, s_full = q_full + 16,
-                   p_full = q_full + 32, o_full = q_full + 48, drain = q_full + 64, v_ok = q_full + 72, e_full = v_ok + 8 * L::OKS;
+                   p_full = q_full + 32, o_full = q_full + 48, drain = q_full + 64, v_ok = q_full + 72, e_full = v_ok + 8 * L::OKS, g_full = e_full + 8 * L::OKS,
+                   g_empty = g_full + 8 * TA_SEGS;
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem + L::MISC);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::MISC + 4);        // [0] flag, [1] limit
     volatile int *seg_bad = reinterpret_cast<volatile int *>(smem + L::MISC + 16), *seg_odd = seg_bad + 4;
@@ -159,6 +214,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             mbar_init(o_full + 8 * i, 1);
         }
         for (int i = 0; i < 2 * L::OKS; ++i) mbar_init(v_ok + 8 * i, 1);       // and e_full
+        for (int i = 0; i < TA_SEGS; ++i) { mbar_init(g_full + 8 * i, 1); mbar_init(g_empty + 8 * i, TA_SEG_USERS); }
         mbar_init(drain, 1);
         for (int i = 0; i < 4; ++i) seg_bad[i] = seg_odd[i] = 0;
         abort_flag[0] = 0;
@@ -168,55 +224,63 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     if (warp == 8) tc5_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), 512);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    AttnCut first, last;
-    attn_share(a, blockIdx.x, gridDim.x, TA_UNIT_SHIFT, min_units, first, last);
     tc5_fence_before();
     __syncthreads();
     tc5_fence_after();
     const uint32_t tmem = *tmem_slot;                       // S of the tiles at columns 0, 128; O at 256, 384
-    AttnWalk walk;
-    walk.begin(first, last);
-    AttnSeg g;
+    volatile TaSeg *const ring = reinterpret_cast<volatile TaSeg *>(smem + L::SEGS);
     bool ok = true;
+    uint32_t gi = 0;                                        // segments seen
+    // the next segment, or NULL at the end of the share
+    auto seg_next = [&]() -> const volatile TaSeg * {
+        ok = ok && __all_sync(0xffffffffu, tc5_wait(g_full + 8 * (gi % TA_SEGS), (gi / TA_SEGS) & 1, abort_flag));
+        const volatile TaSeg *t = ring + gi % TA_SEGS;
+        return ok && t->seq >= 0 ? t : nullptr;
+    };
+    auto seg_done = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(g_empty + 8 * (gi % TA_SEGS));
+        gi++;
+    };
 #define TA_REGS(how, n) asm volatile("setmaxnreg." how ".sync.aligned.u32 %0;" ::"n"(n))
 
     if (warp == 9) {
         TA_REGS("dec", TA_REGS_OTHER);
         // ------------------------------------------------ producer
         uint32_t it = 0, segs = 0, edges = 0;               // tiles issued, segments with work, edge tiles of V
-        while (ok && walk.next(a, TA_UNIT_SHIFT, g)) {
-            const TaSeg t = ta_seg(a, g);
-            const int E = max(t.e[0], t.e[1]);
-            if (E == 0) continue;
+        while (const volatile TaSeg *t = seg_next()) {
+            const int u0 = t->u0, E = max(t->e[0], t->e[1]);
+            if (E == 0) { seg_done(); continue; }
             if (segs) ok = __all_sync(0xffffffffu, tc5_wait(q_empty, (segs - 1) & 1, abort_flag));
             if (!ok) break;
+            const int u1 = u0 + E, len = t->len, head = t->head, row = t->row, edge = t->edge;
+            const int *table = a.table ? a.table + (long long)t->seq * a.max_pages : nullptr;
             if (lane == 0) {
-                seg_bad[segs & 3] = g.q.over;
-                const int tiles = t.ntok > tq ? 2 : 1;      // of Q; boxes of g heads x tq tokens x 64 columns
+                seg_bad[segs & 3] = t->over;
+                const int tiles = t->ntok > tq ? 2 : 1;      // of Q; boxes of g heads x tq tokens x 64 columns
                 mbar_arrive_expect_tx(q_full, tiles * L::NH * a.g * tq * 128);
                 for (int i = 0; i < tiles; ++i)
                     for (int h = 0; h < L::NH; ++h)
-                        ta_tma_3d(sbase + L::Q + i * L::TILE + h * L::HALF, &qmap, h * 64, g.head * a.g, g.q.row + t.tok0 + i * tq, q_full);
+                        ta_tma_3d(sbase + L::Q + i * L::TILE + h * L::HALF, &qmap, h * 64, head * a.g, row + t->tok0 + i * tq, q_full);
             }
             __syncwarp();
             // lane b * NH + h fetches box b (box_rows positions) of 64-column half h
             const int box = lane / L::NH, half = lane % L::NH, nbox = TA_KV / box_rows;
             auto page_of = [&](int u) -> int {
                 const int p = u * TA_KV + box * box_rows;
-                if (!a.table || box >= nbox || u >= g.u1 || p >= g.q.len) return 0;
-                return __ldg(a.table + (long long)g.seq * a.max_pages + (p >> a.page_shift));
+                return table && box < nbox && u < u1 && p < len ? __ldg(table + (p >> a.page_shift)) : 0;
             };
-            int page = page_of(g.u0);
-            for (int u = g.u0; u < g.u0 + E && ok; ++u) {
+            int page = page_of(u0);
+            for (int u = u0; u < u1 && ok; ++u) {
                 const int p = u * TA_KV + box * box_rows;
-                const int boxes = min(nbox, (g.q.len - u * TA_KV + box_rows - 1) / box_rows);
+                const int boxes = min(nbox, (len - u * TA_KV + box_rows - 1) / box_rows);
                 const bool mine = box < boxes;
                 int y, z = page;
-                if (a.table) {
+                if (table) {
                     y = p & ((1 << a.page_shift) - 1);
                     if (mine && (unsigned)page >= (unsigned)a.n_pages) { z = a.n_pages; seg_bad[segs & 3] = 1; }   // out of the map: zeros
                 } else {
-                    y = g.q.row + p;
+                    y = row + p;
                 }
                 page = page_of(u + 1);
 #pragma unroll
@@ -228,18 +292,19 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     // an edge tile of V lands on a barrier of its own, which the edge warp waits for: it sees no other tile, and a
                     // stage's barrier would look to it as if a fill that it has not seen were the one it wants
                     uint32_t full = kv_full + 8 * s;
-                    if (kv && u >= t.edge) {
+                    if (kv && u >= edge) {
                         if (lane == 0) mbar_arrive(full);
                         full = e_full + 8 * (edges++ % L::OKS);
                     }
                     if (lane == 0) mbar_arrive_expect_tx(full, boxes * L::NH * box_rows * 128);
                     __syncwarp();
                     if (mine)
-                        ta_tma_4d(sbase + L::KV + s * L::TILE + half * L::HALF + box * box_rows * 128, kv ? &vmap : &kmap, half * 64, y, g.head, z,
+                        ta_tma_4d(sbase + L::KV + s * L::TILE + half * L::HALF + box * box_rows * 128, kv ? &vmap : &kmap, half * 64, y, head, z,
                                   full);
                 }
             }
             segs++;
+            seg_done();
         }
         // a copy must not outlive its CTA: after a failed wait elsewhere those in flight are waited for here
         if (*abort_flag) {
@@ -257,10 +322,10 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         constexpr uint32_t id_s = tc5_idesc(128, 128) | type, id_o = tc5_idesc(128, D) | type | (1u << 16);   // V: N contiguous
         const bool leader = tc5_elect();
         uint32_t it = 0, segs = 0, done[2] = {0, 0}, edges = 0;      // tiles of the ring consumed, segments, P tiles consumed, edge tiles
-        while (ok && walk.next(a, TA_UNIT_SHIFT, g)) {
-            const TaSeg t = ta_seg(a, g);
-            const int E = max(t.e[0], t.e[1]);
-            if (E == 0) continue;
+        while (const volatile TaSeg *t = seg_next()) {
+            const int u0 = t->u0, E = max(t->e[0], t->e[1]);
+            if (E == 0) { seg_done(); continue; }
+            const int e[2] = {t->e[0], t->e[1]}, edge = t->edge - u0;
             ok = __all_sync(0xffffffffu, tc5_wait(q_full, segs & 1, abort_flag)) &&
                  __all_sync(0xffffffffu, tc5_wait(kv_full + 8 * (it % L::STAGES), (it / L::STAGES) & 1, abort_flag));
             if (!ok) break;
@@ -275,14 +340,14 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             };
             if (leader) {
                 for (int i = 0; i < 2; ++i)
-                    if (t.e[i] > 0) scores(i, it % L::STAGES);
+                    if (e[i] > 0) scores(i, it % L::STAGES);
                 tc5_commit(kv_empty + 8 * (it % L::STAGES));
                 if (E == 1) tc5_commit(q_empty);
             }
             it++;                                                    // now at V of unit 0
             for (int j = 0; j < E && ok; ++j, it += 2) {
                 const uint32_t sv = it % L::STAGES, sk = (it + 1) % L::STAGES;
-                if (g.u0 + j >= t.edge) {
+                if (j >= edge) {
                     ok = __all_sync(0xffffffffu, tc5_wait(v_ok + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag));
                     edges++;
                 } else {
@@ -290,7 +355,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 }
                 if (ok && j + 1 < E) ok = __all_sync(0xffffffffu, tc5_wait(kv_full + 8 * sk, ((it + 1) / L::STAGES) & 1, abort_flag));
                 for (int i = 0; i < 2 && ok; ++i) {
-                    if (j >= t.e[i]) continue;
+                    if (j >= e[i]) continue;
                     ok = __all_sync(0xffffffffu, tc5_wait(p_full + 8 * i, done[i] & 1, abort_flag));
                     if (!ok) break;
                     done[i]++;
@@ -305,7 +370,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                             for (int x = 0; x < TA_KV / 16; ++x)
                                 ta_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + 64 + 8 * x, ta_desc_mn(v + x * 2048), id_o, 1);
                         }
-                        if (j + 1 < t.e[i]) scores(i, sk);
+                        if (j + 1 < e[i]) scores(i, sk);
                         else tc5_commit(o_full + 8 * i);
                     }
                 }
@@ -317,6 +382,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             }
             it--;                                                    // the last round counted a K tile that was not there
             segs++;
+            seg_done();
         }
         if (leader) tc5_commit(drain);                               // nothing of the tensor core's is left when TMEM is given back
         __syncwarp();
@@ -328,18 +394,18 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         // or what was in the stage before), and so does what is infinite or NaN: its weight is zero for the rows that do not see it,
         // and 0 * inf is not. The rows that do see it get it back at the end (seg_odd).
         uint32_t it = 0, segs = 0, edges = 0;
-        while (ok && walk.next(a, TA_UNIT_SHIFT, g)) {
-            const TaSeg t = ta_seg(a, g);
-            const int E = max(t.e[0], t.e[1]);
-            if (E == 0) continue;
+        while (const volatile TaSeg *t = seg_next()) {
+            const int u0 = t->u0, E = max(t->e[0], t->e[1]);
+            if (E == 0) { seg_done(); continue; }
+            const int edge = t->edge - u0, left = t->len - u0 * TA_KV;
             if (lane == 0) seg_odd[segs & 3] = 0;
             __syncwarp();
             for (int j = 0; j < E && ok; ++j, it += 2) {
-                if (g.u0 + j < t.edge) continue;
+                if (j < edge) continue;
                 const uint32_t s = (it + 1) % L::STAGES;
                 ok = __all_sync(0xffffffffu, tc5_wait(e_full + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag));
                 if (!ok) break;
-                const int rows = g.q.len - (g.u0 + j) * TA_KV;       // of the sequence
+                const int rows = left - j * TA_KV;       // of the sequence
                 const uint32_t v = sbase + L::KV + s * L::TILE;
                 bool odd = false;
 #pragma unroll 2
@@ -368,9 +434,26 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 edges++;
             }
             segs++;
+            seg_done();
         }
     } else if (warp == 11) {
         TA_REGS("dec", TA_REGS_OTHER);
+        // ------------------------------------------------ the walk
+        AttnCut first, last;
+        attn_share(a, blockIdx.x, gridDim.x, TA_UNIT_SHIFT, min_units, first, last);
+        AttnWalk walk;
+        walk.begin(first, last);
+        AttnSeg g;
+        for (bool more = true; more && ok; ++gi) {
+            if (gi >= TA_SEGS) ok = __all_sync(0xffffffffu, tc5_wait_relaxed(g_empty + 8 * (gi % TA_SEGS), (gi / TA_SEGS + 1) & 1, abort_flag));
+            if (!ok) break;
+            more = walk.next(a, TA_UNIT_SHIFT, g);
+            if (lane == 0) {
+                if (more) ta_seg(a, g, ring + gi % TA_SEGS);
+                else ring[gi % TA_SEGS].seq = -1;
+                mbar_arrive(g_full + 8 * (gi % TA_SEGS));
+            }
+        }
     } else {
         TA_REGS("inc", TA_REGS_SOFTMAX);
         // ------------------------------------------------ softmax: warpgroup i owns tile i, a thread one of its rows
@@ -379,15 +462,14 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         const uint32_t S = tmem + i * 128 + lanes, O = tmem + 256 + i * 128 + lanes;
         const float c = a.scale_log2;
         uint32_t tiles = 0, parts = 0, segs = 0;
-        AttnMeta meta = {0, 0, 0, 0, 0, 0};
-        while (ok && walk.next(a, TA_UNIT_SHIFT, g)) {
-            const TaSeg t = ta_seg(a, g);
+        AttnMeta *const meta = a.meta + blockIdx.x;
+        if (threadIdx.x == 0) meta->cont = meta->ends = meta->own = 0;
+        while (const volatile TaSeg *t = seg_next()) {
+            const int E = t->e[i], p_first = t->u0 * TA_KV;
             const int tok = i * tq + r / a.g;                        // of the item
-            const bool live = r < tq * a.g && tok < t.ntok;
-            const int seen = attn_limit(g.q, t.tok0 + min(tok, t.ntok - 1) + 1);
-            const int all_seen = attn_limit(g.q, t.tok0 + i * tq + 1);      // by the tile's first token: below it nothing is masked
+            const int seen = ta_seen(t, t->tok0 + min(tok, t->ntok - 1) + 1) - p_first;      // positions of the segment that the row sees
+            const int all_seen = ta_seen(t, t->tok0 + i * tq + 1) - p_first;                 // by the tile's first token: below it nothing is masked
             float m = -INFINITY, l = 0.f;                            // m: the maximum that O and l are scaled to (of S, unscaled)
-            const int E = t.e[i];
             for (int j = 0; j < E; ++j, ++tiles) {
                 ok = tc5_wait(s_full + 8 * i, tiles & 1, abort_flag);
                 ok = __all_sync(0xffffffffu, ok);
@@ -397,9 +479,8 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
 #pragma unroll
                 for (int x = 0; x < 4; ++x) tc5_ld32(S + 32 * x, s[x]);
                 tc5_wait_ld();
-                const int p0 = (g.u0 + j) * TA_KV;
-                if (p0 + TA_KV > all_seen) {
-                    const int n = seen - p0;
+                if ((j + 1) * TA_KV > all_seen) {
+                    const int n = seen - j * TA_KV;
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
 #pragma unroll
@@ -411,7 +492,8 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 for (int x = 0; x < 4; ++x) {
                     mx[x] = __uint_as_float(s[x][0]);
 #pragma unroll
-                    for (int y = 1; y < 32; ++y) mx[x] = fmaxf(mx[x], __uint_as_float(s[x][y]));
+                    for (int y = 1; y < 31; y += 2) mx[x] = ta_max3(mx[x], __uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1]));
+                    mx[x] = fmaxf(mx[x], __uint_as_float(s[x][31]));
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 const bool grow = top > m && (top - m) * c > 8.f;    // from -inf too
@@ -421,19 +503,19 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     m = next;
                     l *= f;
                     if (j > 0) {
-#pragma unroll
-                        for (int x = 0; x < D / 32; ++x) {
-                            uint32_t o[32];
-                            tc5_ld32(O + 32 * x, o);
+#pragma unroll 1
+                        for (int x = 0; x < D / 16; ++x) {
+                            uint32_t o[16];
+                            tc5_ld16(O + 16 * x, o);
                             tc5_wait_ld();
 #pragma unroll
-                            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-                            ta_st32(O + 32 * x, o);
+                            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                            ta_st16(O + 16 * x, o);
                         }
                     }
                 }
                 const float mc = m == -INFINITY ? 0.f : -m * c;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     uint32_t hi[16], lo[16];
@@ -443,8 +525,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                         tc5_fma2(u, w, __uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1]), c, mc);
                         u = ta_exp2(u);
                         w = ta_exp2(w);
-                        sum[y & 1] += u;
-                        sum[2 + (y & 1)] += w;
+                        ta_add2(sum[y & 1], u, w);
                         hi[y] = ta_pack<BF16>(u, w);
                         if constexpr (HILO) {
                             const float2 b = ta_unpack<BF16>(hi[y]);
@@ -454,15 +535,14 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     ta_st16(S + 16 * x, hi);
                     if constexpr (HILO) ta_st16(S + 64 + 16 * x, lo);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                l += (sum[0][0] + sum[1][0]) + (sum[0][1] + sum[1][1]);
                 ta_wait_st();
                 tc5_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + 8 * i);
             }
             if (!ok) break;
-            const bool work = max(t.e[0], t.e[1]) > 0;
-            const bool whole = g.u0 == 0 && g.u1 == g.units;
+            const bool live = r < tq * a.g && tok < t->ntok, whole = t->whole;
             bool odd = false;
             if (E > 0) {
                 ok = __all_sync(0xffffffffu, tc5_wait(o_full + 8 * i, parts & 1, abort_flag));
@@ -475,17 +555,26 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             const int row = i * tq * a.g + r;                        // of the item
             float *slot = nullptr;
             if (!whole) {
-                const int which = g.u0 > 0 ? 0 : 1;
+                const int which = t->u0 > 0 ? 0 : 1;
                 slot = a.part + ((size_t)blockIdx.x * 2 + which) * attn_slot_floats(ATTN_TC_ROWS, D);
-                if (which == 0) { meta.cont = 1; meta.ends = g.u1 == g.units; }
-                else { meta.own = 1; meta.row = g.q.row + t.tok0; meta.ntok = t.ntok; meta.head = g.head; }
+                if (threadIdx.x == 0) {
+                    if (which == 0) { meta->cont = 1; meta->ends = t->ends; }
+                    else { meta->own = 1; meta->row = t->row + t->tok0; meta->ntok = t->ntok; meta->head = t->head; }
+                }
                 if (live) {
                     slot[ATTN_TC_ROWS * D + row] = m * c;
                     slot[ATTN_TC_ROWS * D + ATTN_TC_ROWS + row] = l;
                 }
             }
             const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-            const size_t at = ((size_t)(g.q.row + t.tok0 + tok) * a.hq + g.head * a.g + r % a.g) * D;
+            // Rows leave through shared memory, 128 bytes of each at a time: a thread has a row, and its own stores would touch 32 lines
+            // an instruction (8 us of an item's time; now under 1). Where the row goes; negative: nowhere.
+            const bool f32 = !whole || a.out_dtype == JL_DT_F32;
+            uint8_t *const dst = whole ? static_cast<uint8_t *>(a.out) : reinterpret_cast<uint8_t *>(slot);
+            const long long at = !live || (!whole && E == 0) ? -1
+                                 : (whole ? (long long)(t->row + t->tok0 + tok) * a.hq + t->head * a.g + r % a.g : (long long)row) * (f32 ? 4 : 2) * D;
+            const uint32_t stage = sbase + L::OUT + warp * 4096;
+            uint32_t w[32];                                          // the 128 bytes
 #pragma unroll 1
             for (int x = 0; x < D / 32; ++x) {
                 uint32_t o[32];
@@ -496,36 +585,39 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
 #pragma unroll
                     for (int y = 0; y < 32; ++y) o[y] = 0u;
                 }
-                if (odd && live) {
-                    for (int p = max(g.u0, t.edge) * TA_KV; p < min(seen, (g.u0 + E) * TA_KV); ++p) {
-                        long long o0 = a.table ? 0 : (long long)(g.q.row + p) * a.kv_tok + g.head * a.kv_head;
-                        if (a.table) {
-                            const int page = __ldg(a.table + (long long)g.seq * a.max_pages + (p >> a.page_shift));
-                            if ((unsigned)page >= (unsigned)a.n_pages) continue;
-                            o0 = page * a.kv_page + g.head * a.kv_head + (p & ((1 << a.page_shift) - 1)) * a.kv_tok;
-                        }
+                if (odd && live) ta_odd<BF16>(a, t->seq, t->head, t->row, max(t->u0, t->edge) * TA_KV, p_first + min(seen, E * TA_KV), 32 * x, o);
+                if (f32) {
 #pragma unroll
-                        for (int y = 0; y < 16; ++y) {
-                            const uint32_t w = __ldg(reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.v) + o0 + 32 * x) + y);
-                            if (ta_finite<BF16>(w) == w) continue;
-                            const float2 f = ta_unpack<BF16>(w);
-                            if (!isfinite(f.x)) o[2 * y] = __float_as_uint(__uint_as_float(o[2 * y]) + f.x);
-                            if (!isfinite(f.y)) o[2 * y + 1] = __float_as_uint(__uint_as_float(o[2 * y + 1]) + f.y);
-                        }
+                    for (int y = 0; y < 32; ++y) w[y] = __float_as_uint(__uint_as_float(o[y]) * inv);
+                } else {
+#pragma unroll
+                    for (int y = 0; y < 16; ++y) {
+                        const float u = __uint_as_float(o[2 * y]) * inv, v = __uint_as_float(o[2 * y + 1]) * inv;
+                        const uint32_t p = a.out_dtype == JL_DT_BF16 ? ta_pack<true>(u, v) : ta_pack<false>(u, v);
+                        if (x & 1) w[16 + y] = p; else w[y] = p;
                     }
+                    if (!(x & 1)) continue;
                 }
-                if (!live) continue;
+                __syncwarp();                                        // the last pass's rows have been read
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128 + ((y ^ (lane & 7)) << 4)), "r"(w[4 * y]),
+                                 "r"(w[4 * y + 1]), "r"(w[4 * y + 2]), "r"(w[4 * y + 3]) : "memory");
+                __syncwarp();
+                const int col = f32 ? 128 * x : 64 * (x - 1);        // in bytes
 #pragma unroll
                 for (int y = 0; y < 8; ++y) {
-                    const float4 v = make_float4(__uint_as_float(o[4 * y]) * inv, __uint_as_float(o[4 * y + 1]) * inv,
-                                                 __uint_as_float(o[4 * y + 2]) * inv, __uint_as_float(o[4 * y + 3]) * inv);
-                    if (whole) attn_store4(a.out, a.out_dtype, at + 32 * x + 4 * y, v);
-                    else if (E > 0) *reinterpret_cast<float4 *>(slot + (size_t)row * D + 32 * x + 4 * y) = v;
+                    const int rr = 4 * y + (lane >> 3), pc = lane & 7;
+                    const long long to = __shfl_sync(0xffffffffu, at, rr);
+                    uint4 v;
+                    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                 : "r"(stage + rr * 128 + ((pc ^ (rr & 7)) << 4)));
+                    if (to >= 0) *reinterpret_cast<uint4 *>(dst + to + col + 16 * pc) = v;
                 }
             }
-            if (work) segs++;
+            if (max(t->e[0], t->e[1]) > 0) segs++;
+            seg_done();
         }
-        if (threadIdx.x == 0) a.meta[blockIdx.x] = meta;
     }
     tc5_fence_before();
     __syncthreads();
