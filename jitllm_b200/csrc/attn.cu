@@ -346,7 +346,7 @@ JL_EXPORT int jl_test_attn_share(const int32_t *starts, const int32_t *lens, int
     a.starts = starts; a.lens = lens; a.nseq = nseq; a.total = total; a.hkv = hkv; a.tok_item = tok_item;
     a.table = max_pages > 0 ? starts : nullptr;       // only its presence matters here
     a.page_shift = page_shift; a.max_pages = max_pages;
-    a.g = 1; a.row_hi = INT_MAX;
+    a.g = 1; a.row_hi = INT_MAX; a.item_cost = 1;
     AttnCut first, last;
     attn_share_host(a, cta, grid, unit_shift, min_units, first, last);
     AttnWalk w;

@@ -21,6 +21,7 @@ struct AttnArgs {
     int page_shift, n_pages, max_pages;
     int row_lo, row_hi;          // the launch takes the sequences with row_lo < new rows * g <= row_hi
     int tok_item;                // tokens of one item
+    int item_cost;               // what an item's start and end take, in units
     int out_dtype;
     float scale_log2;            // scale * log2(e): softmax is taken to the base 2
 };
@@ -55,11 +56,10 @@ __host__ __device__ static inline int attn_limit(const AttnSeq &q, int t1) {
 }
 
 // The work is a line of items -- (sequence, block of tok_item tokens, kv head), heads innermost -- and item i is as long on it as
-// the positions that it walks plus ATTN_ITEM_COST * unit for its start and end. The line is cut into equal shares, one to a CTA,
+// the positions that it walks plus item_cost units for its start and end. The line is cut into equal shares, one to a CTA,
 // the cuts rounded to whole units of positions inside an item; an item that a cut divides leaves a partial result in each CTA,
 // and attn_merge_kernel joins them in ascending order of positions. A few long sequences thus fill the GPU as well as many short
 // ones, whatever the lengths, which only the device knows; results depend on the cuts in their rounding and on nothing else.
-#define ATTN_ITEM_COST 1         // units
 #define ATTN_SNAP 2              // units: cuts nearer than this to an item's end move onto it, if the shares are long
 
 struct AttnCut { int seq, blk, head, unit; };     // before `unit` of item (seq, blk, head); seq == nseq: the line's end
@@ -80,7 +80,7 @@ __host__ __device__ static inline int attn_blocks(const AttnSeq &q, int T) { ret
 
 // Where a cut at `x` (0 <= x < weight of the sequence times the heads) falls inside sequence s.
 __host__ __device__ static inline AttnCut attn_cut_in(const AttnArgs &a, int s, const AttnSeq &q, long long x, int unit_shift, int snap) {
-    const int T = a.tok_item, cost = ATTN_ITEM_COST << unit_shift;
+    const int T = a.tok_item, cost = a.item_cost << unit_shift;
     int lo = 0, hi = attn_blocks(q, T) - 1;                  // the last block whose blocks in front weigh no more than x
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -147,7 +147,7 @@ struct AttnWalk {
 };
 
 __host__ __device__ static inline long long attn_seq_weight(const AttnArgs &a, const AttnSeq &q, int unit_shift) {
-    return attn_blocks_weight(q, attn_blocks(q, a.tok_item), a.tok_item, ATTN_ITEM_COST << unit_shift) * a.hkv;
+    return attn_blocks_weight(q, attn_blocks(q, a.tok_item), a.tok_item, a.item_cost << unit_shift) * a.hkv;
 }
 // The shares of a line of `total`: how many there are (each min_units units at least), where share `cta` lies, and how near an item's
 // end a cut snaps onto it. False: the CTA has no share.

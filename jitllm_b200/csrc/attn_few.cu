@@ -10,6 +10,7 @@
 
 #define FEW_UNIT_SHIFT 6
 #define FEW_STAGES 2
+#define FEW_ITEM_COST 1
 
 template <int D> struct FewTile {
     static constexpr int ROW = 2 * D + 16;            // bytes of a staged row: padded, so that rows start in different banks
@@ -331,6 +332,7 @@ static int few_go(jl_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
 int attn_launch_few(jl_ctx *ctx, const AttnArgs &args, int dtype, cudaStream_t s) {
     AttnArgs a = args;
     a.tok_item = ATTN_FEW_ROWS / a.g;
+    a.item_cost = FEW_ITEM_COST;
     if (a.d == 128) return dtype == JL_DT_BF16 ? few_go<128, true>(ctx, a, s) : few_go<128, false>(ctx, a, s);
     return dtype == JL_DT_BF16 ? few_go<64, true>(ctx, a, s) : few_go<64, false>(ctx, a, s);
 }

@@ -17,16 +17,49 @@
 #include "attn.cuh"
 #include "tc5.cuh"
 
+#include <type_traits>
+
 #define TA_UNIT_SHIFT 7
 #define TA_KV 128                        // positions of a unit
-#define TA_WARPS 12                      // 0-3, 4-7 softmax of tile 0, 1; 8 MMA; 9 producer; 10 edges; 11 the walk
-// Registers: launched with 168 a thread (384 threads: 64512); the softmax warpgroups, whose rows of S live in registers, go up by 40 a
-// thread (256 threads: 10240), the third goes down by 80 (128 threads: 10240).
+#define TA_WARPS 12                      // 0-3, 4-7 softmax of tile 0, 1; then
+#define TA_MMA 8
+#define TA_PRODUCER 9
+#define TA_EDGES 10
+#define TA_WALK 11
+// Registers: launched with 168 a thread (384 threads: 64512); the softmax warpgroups, whose rows of S and P live in registers, go up by 40
+// a thread (256 threads: 10240), the others go down by 80 (128 threads: 10240).
 #define TA_REGS_SOFTMAX 208
 #define TA_REGS_OTHER 88
 #define TA_STATUS_CODE 7
+#define TA_ITEM_COST 4
+#define TA_LIMIT 16384.f                 // of a tile's sum of weights: f16 holds each
+#ifndef TA_POLY
+#define TA_POLY 0  // pairs of 16 whose exponentials run on the FMA pipe
+#endif
 
 
+// The bounded wait of this kernel's roles. A try that may sleep for up to 20 us: the warps that wait are many, and their polling would take
+// the issue slots of those that work.
+__device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+    uint64_t t0 = 0;
+    for (;;) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity), "r"(20000u)
+            : "memory");
+        if (done) return true;
+        if (*abort_flag) return false;
+        const uint64_t t = jl_gtime_ns();
+        if (!t0) t0 = t;
+        else if (t - t0 > tc5_limit_ns(abort_flag)) break;
+    }
+    *abort_flag = 1;
+    return false;
+}
 // D[tmem] (+)= A[tmem] * B[smem desc].
 __device__ __forceinline__ void ta_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -54,6 +87,24 @@ __device__ __forceinline__ void ta_st16(uint32_t taddr, const uint32_t (&r)[16])
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+// The loads into r are complete. The registers are operands, so that nothing that reads them moves in front of the wait.
+__device__ __forceinline__ void ta_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]),
+                 "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void ta_wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void ta_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void ta_tma_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -75,9 +126,9 @@ __device__ __forceinline__ uint64_t ta_desc_mn(uint32_t smem_addr) {
     d |= (uint64_t)2 << 61;
     return d;
 }
-__device__ __forceinline__ float ta_max3(float x, float y, float z) {
+__device__ __forceinline__ float ta_max(float x, float y) {          // NaN if either is
     float m;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(x), "f"(y), "f"(z));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
     return m;
 }
 // d += x on both halves.
@@ -94,6 +145,45 @@ __device__ __forceinline__ float ta_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// 2^x of two values on the FMA pipe, for x up to 2^7: x = n + f with n the nearest whole number (the low bits of x + 1.5 2^23), 2^f by
+// a polynomial with the least largest relative error on [-1/2, 1/2] (Remez exchange; 7.5e-5 at degree 3, 2.7e-6 at degree 4: a fiftieth
+// and a hundred-and-eightieth of half a unit of the bf16 or f16 that the result is rounded to), n added to the exponent. What lies below
+// 2^-125 comes out as about that, what lies above 2^127 and NaN as something above 2^126 or NaN.
+template <int DEG>
+__device__ __forceinline__ void ta_exp2_poly(float &x0, float &x1) {
+    constexpr float C3[5] = {0.999928057f, 0.693260968f, 0.242611125f, 0.0551716685f, 0.f};
+    constexpr float C4[5] = {0.999999285f, 0.693121791f, 0.240247443f, 0.0559178591f, 0.00957010221f};
+    const float a0 = fminf(ta_max(x0, -125.f), 127.f), a1 = fminf(ta_max(x1, -125.f), 127.f);
+    float t0, t1, f0, f1, p0, p1;
+    asm("{\n\t.reg .b64 x, m, t, f, p, c;\n\t"
+        "mov.b64 x, {%6, %7};\n\t"
+        "mov.b64 m, {%8, %8};\n\t"
+        "add.rn.f32x2 t, x, m;\n\t"
+        "mov.b64 {%0, %1}, t;\n\t"
+        "sub.rn.f32x2 f, t, m;\n\t"
+        "sub.rn.f32x2 f, x, f;\n\t"
+        "mov.b64 {%2, %3}, f;\n\t"
+        "mov.b64 p, {%9, %9};\n\t"
+        "mov.b64 c, {%10, %10};\n\t"
+        "fma.rn.f32x2 p, p, f, c;\n\t"
+        "mov.b64 {%4, %5}, p;\n\t}"
+        : "=f"(t0), "=f"(t1), "=f"(f0), "=f"(f1), "=f"(p0), "=f"(p1)
+        : "f"(a0), "f"(a1), "f"(12582912.f), "f"(DEG == 3 ? C3[3] : C4[4]), "f"(DEG == 3 ? C3[2] : C4[3]));
+#pragma unroll
+    for (int i = DEG - 2; i >= 0; --i) {
+        const float c = DEG == 3 ? C3[i] : C4[i];
+        asm("{\n\t.reg .b64 p, f, c;\n\t"
+            "mov.b64 p, {%0, %1};\n\t"
+            "mov.b64 f, {%2, %3};\n\t"
+            "mov.b64 c, {%4, %4};\n\t"
+            "fma.rn.f32x2 p, p, f, c;\n\t"
+            "mov.b64 {%0, %1}, p;\n\t}"
+            : "+f"(p0), "+f"(p1)
+            : "f"(f0), "f"(f1), "f"(c));
+    }
+    x0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+    x1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 template <bool BF16> __device__ __forceinline__ uint32_t ta_pack(float x, float y) {
     if constexpr (BF16) {
@@ -163,27 +253,36 @@ template <int D> struct TaSmem {
     static constexpr int TOTAL = MISC + 64 + 1024;           // 1024: the tiles start on a swizzle atom
 };
 
-// Columns c0 .. c0 + 31 of a row's sum get back what the edge warp took out of positions [p0, p1), which the row sees.
+// A row's results get back what the edge warp took out of positions [p0, p1), which the row sees. The row is `dtype` at dst.
 template <bool BF16>
-__device__ __forceinline__ void ta_odd(const AttnArgs &a, int seq, int head, int row, int p0, int p1, int c0, uint32_t (&o)[32]) {
-#pragma unroll 1
+__device__ __noinline__ void ta_odd(const AttnArgs *a, int seq, int head, int row, int p0, int p1, void *dst, int dtype) {
     for (int p = p0; p < p1; ++p) {
         long long at;
-        if (a.table) {
-            const int page = __ldg(a.table + (long long)seq * a.max_pages + (p >> a.page_shift));
-            if ((unsigned)page >= (unsigned)a.n_pages) continue;
-            at = page * a.kv_page + head * a.kv_head + (p & ((1 << a.page_shift) - 1)) * a.kv_tok;
+        if (a->table) {
+            const int page = __ldg(a->table + (long long)seq * a->max_pages + (p >> a->page_shift));
+            if ((unsigned)page >= (unsigned)a->n_pages) continue;
+            at = page * a->kv_page + head * a->kv_head + (p & ((1 << a->page_shift) - 1)) * a->kv_tok;
         } else {
-            at = (long long)(row + p) * a.kv_tok + head * a.kv_head;
+            at = (long long)(row + p) * a->kv_tok + head * a->kv_head;
         }
-        const uint32_t *v = reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a.v) + at + c0);
-#pragma unroll
-        for (int y = 0; y < 16; ++y) {
+        const uint32_t *v = reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a->v) + at);
+#pragma unroll 1
+        for (int y = 0; y < a->d / 2; ++y) {
             const uint32_t w = __ldg(v + y);
             if (ta_finite<BF16>(w) == w) continue;
-            const float2 f = ta_unpack<BF16>(w);
-            if (!isfinite(f.x)) o[2 * y] = __float_as_uint(__uint_as_float(o[2 * y]) + f.x);
-            if (!isfinite(f.y)) o[2 * y + 1] = __float_as_uint(__uint_as_float(o[2 * y + 1]) + f.y);
+            float2 f = ta_unpack<BF16>(w);                   // what is finite of the pair is in the sum already
+            f.x = isfinite(f.x) ? 0.f : f.x;
+            f.y = isfinite(f.y) ? 0.f : f.y;
+            if (dtype == JL_DT_F32) {
+                float *o = static_cast<float *>(dst) + 2 * y;
+                o[0] += f.x; o[1] += f.y;
+            } else if (dtype == JL_DT_BF16) {
+                __nv_bfloat16 *o = static_cast<__nv_bfloat16 *>(dst) + 2 * y;
+                o[0] = __float2bfloat16(__bfloat162float(o[0]) + f.x); o[1] = __float2bfloat16(__bfloat162float(o[1]) + f.y);
+            } else {
+                __half *o = static_cast<__half *>(dst) + 2 * y;
+                o[0] = __float2half(__half2float(o[0]) + f.x); o[1] = __float2half(__half2float(o[1]) + f.y);
+            }
         }
     }
 }
@@ -221,7 +320,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         abort_flag[1] = a.status[1];
         mbar_init_fence();
     }
-    if (warp == 8) tc5_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), 512);
+    if (warp == TA_MMA) tc5_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), 512);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     tc5_fence_before();
@@ -233,7 +332,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     uint32_t gi = 0;                                        // segments seen
     // the next segment, or NULL at the end of the share
     auto seg_next = [&]() -> const volatile TaSeg * {
-        ok = ok && __all_sync(0xffffffffu, tc5_wait(g_full + 8 * (gi % TA_SEGS), (gi / TA_SEGS) & 1, abort_flag));
+        ok = ok && __all_sync(0xffffffffu, ta_wait(g_full + 8 * (gi % TA_SEGS), (gi / TA_SEGS) & 1, abort_flag));
         const volatile TaSeg *t = ring + gi % TA_SEGS;
         return ok && t->seq >= 0 ? t : nullptr;
     };
@@ -244,63 +343,66 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     };
 #define TA_REGS(how, n) asm volatile("setmaxnreg." how ".sync.aligned.u32 %0;" ::"n"(n))
 
-    if (warp == 9) {
+    if (warp == TA_PRODUCER) {
         TA_REGS("dec", TA_REGS_OTHER);
-        // ------------------------------------------------ producer
+        // ------------------------------------------------ producer: the ring's tiles are K's and V's in turn
+        const uint32_t sb = (uint32_t)tc5_uniform((int)sbase);
         uint32_t it = 0, segs = 0, edges = 0;               // tiles issued, segments with work, edge tiles of V
+        const bool leader = tc5_elect();
         while (const volatile TaSeg *t = seg_next()) {
-            const int u0 = t->u0, E = max(t->e[0], t->e[1]);
+            const int u0 = tc5_uniform(t->u0), E = tc5_uniform(max(t->e[0], t->e[1]));
             if (E == 0) { seg_done(); continue; }
-            if (segs) ok = __all_sync(0xffffffffu, tc5_wait(q_empty, (segs - 1) & 1, abort_flag));
-            if (!ok) break;
-            const int u1 = u0 + E, len = t->len, head = t->head, row = t->row, edge = t->edge;
+            const int u1 = u0 + E, len = tc5_uniform(t->len), head = tc5_uniform(t->head), row = tc5_uniform(t->row), edge = tc5_uniform(t->edge);
             const int *table = a.table ? a.table + (long long)t->seq * a.max_pages : nullptr;
-            if (lane == 0) {
+            if (segs) ok = __all_sync(0xffffffffu, ta_wait(q_empty, (segs - 1) & 1, abort_flag));
+            if (!ok) break;
+            const int tiles = tc5_uniform(t->ntok > tq ? 2 : 1), tok = row + tc5_uniform(t->tok0);
+            if (leader) {
                 seg_bad[segs & 3] = t->over;
-                const int tiles = t->ntok > tq ? 2 : 1;      // of Q; boxes of g heads x tq tokens x 64 columns
-                mbar_arrive_expect_tx(q_full, tiles * L::NH * a.g * tq * 128);
+                mbar_arrive_expect_tx(q_full, tiles * L::NH * a.g * tq * 128);       // boxes of g heads x tq tokens x 64 columns
                 for (int i = 0; i < tiles; ++i)
+#pragma unroll
                     for (int h = 0; h < L::NH; ++h)
-                        ta_tma_3d(sbase + L::Q + i * L::TILE + h * L::HALF, &qmap, h * 64, head * a.g, row + t->tok0 + i * tq, q_full);
+                        ta_tma_3d(sb + L::Q + i * L::TILE + h * L::HALF, &qmap, h * 64, head * a.g, tok + i * tq, q_full);
             }
             __syncwarp();
-            // lane b * NH + h fetches box b (box_rows positions) of 64-column half h
-            const int box = lane / L::NH, half = lane % L::NH, nbox = TA_KV / box_rows;
+            const int nbox = TA_KV / box_rows;               // a page, or the part of it in a unit; lane b looks up the page of box b
             auto page_of = [&](int u) -> int {
-                const int p = u * TA_KV + box * box_rows;
-                return table && box < nbox && u < u1 && p < len ? __ldg(table + (p >> a.page_shift)) : 0;
+                const int p = u * TA_KV + lane * box_rows;
+                return table && lane < nbox && u < u1 && p < len ? __ldg(table + (p >> a.page_shift)) : 0;
             };
             int page = page_of(u0);
             for (int u = u0; u < u1 && ok; ++u) {
-                const int p = u * TA_KV + box * box_rows;
                 const int boxes = min(nbox, (len - u * TA_KV + box_rows - 1) / box_rows);
-                const bool mine = box < boxes;
-                int y, z = page;
-                if (table) {
-                    y = p & ((1 << a.page_shift) - 1);
-                    if (mine && (unsigned)page >= (unsigned)a.n_pages) { z = a.n_pages; seg_bad[segs & 3] = 1; }   // out of the map: zeros
-                } else {
-                    y = row + p;
+                int z = page;
+                if (table && (unsigned)z >= (unsigned)a.n_pages) {           // out of the map: zeros
+                    z = a.n_pages;
+                    seg_bad[segs & 3] = 1;
                 }
                 page = page_of(u + 1);
+                const int y = table ? (u * TA_KV) & ((1 << a.page_shift) - 1) : row + u * TA_KV;
 #pragma unroll
-                for (int kv = 0; kv < 2; ++kv, ++it) {
+                for (int kv = 0; kv < 2 && ok; ++kv, ++it) {
                     const uint32_t s = it % L::STAGES;
-                    if (it >= (uint32_t)L::STAGES)
-                        ok = __all_sync(0xffffffffu, tc5_wait(kv_empty + 8 * s, (it / L::STAGES + 1) & 1, abort_flag));
+                    if (it >= (uint32_t)L::STAGES) ok = __all_sync(0xffffffffu, ta_wait(kv_empty + 8 * s, (it / L::STAGES + 1) & 1, abort_flag));
                     if (!ok) break;
                     // an edge tile of V lands on a barrier of its own, which the edge warp waits for: it sees no other tile, and a
                     // stage's barrier would look to it as if a fill that it has not seen were the one it wants
                     uint32_t full = kv_full + 8 * s;
                     if (kv && u >= edge) {
-                        if (lane == 0) mbar_arrive(full);
+                        if (leader) mbar_arrive(full);
                         full = e_full + 8 * (edges++ % L::OKS);
                     }
-                    if (lane == 0) mbar_arrive_expect_tx(full, boxes * L::NH * box_rows * 128);
+                    if (leader) mbar_arrive_expect_tx(full, boxes * L::NH * box_rows * 128);
+                    uint32_t dst = sb + L::KV + s * L::TILE;
+                    for (int b = 0; b < boxes; ++b, dst += box_rows * 128) { // one lane issues: its operands are the same in every lane
+                        const int zb = __shfl_sync(0xffffffffu, z, b);
+                        if (leader) {
+#pragma unroll
+                            for (int h = 0; h < L::NH; ++h) ta_tma_4d(dst + h * L::HALF, kv ? &vmap : &kmap, h * 64, y, head, zb, full);
+                        }
+                    }
                     __syncwarp();
-                    if (mine)
-                        ta_tma_4d(sbase + L::KV + s * L::TILE + half * L::HALF + box * box_rows * 128, kv ? &vmap : &kmap, half * 64, y, head, z,
-                                  full);
                 }
             }
             segs++;
@@ -315,32 +417,35 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             for (uint32_t i = edges > (uint32_t)L::OKS ? edges - L::OKS : 0; i < edges; ++i)
                 mbar_wait_ns(e_full + 8 * (i % L::OKS), (i / L::OKS) & 1, limit);
         }
-    } else if (warp == 8) {
+    } else if (warp == TA_MMA) {
         TA_REGS("dec", TA_REGS_OTHER);
-        // ------------------------------------------------ MMA
+        // ------------------------------------------------ products
         constexpr uint32_t type = BF16 ? (1u << 7) | (1u << 10) : 0u;
         constexpr uint32_t id_s = tc5_idesc(128, 128) | type, id_o = tc5_idesc(128, D) | type | (1u << 16);   // V: N contiguous
         const bool leader = tc5_elect();
+        // What the instructions take has to be known to be the same in every lane: otherwise each operand of each is moved to a uniform
+        // register on its own, and a product takes longer to issue than to run (95 clocks against 60).
+        const uint32_t tm = (uint32_t)tc5_uniform((int)tmem), sb = (uint32_t)tc5_uniform((int)sbase);
+        const uint64_t qd = tc5_smem_desc(sb + L::Q), kd = tc5_smem_desc(sb + L::KV), vd = ta_desc_mn(sb + L::KV);
         uint32_t it = 0, segs = 0, done[2] = {0, 0}, edges = 0;      // tiles of the ring consumed, segments, P tiles consumed, edge tiles
+        auto scores = [&](int i, uint32_t stage) {                   // S of tile i = Q K^T
+            const uint64_t q = qd + i * (L::TILE >> 4), k = kd + stage * (L::TILE >> 4);
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x)
+                tc5_mma_f16(tm + i * 128, q + ((x / 4) * (L::HALF >> 4) + 2 * (x % 4)), k + ((x / 4) * (L::HALF >> 4) + 2 * (x % 4)), id_s, x != 0);
+            tc5_commit(s_full + 8 * i);
+        };
         while (const volatile TaSeg *t = seg_next()) {
-            const int u0 = t->u0, E = max(t->e[0], t->e[1]);
+            const int u0 = tc5_uniform(t->u0), e0 = tc5_uniform(t->e[0]), e1 = tc5_uniform(t->e[1]), E = max(e0, e1);
             if (E == 0) { seg_done(); continue; }
-            const int e[2] = {t->e[0], t->e[1]}, edge = t->edge - u0;
-            ok = __all_sync(0xffffffffu, tc5_wait(q_full, segs & 1, abort_flag)) &&
-                 __all_sync(0xffffffffu, tc5_wait(kv_full + 8 * (it % L::STAGES), (it / L::STAGES) & 1, abort_flag));
+            const int edge = tc5_uniform(t->edge) - u0;
+            ok = __all_sync(0xffffffffu, ta_wait(q_full, segs & 1, abort_flag)) &&
+                 __all_sync(0xffffffffu, ta_wait(kv_full + 8 * (it % L::STAGES), (it / L::STAGES) & 1, abort_flag));
             if (!ok) break;
             tc5_fence_after();
-            auto scores = [&](int i, uint32_t stage) {               // S of tile i = Q K^T
-                const uint32_t q = sbase + L::Q + i * L::TILE, k = sbase + L::KV + stage * L::TILE;
-#pragma unroll
-                for (int x = 0; x < D / 16; ++x)
-                    tc5_mma_f16(tmem + i * 128, tc5_smem_desc(q + (x / 4) * L::HALF) + 2 * (x % 4), tc5_smem_desc(k + (x / 4) * L::HALF) + 2 * (x % 4),
-                                id_s, x != 0);
-                tc5_commit(s_full + 8 * i);
-            };
             if (leader) {
-                for (int i = 0; i < 2; ++i)
-                    if (e[i] > 0) scores(i, it % L::STAGES);
+                if (e0 > 0) scores(0, it % L::STAGES);
+                if (e1 > 0) scores(1, it % L::STAGES);
                 tc5_commit(kv_empty + 8 * (it % L::STAGES));
                 if (E == 1) tc5_commit(q_empty);
             }
@@ -348,31 +453,31 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             for (int j = 0; j < E && ok; ++j, it += 2) {
                 const uint32_t sv = it % L::STAGES, sk = (it + 1) % L::STAGES;
                 if (j >= edge) {
-                    ok = __all_sync(0xffffffffu, tc5_wait(v_ok + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag));
+                    ok = __all_sync(0xffffffffu, ta_wait(v_ok + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag));
                     edges++;
                 } else {
-                    ok = __all_sync(0xffffffffu, tc5_wait(kv_full + 8 * sv, (it / L::STAGES) & 1, abort_flag));
+                    ok = __all_sync(0xffffffffu, ta_wait(kv_full + 8 * sv, (it / L::STAGES) & 1, abort_flag));
                 }
-                if (ok && j + 1 < E) ok = __all_sync(0xffffffffu, tc5_wait(kv_full + 8 * sk, ((it + 1) / L::STAGES) & 1, abort_flag));
-                for (int i = 0; i < 2 && ok; ++i) {
-                    if (j >= e[i]) continue;
-                    ok = __all_sync(0xffffffffu, tc5_wait(p_full + 8 * i, done[i] & 1, abort_flag));
-                    if (!ok) break;
-                    done[i]++;
+                if (ok && j + 1 < E) ok = __all_sync(0xffffffffu, ta_wait(kv_full + 8 * sk, ((it + 1) / L::STAGES) & 1, abort_flag));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int e = i ? e1 : e0;
+                    if (!ok || j >= e) continue;
+                    ok = __all_sync(0xffffffffu, ta_wait(p_full + 8 * i, done[i] & 1, abort_flag));
+                    if (!ok) continue;
                     tc5_fence_after();
                     if (leader) {
-                        const uint32_t v = sbase + L::KV + sv * L::TILE;
+                        const uint64_t v = vd + sv * (L::TILE >> 4);
+                        const uint32_t p = tm + i * 128, o = tm + 256 + i * 128;
 #pragma unroll
-                        for (int x = 0; x < TA_KV / 16; ++x)
-                            ta_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * x, ta_desc_mn(v + x * 2048), id_o, j != 0 || x != 0);
-                        if constexpr (HILO) {
-#pragma unroll
-                            for (int x = 0; x < TA_KV / 16; ++x)
-                                ta_mma_ts(tmem + 256 + i * 128, tmem + i * 128 + 64 + 8 * x, ta_desc_mn(v + x * 2048), id_o, 1);
+                        for (int x = 0; x < TA_KV / 16; ++x) {
+                            ta_mma_ts(o, p + 32 * (x >> 1) + 8 * (x & 1), v + x * (2048 >> 4), id_o, j != 0 || x != 0);
+                            if constexpr (HILO) ta_mma_ts(o, p + 32 * (x >> 1) + 16 + 8 * (x & 1), v + x * (2048 >> 4), id_o, 1);
                         }
-                        if (j + 1 < e[i]) scores(i, sk);
+                        if (j + 1 < e) scores(i, sk);
                         else tc5_commit(o_full + 8 * i);
                     }
+                    done[i]++;
                 }
                 if (ok && leader) {
                     tc5_commit(kv_empty + 8 * sv);
@@ -387,7 +492,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         if (leader) tc5_commit(drain);                               // nothing of the tensor core's is left when TMEM is given back
         __syncwarp();
         if (!mbar_wait_ns(drain, 0, tc5_limit_ns(abort_flag))) *abort_flag = 1;
-    } else if (warp == 10) {
+    } else if (warp == TA_EDGES) {
         TA_REGS("dec", TA_REGS_OTHER);
         // ------------------------------------------------ edges
         // V tiles at the edge of what the item's rows see. Positions behind the sequence's end become zeros (another sequence's rows,
@@ -403,29 +508,35 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             for (int j = 0; j < E && ok; ++j, it += 2) {
                 if (j < edge) continue;
                 const uint32_t s = (it + 1) % L::STAGES;
-                ok = __all_sync(0xffffffffu, tc5_wait(e_full + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag));
+                ok = __all_sync(0xffffffffu, ta_wait(e_full + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag));
                 if (!ok) break;
                 const int rows = left - j * TA_KV;       // of the sequence
                 const uint32_t v = sbase + L::KV + s * L::TILE;
-                bool odd = false;
-#pragma unroll 2
-                for (int x = lane; x < L::NH * 128 * 8; x += 32) {   // 16-byte pieces, eight to a row of a half
-                    const uint32_t at = v + x * 16;
-                    uint32_t w[4] = {0, 0, 0, 0};
-                    bool write = true;
-                    if (((x >> 3) & 127) < rows) {
-                        uint32_t f[4];
-                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
-                        write = false;
+                const int used = min(rows, TA_KV) * 8;               // 16-byte pieces of a half, eight to a row
+                uint32_t seen = 0;
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            f[y] = ta_finite<BF16>(w[y]);
-                            write = write || f[y] != w[y];
-                            w[y] = f[y];
-                        }
-                        odd = odd || write;
+                for (int h = 0; h < L::NH; ++h) {
+#pragma unroll 8
+                    for (int x = lane; x < used; x += 32) {
+                        uint32_t w[4];
+                        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(v + h * L::HALF + x * 16));
+                        // an exponent of all ones carries into the sign's place
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) seen |= (w[y] & 0x7FFF7FFFu) + (BF16 ? 0x00800080u : 0x04000400u);
                     }
-                    if (write) asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                    for (int x = used + lane; x < TA_KV * 8; x += 32)
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v + h * L::HALF + x * 16), "r"(0u) : "memory");
+                }
+                const bool odd = __any_sync(0xffffffffu, (seen & 0x80008000u) != 0);
+                if (odd) {
+#pragma unroll 1
+                    for (int x = lane; x < L::NH * TA_KV * 8 * 4; x += 32) {
+                        const uint32_t at = v + x * 4;
+                        uint32_t w;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(at));
+                        const uint32_t f = ta_finite<BF16>(w);
+                        if (f != w) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(f) : "memory");
+                    }
                 }
                 if (odd) seg_odd[segs & 3] = 1;
                 fence_async_smem();
@@ -436,7 +547,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             segs++;
             seg_done();
         }
-    } else if (warp == 11) {
+    } else if (warp == TA_WALK) {
         TA_REGS("dec", TA_REGS_OTHER);
         // ------------------------------------------------ the walk
         AttnCut first, last;
@@ -445,7 +556,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         walk.begin(first, last);
         AttnSeg g;
         for (bool more = true; more && ok; ++gi) {
-            if (gi >= TA_SEGS) ok = __all_sync(0xffffffffu, tc5_wait_relaxed(g_empty + 8 * (gi % TA_SEGS), (gi / TA_SEGS + 1) & 1, abort_flag));
+            if (gi >= TA_SEGS) ok = __all_sync(0xffffffffu, ta_wait(g_empty + 8 * (gi % TA_SEGS), (gi / TA_SEGS + 1) & 1, abort_flag));
             if (!ok) break;
             more = walk.next(a, TA_UNIT_SHIFT, g);
             if (lane == 0) {
@@ -457,6 +568,10 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     } else {
         TA_REGS("inc", TA_REGS_SOFTMAX);
         // ------------------------------------------------ softmax: warpgroup i owns tile i, a thread one of its rows
+        // The weights of a tile are taken to the maximum of the tiles before it, without looking for the tile's own first: nothing is
+        // lost as long as they stay in range, and their sum, which is taken anyway, says whether they do. Only where it passes TA_LIMIT
+        // (or is NaN), and at a row's first tile, S is read for its maximum, O rescaled and the weights taken again: S stays whole until
+        // P is written over it at the end. The sums and products are f32, so scaled by up to TA_LIMIT they lose nothing.
         const int i = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // 32 lanes a warp, in bits 16 and up of a TMEM address
         const uint32_t S = tmem + i * 128 + lanes, O = tmem + 256 + i * 128 + lanes;
@@ -467,64 +582,35 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         while (const volatile TaSeg *t = seg_next()) {
             const int E = t->e[i], p_first = t->u0 * TA_KV;
             const int tok = i * tq + r / a.g;                        // of the item
+            const bool live = r < tq * a.g && tok < t->ntok;
             const int seen = ta_seen(t, t->tok0 + min(tok, t->ntok - 1) + 1) - p_first;      // positions of the segment that the row sees
             const int all_seen = ta_seen(t, t->tok0 + i * tq + 1) - p_first;                 // by the tile's first token: below it nothing is masked
+            const bool idle = !__any_sync(0xffffffffu, live);        // no row of the warp is used: its columns of P stay as they are
             float m = -INFINITY, l = 0.f;                            // m: the maximum that O and l are scaled to (of S, unscaled)
             for (int j = 0; j < E; ++j, ++tiles) {
-                ok = tc5_wait(s_full + 8 * i, tiles & 1, abort_flag);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = __all_sync(0xffffffffu, ta_wait(s_full + 8 * i, tiles & 1, abort_flag));
                 if (!ok) break;
+                if (idle) {
+                    if (lane == 0) mbar_arrive(p_full + 8 * i);
+                    continue;
+                }
                 tc5_fence_after();
-                uint32_t s[4][32];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) tc5_ld32(S + 32 * x, s[x]);
-                tc5_wait_ld();
-                if ((j + 1) * TA_KV > all_seen) {
-                    const int n = seen - j * TA_KV;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-#pragma unroll
-                        for (int y = 0; y < 32; ++y)
-                            if (32 * x + y >= n) s[x][y] = 0xFF800000u;
-                }
-                float mx[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    mx[x] = __uint_as_float(s[x][0]);
-#pragma unroll
-                    for (int y = 1; y < 31; y += 2) mx[x] = ta_max3(mx[x], __uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1]));
-                    mx[x] = fmaxf(mx[x], __uint_as_float(s[x][31]));
-                }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                const bool grow = top > m && (top - m) * c > 8.f;    // from -inf too
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float next = fmaxf(m, top);
-                    const float f = next == -INFINITY ? 1.f : ta_exp2((m - next) * c);
-                    m = next;
-                    l *= f;
-                    if (j > 0) {
-#pragma unroll 1
-                        for (int x = 0; x < D / 16; ++x) {
-                            uint32_t o[16];
-                            tc5_ld16(O + 16 * x, o);
-                            tc5_wait_ld();
-#pragma unroll
-                            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
-                            ta_st16(O + 16 * x, o);
-                        }
-                    }
-                }
-                const float mc = m == -INFINITY ? 0.f : -m * c;
-                float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    uint32_t hi[16], lo[16];
+                const int n = seen - j * TA_KV;                      // positions of the tile that the row sees
+                const bool masked = (j + 1) * TA_KV > all_seen;
+                // 32 positions' weights, packed, and (HILO) what the packing left; their sum
+                auto weights = [&](auto poly, const uint32_t (&v)[32], float mc, float (&sum)[2][2], uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+                    constexpr int POLY = HILO ? 0 : decltype(poly)::value;
 #pragma unroll
                     for (int y = 0; y < 16; ++y) {
                         float u, w;
-                        tc5_fma2(u, w, __uint_as_float(s[x][2 * y]), __uint_as_float(s[x][2 * y + 1]), c, mc);
-                        u = ta_exp2(u);
-                        w = ta_exp2(w);
+                        tc5_fma2(u, w, __uint_as_float(v[2 * y]), __uint_as_float(v[2 * y + 1]), c, mc);
+                        // some of the exponentials on the FMA pipe
+                        if ((y * POLY) % 16 < POLY) {
+                            ta_exp2_poly<BF16 ? 3 : 4>(u, w);
+                        } else {
+                            u = ta_exp2(u);
+                            w = ta_exp2(w);
+                        }
                         ta_add2(sum[y & 1], u, w);
                         hi[y] = ta_pack<BF16>(u, w);
                         if constexpr (HILO) {
@@ -532,20 +618,88 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                             lo[y] = ta_pack<BF16>(u - b.x, w - b.y);
                         }
                     }
-                    ta_st16(S + 16 * x, hi);
-                    if constexpr (HILO) ta_st16(S + 64 + 16 * x, lo);
+                };
+                bool slow = masked;
+                if (!slow) {
+                    uint32_t s[4][32], hi[4][16], lo[HILO ? 4 : 1][16];
+                    float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) tc5_ld32(S + 32 * x, s[x]);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) ta_wait_ld(s[x]);
+                    if (j == 0) {                                    // any of the row's scores may be the first reference
+                        float top = __uint_as_float(s[0][0]);
+#pragma unroll
+                        for (int y = 1; y < 32; ++y) top = fmaxf(top, __uint_as_float(s[0][y]));
+                        m = top < INFINITY ? top : 0.f;              // the sum tells of NaN and +inf
+                    }
+                    const float mc = m == -INFINITY ? 0.f : -m * c;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) weights(std::integral_constant<int, TA_POLY>(), s[x], mc, sum, hi[x], lo[HILO ? x : 0]);
+                    const float total = (sum[0][0] + sum[1][0]) + (sum[0][1] + sum[1][1]);
+                    slow = __any_sync(0xffffffffu, live && m == m && (!(total <= TA_LIMIT) || (m == -INFINITY && total > 0.f)));
+                    if (!slow) {
+                        l += total;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {                // over the positions' own columns
+                            ta_st16(S + 32 * x, hi[x]);
+                            if constexpr (HILO) ta_st16(S + 32 * x + 16, lo[x]);
+                        }
+                    }
                 }
-                l += (sum[0][0] + sum[1][0]) + (sum[0][1] + sum[1][1]);
+                if (slow) {
+                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t v[32];
+                        tc5_ld32(S + 32 * x, v);
+                        ta_wait_ld(v);
+#pragma unroll
+                        for (int y = 0; y < 32; ++y) tops[y & 3] = ta_max(tops[y & 3], 32 * x + y < n ? __uint_as_float(v[y]) : -INFINITY);
+                    }
+                    const float top = ta_max(ta_max(tops[0], tops[1]), ta_max(tops[2], tops[3]));      // of the row; m, l and O go up to it
+                    const float next = ta_max(m, top);               // NaN stays
+                    const float f = next == m || next == -INFINITY ? 1.f : ta_exp2((m - next) * c);
+                    m = next < INFINITY ? next : __int_as_float(0x7fffffff);      // a score of NaN or +inf: so is every weight of the row
+                    l *= f;
+                    if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll 1
+                        for (int x = 0; x < D / 16; ++x) {
+                            uint32_t o[16];
+                            tc5_ld16(O + 16 * x, o);
+                            ta_wait_ld(o);
+#pragma unroll
+                            for (int y = 0; y < 16; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f);
+                            ta_st16(O + 16 * x, o);
+                        }
+                    }
+                    const float mc = m == -INFINITY ? 0.f : -m * c;
+                    float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll 1
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t v[32], hi[16], lo[16];
+                        tc5_ld32(S + 32 * x, v);
+                        ta_wait_ld(v);
+#pragma unroll
+                        for (int y = 0; y < 32; ++y)
+                            if (32 * x + y >= n) v[y] = 0xFF800000u;
+                        weights(std::integral_constant<int, 0>(), v, mc, sum, hi, lo);
+                        ta_st16(S + 32 * x, hi);
+                        if constexpr (HILO) ta_st16(S + 32 * x + 16, lo);
+                    }
+                    l += (sum[0][0] + sum[1][0]) + (sum[0][1] + sum[1][1]);
+                }
                 ta_wait_st();
                 tc5_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + 8 * i);
             }
             if (!ok) break;
-            const bool live = r < tq * a.g && tok < t->ntok, whole = t->whole;
+            if (m == -INFINITY) l = 0.f;                             // sees nothing
+            const bool whole = t->whole;
             bool odd = false;
             if (E > 0) {
-                ok = __all_sync(0xffffffffu, tc5_wait(o_full + 8 * i, parts & 1, abort_flag));
+                ok = __all_sync(0xffffffffu, ta_wait(o_full + 8 * i, parts & 1, abort_flag));
                 if (!ok) break;
                 parts++;
                 tc5_fence_after();
@@ -568,7 +722,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             }
             const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
             // Rows leave through shared memory, 128 bytes of each at a time: a thread has a row, and its own stores would touch 32 lines
-            // an instruction (8 us of an item's time; now under 1). Where the row goes; negative: nowhere.
+            // an instruction (8 us of an item's time). Where the row goes; negative: nowhere.
             const bool f32 = !whole || a.out_dtype == JL_DT_F32;
             uint8_t *const dst = whole ? static_cast<uint8_t *>(a.out) : reinterpret_cast<uint8_t *>(slot);
             const long long at = !live || (!whole && E == 0) ? -1
@@ -576,16 +730,15 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             const uint32_t stage = sbase + L::OUT + warp * 4096;
             uint32_t w[32];                                          // the 128 bytes
 #pragma unroll 1
-            for (int x = 0; x < D / 32; ++x) {
+            for (int x = 0; x < D / 32 && !idle; ++x) {
                 uint32_t o[32];
                 if (E > 0) {
                     tc5_ld32(O + 32 * x, o);
-                    tc5_wait_ld();
+                    ta_wait_ld(o);
                 } else {
 #pragma unroll
                     for (int y = 0; y < 32; ++y) o[y] = 0u;
                 }
-                if (odd && live) ta_odd<BF16>(a, t->seq, t->head, t->row, max(t->u0, t->edge) * TA_KV, p_first + min(seen, E * TA_KV), 32 * x, o);
                 if (f32) {
 #pragma unroll
                     for (int y = 0; y < 32; ++y) w[y] = __float_as_uint(__uint_as_float(o[y]) * inv);
@@ -615,6 +768,9 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     if (to >= 0) *reinterpret_cast<uint4 *>(dst + to + col + 16 * pc) = v;
                 }
             }
+            __syncwarp();
+            if (odd && at >= 0)
+                ta_odd<BF16>(&a, t->seq, t->head, t->row, max(t->u0, t->edge) * TA_KV, p_first + min(seen, E * TA_KV), dst + at, f32 ? JL_DT_F32 : a.out_dtype);
             if (max(t->e[0], t->e[1]) > 0) segs++;
             seg_done();
         }
@@ -623,7 +779,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     __syncthreads();
     tc5_fence_after();
     if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, TA_STATUS_CODE);
-    if (warp == 8) tc5_dealloc(tmem, 512);
+    if (warp == TA_MMA) tc5_dealloc(tmem, 512);
 }
 
 static bool ta_map(CUtensorMap *map, const void *base, bool bf16, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
@@ -650,6 +806,7 @@ int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &args, int dtype, cudaStream_t s
     AttnArgs a = args;
     const int tq = 128 / a.g;
     a.tok_item = 2 * tq;
+    a.item_cost = TA_ITEM_COST;
     const bool bf16 = dtype == JL_DT_BF16, hilo = a.out_dtype == JL_DT_F32;
     CUtensorMap q, k, v;
     const cuuint64_t d = a.d;
