@@ -6,100 +6,173 @@
 #include <math.h>
 
 // ------------------------------------------------------------------ join of partial results
-// Block (c, y) joins rows of the item that CTA c began and the CTAs behind it continued: the softmax weights of the parts are
-// 2^(their maximum - the largest), the parts added in ascending order of positions. Bound by the parts' bytes, which come from L2, and,
-// where a long sequence has few rows, by the loads' latency: WAYS warps share a row then, each a run of the parts, the runs added in
-// order (131,071 positions of two kv heads, 222 parts to a row: 150 us with one warp and one part at a time, 4 with eight).
-template <int ROWS, int D, int WAYS>
-__global__ void __launch_bounds__(256) attn_merge_kernel(const __grid_constant__ AttnArgs a, int ctas) {
-    constexpr int RPB = 8 / WAYS, V = D / 32;                     // rows of a block; values of a lane
+// The item that CTA c began, and the CTAs behind it continued: the softmax weights of the parts are 2^(their maximum - the largest), the
+// parts added in ascending order of positions.
+
+// The CTA that holds the item's last part; eight of a lane's looks on their way at a time.
+__device__ __forceinline__ int attn_item_end(const AttnMeta *meta, int c, int ctas) {
+    const int lane = threadIdx.x & 31;
+    for (int at = c + 1;; at += 256) {
+        unsigned m[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = min(at + 32 * k + lane, ctas - 1);
+            m[k] = i == ctas - 1 || (meta[i].cont && meta[i].ends);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const unsigned b = __ballot_sync(0xffffffffu, m[k]);
+            if (b) return min(at + 32 * k + __ffs(b) - 1, ctas - 1);
+        }
+    }
+}
+template <int D>
+__device__ __forceinline__ void attn_merge_store(const AttnArgs &a, const AttnMeta &own, int r, int col, const float (&acc)[D / 32], float L) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const size_t at = ((size_t)(own.row + r / a.g) * a.hq + own.head * a.g + r % a.g) * D + col;
+    if constexpr (D == 128) attn_store4(a.out, a.out_dtype, at, make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv));
+    else attn_store2(a.out, a.out_dtype, at, acc[0] * inv, acc[1] * inv);
+}
+template <int D>
+__device__ __forceinline__ void attn_merge_load(const float *p, float (&v)[D / 32]) {
+    if constexpr (D == 128) {
+        const float4 u = __ldcg(reinterpret_cast<const float4 *>(p));
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+    } else {
+        const float2 u = __ldcg(reinterpret_cast<const float2 *>(p));
+        v[0] = u.x; v[1] = u.y;
+    }
+}
+
+// Many rows and, as a rule, few parts: block (c, y) takes eight rows, a warp each. Bound by the parts' bytes, which come from L2: small
+// warps, many of them.
+template <int ROWS, int D>
+__global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+    constexpr int V = D / 32;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int c = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const AttnMeta own = a.meta[c];
+    if (!own.own || r >= own.ntok * a.g) return;
+    const int end = attn_item_end(a.meta, c, ctas);
+    const size_t slot = attn_slot_floats(ROWS, D);
+    float M = -INFINITY;
+    for (int i = c + lane; i <= end; i += 32)
+        if (i == c || a.meta[i].cont) M = fmaxf(M, __ldcg(a.part + ((size_t)i * 2 + (i == c)) * slot + ROWS * D + r));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float mu = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc[V] = {};
+    for (int i0 = c; i0 <= end; i0 += 32) {
+        float w = 0.f, l = 0.f;                                   // of part i0 + lane
+        if (i0 + lane <= end && (i0 + lane == c || a.meta[i0 + lane].cont)) {
+            const float *p = a.part + ((size_t)(i0 + lane) * 2 + (i0 + lane == c)) * slot + ROWS * D + r;
+            w = exp2f(__ldcg(p) - mu);
+            l = __ldcg(p + ROWS);
+        }
+        const int cnt = min(32, end - i0 + 1);
+#pragma unroll 4
+        for (int k = 0; k < cnt; ++k) {
+            const float wk = __shfl_sync(0xffffffffu, w, k), lk = __shfl_sync(0xffffffffu, l, k);
+            if (lk == 0.f) continue;                              // the part holds nothing of this row, perhaps not even numbers
+            float v[V];
+            attn_merge_load<D>(a.part + ((size_t)(i0 + k) * 2 + (i0 + k == c)) * slot + (size_t)r * D + V * lane, v);
+            L = fmaf(wk, lk, L);
+#pragma unroll
+            for (int x = 0; x < V; ++x) acc[x] = fmaf(wk, v[x], acc[x]);
+        }
+    }
+    attn_merge_store<D>(a, own, r, V * lane, acc, L);
+}
+
+// Few rows and perhaps hundreds of parts: bound by the loads' latency. The eight warps of a block share a row, each a run of its parts with
+// eight loads on their way, the runs added in order (131,071 positions of two kv heads, 222 parts to a row: 150 us with one warp and one
+// part at a time). Most CTAs begin no such item: a block looks over its share of the (CTA, row) pairs in one load and works on those there are.
+template <int ROWS, int D>
+__global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+    constexpr int V = D / 32;
     __shared__ float sums[8][D + 1];                              // a warp's weighted sums, and its sum of weights
     __shared__ float tops[8];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % WAYS;
-    const AttnMeta own = a.meta[c];
-    if (!own.own) return;
-    const int r = blockIdx.y * RPB + warp / WAYS;
-    if (blockIdx.y * RPB >= own.ntok * a.g) return;
-    int end = c + 1;                                              // the CTA that holds the item's last part
-    for (;; end += 32) {
-        const int i = min(end + lane, ctas - 1);
-        const unsigned m = __ballot_sync(0xffffffffu, i == ctas - 1 || (a.meta[i].cont && a.meta[i].ends));
-        if (m) { end = min(end + __ffs(m) - 1, ctas - 1); break; }
-    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const size_t slot = attn_slot_floats(ROWS, D);
-    const bool live = r < own.ntok * a.g;
-    const int n = end - c + 1, lo = c + n * way / WAYS, hi = c + n * (way + 1) / WAYS;
-    // part i of the row: its maximum (none: no weight)
-    auto top_of = [&](int i) { return i > c && !a.meta[i].cont ? -INFINITY : __ldcg(a.part + ((size_t)i * 2 + (i == c)) * slot + ROWS * D + r); };
-    float M = -INFINITY;
-    if (live)
-        for (int i = lo + lane; i < hi; i += 32) M = fmaxf(M, top_of(i));
+    for (int s0 = blockIdx.x; s0 < ctas * ROWS; s0 += 32 * gridDim.x) {
+        const int mine = s0 + lane * (int)gridDim.x;
+        bool is = mine < ctas * ROWS;
+        if (is) {
+            const AttnMeta &m = a.meta[mine / ROWS];
+            is = m.own && mine % ROWS < m.ntok * a.g;
+        }
+        for (unsigned todo = __ballot_sync(0xffffffffu, is); todo; todo &= todo - 1) {
+            const int pick = s0 + (__ffs(todo) - 1) * (int)gridDim.x, c = pick / ROWS, r = pick % ROWS;
+            const AttnMeta own = a.meta[c];
+            const int n = attn_item_end(a.meta, c, ctas) - c + 1, lo = c + n * warp / 8, hi = c + n * (warp + 1) / 8;
+            auto part_of = [&](int i) { return a.part + ((size_t)i * 2 + (i == c)) * slot; };
+            auto there = [&](int i) { return i == c || a.meta[i].cont; };
+            float M = -INFINITY;
+            for (int i = lo + lane; i < hi; i += 32)
+                if (there(i)) M = fmaxf(M, __ldcg(part_of(i) + ROWS * D + r));
 #pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if constexpr (WAYS > 1) {
-        if (lane == 0) tops[warp] = M;
-        __syncthreads();
+            for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+            if (lane == 0) tops[warp] = M;
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < WAYS; ++i) M = fmaxf(M, tops[warp - way + i]);
-    }
-    const float mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[V];
+            for (int i = 0; i < 8; ++i) M = fmaxf(M, tops[i]);
+            const float mu = M == -INFINITY ? 0.f : M;
+            float L = 0.f, acc[V] = {};
+            for (int i0 = lo; i0 < hi; i0 += 32) {
+                float w = 0.f, l = 0.f;                           // of part i0 + lane
+                if (i0 + lane < hi && there(i0 + lane)) {
+                    const float *p = part_of(i0 + lane) + ROWS * D + r;
+                    l = __ldcg(p + ROWS);
+                    w = l == 0.f ? 0.f : exp2f(__ldcg(p) - mu);   // a part that holds nothing of the row, perhaps not even numbers
+                }
+                const int cnt = min(32, hi - i0);
+                for (int k0 = 0; k0 < cnt; k0 += 8) {
+                    float v[8][V], wk[8];
 #pragma unroll
-    for (int x = 0; x < V; ++x) acc[x] = 0.f;
-    if (live)
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            float w = 0.f, l = 0.f;                               // of part i0 + lane
-            if (i0 + lane < hi) {
-                w = exp2f(top_of(i0 + lane) - mu);
-                l = i0 + lane > c && !a.meta[i0 + lane].cont ? 0.f : __ldcg(a.part + ((size_t)(i0 + lane) * 2 + (i0 + lane == c)) * slot + ROWS * D + ROWS + r);
-            }
-            const int cnt = min(32, hi - i0);
-#pragma unroll 8
-            for (int k = 0; k < cnt; ++k) {
-                const float wk = __shfl_sync(0xffffffffu, w, k), lk = __shfl_sync(0xffffffffu, l, k);
-                if (lk == 0.f) continue;                          // the part holds nothing of this row, perhaps not even numbers
-                const float *p = a.part + ((size_t)(i0 + k) * 2 + (i0 + k == c)) * slot + (size_t)r * D + V * lane;
-                L = fmaf(wk, lk, L);
-                if constexpr (V == 4) {
-                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(p));
-                    acc[0] = fmaf(wk, v.x, acc[0]); acc[1] = fmaf(wk, v.y, acc[1]); acc[2] = fmaf(wk, v.z, acc[2]); acc[3] = fmaf(wk, v.w, acc[3]);
-                } else {
-                    const float2 v = __ldcg(reinterpret_cast<const float2 *>(p));
-                    acc[0] = fmaf(wk, v.x, acc[0]); acc[1] = fmaf(wk, v.y, acc[1]);
+                    for (int k = 0; k < 8; ++k) {
+                        wk[k] = __shfl_sync(0xffffffffu, w, (k0 + k) & 31);
+                        const float lk = __shfl_sync(0xffffffffu, l, (k0 + k) & 31);
+                        const bool use = k0 + k < cnt && lk != 0.f;
+                        if (use) L = fmaf(wk[k], lk, L);
+                        else wk[k] = 0.f;
+#pragma unroll
+                        for (int x = 0; x < V; ++x) v[k][x] = 0.f;
+                        if (use) attn_merge_load<D>(part_of(i0 + k0 + k) + (size_t)r * D + V * lane, v[k]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+#pragma unroll
+                        for (int x = 0; x < V; ++x) acc[x] = fmaf(wk[k], v[k][x], acc[x]);
                 }
             }
-        }
-    if constexpr (WAYS > 1) {
 #pragma unroll
-        for (int x = 0; x < V; ++x) sums[warp][V * lane + x] = acc[x];
-        if (lane == 0) sums[warp][D] = L;
-        __syncthreads();
-        if (way) return;
+            for (int x = 0; x < V; ++x) sums[warp][V * lane + x] = acc[x];
+            if (lane == 0) sums[warp][D] = L;
+            __syncthreads();
+            if (warp == 0) {
 #pragma unroll
-        for (int i = 1; i < WAYS; ++i) {
+                for (int i = 1; i < 8; ++i) {
 #pragma unroll
-            for (int x = 0; x < V; ++x) acc[x] += sums[warp + i][V * lane + x];
-            L += sums[warp + i][D];
+                    for (int x = 0; x < V; ++x) acc[x] += sums[i][V * lane + x];
+                    L += sums[i][D];
+                }
+                attn_merge_store<D>(a, own, r, V * lane, acc, L);
+            }
+            __syncthreads();                                      // sums and tops are read
         }
     }
-    if (!live) return;
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    const size_t at = ((size_t)(own.row + r / a.g) * a.hq + own.head * a.g + r % a.g) * D + V * lane;
-    if constexpr (V == 4) attn_store4(a.out, a.out_dtype, at, make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv));
-    else attn_store2(a.out, a.out_dtype, at, acc[0] * inv, acc[1] * inv);
-}
-
-template <int ROWS, int D, int WAYS>
-static cudaError_t merge_go(const AttnArgs &a, int ctas, cudaStream_t s) {
-    constexpr int RPB = 8 / WAYS;
-    return attn_launch_pdl(attn_merge_kernel<ROWS, D, WAYS>, dim3(ctas, (ROWS + RPB - 1) / RPB), dim3(256), 0, s, a, ctas);
 }
 
 int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s) {
-    const cudaError_t e = rows == ATTN_FEW_ROWS ? (a.d == 128 ? merge_go<ATTN_FEW_ROWS, 128, 8>(a, ctas, s) : merge_go<ATTN_FEW_ROWS, 64, 8>(a, ctas, s))
-                                                : (a.d == 128 ? merge_go<ATTN_TC_ROWS, 128, 1>(a, ctas, s) : merge_go<ATTN_TC_ROWS, 64, 1>(a, ctas, s));
+    const dim3 few(ctas * ATTN_FEW_ROWS < ctx->sm_count * 8 ? ctas * ATTN_FEW_ROWS : ctx->sm_count * 8), many(ctas, ATTN_TC_ROWS / 8);
+    const cudaError_t e = rows == ATTN_FEW_ROWS
+        ? (a.d == 128 ? attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 128>, few, dim3(256), 0, s, a, ctas)
+                      : attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 64>, few, dim3(256), 0, s, a, ctas))
+        : (a.d == 128 ? attn_launch_pdl(attn_merge_many_kernel<ATTN_TC_ROWS, 128>, many, dim3(256), 0, s, a, ctas)
+                      : attn_launch_pdl(attn_merge_many_kernel<ATTN_TC_ROWS, 64>, many, dim3(256), 0, s, a, ctas));
     JL_CUDA(ctx, e);
     ctx->st.launches++;
     return JL_OK;

@@ -179,30 +179,30 @@ static inline void attn_share_host(const AttnArgs &a, int cta, int grid, int uni
 }
 
 #ifdef __CUDACC__
-// The two cuts of CTA `cta` of `grid`, found by each warp; every lane returns them.
-__device__ static inline void attn_share(const AttnArgs &a, int cta, int grid, int unit_shift, int min_units,
-                                         AttnCut &first, AttnCut &last) {
+// The two cuts of CTA `cta` of `grid`, found by each warp; every lane returns them. The sequences are gone over twice, for the
+// line's length and for the cuts' places; the first 128 are fetched once, all at a time (a pass of dependent loads is 0.8 us).
+__device__ static inline void attn_share(const AttnArgs &a, int cta, int grid, int unit_shift, int min_units, AttnCut &first, AttnCut &last) {
+    constexpr int KEPT = 4;
     const int lane = threadIdx.x & 31;
-    long long total = 0;
-    for (int s0 = 0; s0 < a.nseq; s0 += 32) {
-        long long w = s0 + lane < a.nseq ? attn_seq_weight(a, attn_seq(a, s0 + lane), unit_shift) : 0;
+    AttnSeq kept[KEPT];
+    long long weight[KEPT], total = 0;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-        total += w;
+    for (int c = 0; c < KEPT; ++c) {
+        kept[c] = AttnSeq{0, 0, 0, 0, 0};
+        if (c * 32 + lane < a.nseq) kept[c] = attn_seq(a, c * 32 + lane);
     }
+#pragma unroll
+    for (int c = 0; c < KEPT; ++c) total += weight[c] = attn_seq_weight(a, kept[c], unit_shift);       // zero for none
+    for (int s0 = KEPT * 32; s0 < a.nseq; s0 += 32)
+        if (s0 + lane < a.nseq) total += attn_seq_weight(a, attn_seq(a, s0 + lane), unit_shift);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     first.seq = last.seq = a.nseq;
     first.blk = first.head = first.unit = last.blk = last.head = last.unit = 0;
-    long long b0, b1;
+    long long b0, b1, base = 0;
     int snap;
     if (!attn_cuts(total, cta, grid, unit_shift, min_units, b0, b1, snap)) return;
-    long long base = 0;
-    for (int s0 = 0; s0 < a.nseq; s0 += 32) {
-        AttnSeq q = {0, 0, 0, 0, 0};
-        long long w = 0;
-        if (s0 + lane < a.nseq) {
-            q = attn_seq(a, s0 + lane);
-            w = attn_seq_weight(a, q, unit_shift);
-        }
+    auto look = [&](int s0, const AttnSeq &q, long long w) {
         long long upto = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -211,22 +211,25 @@ __device__ static inline void attn_share(const AttnArgs &a, int cta, int grid, i
         }
         const long long from = base + upto - w;
         base += __shfl_sync(0xffffffffu, upto, 31);
-        const unsigned m0 = __ballot_sync(0xffffffffu, b0 >= from && b0 < from + w);
-        const unsigned m1 = __ballot_sync(0xffffffffu, b1 >= from && b1 < from + w);
-        AttnCut c = {a.nseq, 0, 0, 0}, e = {a.nseq, 0, 0, 0};
-        if ((m0 >> lane) & 1) c = attn_cut_in(a, s0 + lane, q, b0 - from, unit_shift, snap);
-        if ((m1 >> lane) & 1) e = attn_cut_in(a, s0 + lane, q, b1 - from, unit_shift, snap);
-        if (m0) {
-            const int l = __ffs(m0) - 1;
-            first.seq = __shfl_sync(0xffffffffu, c.seq, l); first.blk = __shfl_sync(0xffffffffu, c.blk, l);
-            first.head = __shfl_sync(0xffffffffu, c.head, l); first.unit = __shfl_sync(0xffffffffu, c.unit, l);
-        }
-        if (m1) {
-            const int l = __ffs(m1) - 1;
-            last.seq = __shfl_sync(0xffffffffu, e.seq, l); last.blk = __shfl_sync(0xffffffffu, e.blk, l);
-            last.head = __shfl_sync(0xffffffffu, e.head, l); last.unit = __shfl_sync(0xffffffffu, e.unit, l);
-        }
-        if (base > b1) break;
+        const unsigned m0 = __ballot_sync(0xffffffffu, b0 >= from && b0 < from + w), m1 = __ballot_sync(0xffffffffu, b1 >= from && b1 < from + w);
+        auto place = [&](unsigned m, long long b, AttnCut &to) {
+            if (!m) return;
+            AttnCut c = {a.nseq, 0, 0, 0};
+            if ((m >> lane) & 1) c = attn_cut_in(a, s0 + lane, q, b - from, unit_shift, snap);
+            const int l = __ffs(m) - 1;
+            to.seq = __shfl_sync(0xffffffffu, c.seq, l); to.blk = __shfl_sync(0xffffffffu, c.blk, l);
+            to.head = __shfl_sync(0xffffffffu, c.head, l); to.unit = __shfl_sync(0xffffffffu, c.unit, l);
+        };
+        place(m0, b0, first);
+        place(m1, b1, last);
+    };
+#pragma unroll
+    for (int c = 0; c < KEPT; ++c)
+        if (c * 32 < a.nseq && base <= b1) look(c * 32, kept[c], weight[c]);
+    for (int s0 = KEPT * 32; s0 < a.nseq && base <= b1; s0 += 32) {
+        AttnSeq q = {0, 0, 0, 0, 0};
+        if (s0 + lane < a.nseq) q = attn_seq(a, s0 + lane);
+        look(s0, q, attn_seq_weight(a, q, unit_shift));
     }
 }
 

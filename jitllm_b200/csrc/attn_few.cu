@@ -10,7 +10,10 @@
 
 #define FEW_UNIT_SHIFT 6
 #define FEW_STAGES 2
-#define FEW_ITEM_COST 1
+#define FEW_ITEM_COST 4          // an item's start and end against a unit: 3.7 us, 0.8 us with the GPU full
+#ifndef FEW_MIN_UNITS
+#define FEW_MIN_UNITS 2
+#endif
 
 template <int D> struct FewTile {
     static constexpr int ROW = 2 * D + 16;            // bytes of a staged row: padded, so that rows start in different banks
@@ -76,14 +79,50 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
     AttnMeta meta = {0, 0, 0, 0, 0, 0};
     AttnWalk walk;
     walk.begin(first, last);
-    AttnSeg sg;
+    AttnSeg sg, ng;
     if (t == 0) bad = 0;
     const uint16_t *kp = static_cast<const uint16_t *>(a.k), *vp = static_cast<const uint16_t *>(a.v);
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(tiles) + warp * FEW_STAGES * TILE;
-    while (walk.next(a, FEW_UNIT_SHIFT, sg)) {
+    // the page of the warp's tile i: 16 positions lie in one (pages are 16 positions at least, cut at multiples of their length)
+    auto page_of = [&](const AttnSeg &g, int i) -> int {
+        const int p = (g.u0 + i) * 64 + warp * 16;
+        if (!a.table || i >= g.u1 - g.u0 || p >= g.q.len) return 0;
+        return __ldg(a.table + (long long)g.seq * a.max_pages + (p >> a.page_shift));
+    };
+    bool more = walk.next(a, FEW_UNIT_SHIFT, ng);
+    int page0 = more ? page_of(ng, 0) : 0, page1 = more ? page_of(ng, 1) : 0;
+    while (more) {
+        sg = ng;
         __syncthreads();                               // bad is set; the last segment's sums are read
         const int tok0 = sg.blk * a.tok_item, ntok = min(a.tok_item, sg.q.n - tok0);
         const int ntile = sg.u1 - sg.u0, base = sg.u0 * 64 + warp * 16;
+        auto issue = [&](int i, int page) {
+            if (i >= ntile) return;
+            const int p = base + i * 64;
+            const uint32_t dst = ring + (i % FEW_STAGES) * TILE;
+            int rows = min(16, sg.q.len - p);          // rows past the sequence arrive as zeros
+            long long at;
+            if (a.table) {
+                if (rows > 0 && (unsigned)page >= (unsigned)a.n_pages) { rows = 0; bad = 1; }
+                if (rows <= 0) page = 0;
+                at = page * a.kv_page + sg.head * a.kv_head + (p & ((1 << a.page_shift) - 1)) * a.kv_tok;
+            } else {
+                at = (long long)(sg.q.row + (rows > 0 ? p : 0)) * a.kv_tok + sg.head * a.kv_head;
+            }
+#pragma unroll
+            for (int j = 0; j < CH / 2; ++j) {
+                const int piece = j * 32 + lane, r = piece / CH, c = piece % CH, bytes = r < rows ? 16 : 0;
+                const long long o = at + (r < rows ? r : 0) * a.kv_tok + c * 8;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * ROW + c * 16), "l"(kp + o), "r"(bytes) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (16 + r) * ROW + c * 16), "l"(vp + o), "r"(bytes) : "memory");
+            }
+        };
+        // Two tiles on their way before anything else is looked up; what the next segment needs is asked for while they come.
+        issue(0, page0);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        issue(1, page1);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        int page = page_of(sg, 2);
         // rows of this thread: gid and gid + 8; row r is token tok0 + r / g, query head r % g of the kv head
         int seen[2];                                   // positions that the row sees
 #pragma unroll
@@ -108,46 +147,14 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
                 qa[ks][2] = __ldg(row[0] + ks * 8 + 4 + tq); qa[ks][3] = __ldg(row[1] + ks * 8 + 4 + tq);
             }
         }
-        // 16 positions lie in one page (pages are 16 positions at least, cut at multiples of their length)
-        auto page_of = [&](int i) -> int {
-            const int p = base + i * 64;
-            if (!a.table || i >= ntile || p >= sg.q.len) return 0;
-            return __ldg(a.table + (long long)sg.seq * a.max_pages + (p >> a.page_shift));
-        };
-        auto issue = [&](int i, int page) {
-            const int p = base + i * 64;
-            const uint32_t dst = ring + (i % FEW_STAGES) * TILE;
-            int rows = min(16, sg.q.len - p);          // rows past the sequence arrive as zeros
-            long long at;
-            if (a.table) {
-                if (rows > 0 && (unsigned)page >= (unsigned)a.n_pages) { rows = 0; bad = 1; }
-                if (rows <= 0) page = 0;
-                at = page * a.kv_page + sg.head * a.kv_head + (p & ((1 << a.page_shift) - 1)) * a.kv_tok;
-            } else {
-                at = (long long)(sg.q.row + (rows > 0 ? p : 0)) * a.kv_tok + sg.head * a.kv_head;
-            }
-#pragma unroll
-            for (int j = 0; j < CH / 2; ++j) {
-                const int piece = j * 32 + lane, r = piece / CH, c = piece % CH, bytes = r < rows ? 16 : 0;
-                const long long o = at + (r < rows ? r : 0) * a.kv_tok + c * 8;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * ROW + c * 16), "l"(kp + o), "r"(bytes) : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (16 + r) * ROW + c * 16), "l"(vp + o), "r"(bytes) : "memory");
-            }
-        };
-        int page = page_of(0);
-        if (ntile > 0) issue(0, page);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        page = page_of(1);
+        more = walk.next(a, FEW_UNIT_SHIFT, ng);
+        if (more) { page0 = page_of(ng, 0); page1 = page_of(ng, 1); }
         float M[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};     // of rows gid, gid + 8 (l: this lane's share)
         float oacc[NJ][4];                                          // O[gid][8 j + 2 tq, + 1], O[gid + 8][same]
 #pragma unroll
         for (int j = 0; j < NJ; ++j) oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f;
 #pragma unroll 1
         for (int i = 0; i < ntile; ++i) {
-            __syncwarp();                                           // every lane is done with the stage that is refilled now
-            if (i + 1 < ntile) issue(i + 1, page);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            page = page_of(i + 2);
             asm volatile("cp.async.wait_group 1;" ::: "memory");
             __syncwarp();
             const uint32_t tile = ring + (i % FEW_STAGES) * TILE;
@@ -259,6 +266,10 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
                     }
                 }
             }
+            __syncwarp();                                           // every lane is done with the stage that is refilled now
+            issue(i + 2, page);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            page = page_of(sg, i + 3);
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
@@ -323,7 +334,7 @@ static int few_go(jl_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
     const int smem = FewTile<D>::SMEM, grid = ctx->sm_count * ATTN_FEW_CTAS;
     auto kern = attn_few_kernel<D, BF16>;
     if (smem > 48 * 1024) JL_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const cudaError_t e = attn_launch_pdl(kern, dim3(grid), dim3(128), smem, s, a, 2);
+    const cudaError_t e = attn_launch_pdl(kern, dim3(grid), dim3(128), smem, s, a, FEW_MIN_UNITS);
     JL_CUDA(ctx, e);
     ctx->st.launches++;
     return attn_launch_merge(ctx, a, ATTN_FEW_ROWS, grid, s);

@@ -17,8 +17,6 @@
 #include "attn.cuh"
 #include "tc5.cuh"
 
-#include <type_traits>
-
 #define TA_UNIT_SHIFT 7
 #define TA_KV 128                        // positions of a unit
 #define TA_WARPS 12                      // 0-3, 4-7 softmax of tile 0, 1; then
@@ -33,9 +31,6 @@
 #define TA_STATUS_CODE 7
 #define TA_ITEM_COST 4
 #define TA_LIMIT 16384.f                 // of a tile's sum of weights: f16 holds each
-#ifndef TA_POLY
-#define TA_POLY 0  // pairs of 16 whose exponentials run on the FMA pipe
-#endif
 
 
 // The bounded wait of this kernel's roles. A try that may sleep for up to 20 us: the warps that wait are many, and their polling would take
@@ -145,45 +140,6 @@ __device__ __forceinline__ float ta_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-// 2^x of two values on the FMA pipe, for x up to 2^7: x = n + f with n the nearest whole number (the low bits of x + 1.5 2^23), 2^f by
-// a polynomial with the least largest relative error on [-1/2, 1/2] (Remez exchange; 7.5e-5 at degree 3, 2.7e-6 at degree 4: a fiftieth
-// and a hundred-and-eightieth of half a unit of the bf16 or f16 that the result is rounded to), n added to the exponent. What lies below
-// 2^-125 comes out as about that, what lies above 2^127 and NaN as something above 2^126 or NaN.
-template <int DEG>
-__device__ __forceinline__ void ta_exp2_poly(float &x0, float &x1) {
-    constexpr float C3[5] = {0.999928057f, 0.693260968f, 0.242611125f, 0.0551716685f, 0.f};
-    constexpr float C4[5] = {0.999999285f, 0.693121791f, 0.240247443f, 0.0559178591f, 0.00957010221f};
-    const float a0 = fminf(ta_max(x0, -125.f), 127.f), a1 = fminf(ta_max(x1, -125.f), 127.f);
-    float t0, t1, f0, f1, p0, p1;
-    asm("{\n\t.reg .b64 x, m, t, f, p, c;\n\t"
-        "mov.b64 x, {%6, %7};\n\t"
-        "mov.b64 m, {%8, %8};\n\t"
-        "add.rn.f32x2 t, x, m;\n\t"
-        "mov.b64 {%0, %1}, t;\n\t"
-        "sub.rn.f32x2 f, t, m;\n\t"
-        "sub.rn.f32x2 f, x, f;\n\t"
-        "mov.b64 {%2, %3}, f;\n\t"
-        "mov.b64 p, {%9, %9};\n\t"
-        "mov.b64 c, {%10, %10};\n\t"
-        "fma.rn.f32x2 p, p, f, c;\n\t"
-        "mov.b64 {%4, %5}, p;\n\t}"
-        : "=f"(t0), "=f"(t1), "=f"(f0), "=f"(f1), "=f"(p0), "=f"(p1)
-        : "f"(a0), "f"(a1), "f"(12582912.f), "f"(DEG == 3 ? C3[3] : C4[4]), "f"(DEG == 3 ? C3[2] : C4[3]));
-#pragma unroll
-    for (int i = DEG - 2; i >= 0; --i) {
-        const float c = DEG == 3 ? C3[i] : C4[i];
-        asm("{\n\t.reg .b64 p, f, c;\n\t"
-            "mov.b64 p, {%0, %1};\n\t"
-            "mov.b64 f, {%2, %3};\n\t"
-            "mov.b64 c, {%4, %4};\n\t"
-            "fma.rn.f32x2 p, p, f, c;\n\t"
-            "mov.b64 {%0, %1}, p;\n\t}"
-            : "+f"(p0), "+f"(p1)
-            : "f"(f0), "f"(f1), "f"(c));
-    }
-    x0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-    x1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 template <bool BF16> __device__ __forceinline__ uint32_t ta_pack(float x, float y) {
     if constexpr (BF16) {
@@ -598,19 +554,13 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 const int n = seen - j * TA_KV;                      // positions of the tile that the row sees
                 const bool masked = (j + 1) * TA_KV > all_seen;
                 // 32 positions' weights, packed, and (HILO) what the packing left; their sum
-                auto weights = [&](auto poly, const uint32_t (&v)[32], float mc, float (&sum)[2][2], uint32_t (&hi)[16], uint32_t (&lo)[16]) {
-                    constexpr int POLY = HILO ? 0 : decltype(poly)::value;
+                auto weights = [&](const uint32_t (&v)[32], float mc, float (&sum)[2][2], uint32_t (&hi)[16], uint32_t (&lo)[16]) {
 #pragma unroll
                     for (int y = 0; y < 16; ++y) {
                         float u, w;
                         tc5_fma2(u, w, __uint_as_float(v[2 * y]), __uint_as_float(v[2 * y + 1]), c, mc);
-                        // some of the exponentials on the FMA pipe
-                        if ((y * POLY) % 16 < POLY) {
-                            ta_exp2_poly<BF16 ? 3 : 4>(u, w);
-                        } else {
-                            u = ta_exp2(u);
-                            w = ta_exp2(w);
-                        }
+                        u = ta_exp2(u);
+                        w = ta_exp2(w);
                         ta_add2(sum[y & 1], u, w);
                         hi[y] = ta_pack<BF16>(u, w);
                         if constexpr (HILO) {
@@ -620,6 +570,16 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     }
                 };
                 bool slow = masked;
+                if (j == 0 && !masked) {                             // any of a row's scores may be the first reference
+                    uint32_t v[16];
+                    tc5_ld16(S, v);
+                    ta_wait_ld(v);
+                    float top[2] = {__uint_as_float(v[0]), __uint_as_float(v[1])};
+#pragma unroll
+                    for (int y = 2; y < 16; ++y) top[y & 1] = fmaxf(top[y & 1], __uint_as_float(v[y]));
+                    m = fmaxf(top[0], top[1]);
+                    if (!(m < INFINITY)) m = 0.f;                    // the sum tells of NaN and +inf
+                }
                 if (!slow) {
                     uint32_t s[4][32], hi[4][16], lo[HILO ? 4 : 1][16];
                     float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
@@ -627,15 +587,9 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     for (int x = 0; x < 4; ++x) tc5_ld32(S + 32 * x, s[x]);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) ta_wait_ld(s[x]);
-                    if (j == 0) {                                    // any of the row's scores may be the first reference
-                        float top = __uint_as_float(s[0][0]);
-#pragma unroll
-                        for (int y = 1; y < 32; ++y) top = fmaxf(top, __uint_as_float(s[0][y]));
-                        m = top < INFINITY ? top : 0.f;              // the sum tells of NaN and +inf
-                    }
                     const float mc = m == -INFINITY ? 0.f : -m * c;
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) weights(std::integral_constant<int, TA_POLY>(), s[x], mc, sum, hi[x], lo[HILO ? x : 0]);
+                    for (int x = 0; x < 4; ++x) weights(s[x], mc, sum, hi[x], lo[HILO ? x : 0]);
                     const float total = (sum[0][0] + sum[1][0]) + (sum[0][1] + sum[1][1]);
                     slow = __any_sync(0xffffffffu, live && m == m && (!(total <= TA_LIMIT) || (m == -INFINITY && total > 0.f)));
                     if (!slow) {
@@ -683,7 +637,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
 #pragma unroll
                         for (int y = 0; y < 32; ++y)
                             if (32 * x + y >= n) v[y] = 0xFF800000u;
-                        weights(std::integral_constant<int, 0>(), v, mc, sum, hi, lo);
+                        weights(v, mc, sum, hi, lo);
                         ta_st16(S + 32 * x, hi);
                         if constexpr (HILO) ta_st16(S + 32 * x + 16, lo);
                     }
