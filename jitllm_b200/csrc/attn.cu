@@ -85,9 +85,9 @@ __global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_const
     attn_merge_store<D>(a, own, r, V * lane, acc, L);
 }
 
-// Few rows and perhaps hundreds of parts: bound by the loads' latency. The eight warps of a block share a row, each a run of its parts with
-// eight loads on their way, the runs added in order (131,071 positions of two kv heads, 222 parts to a row: 150 us with one warp and one
-// part at a time). Most CTAs begin no such item: a block looks over its share of the (CTA, row) pairs in one load and works on those there are.
+// Few rows: block (c, y) takes rows y, y + 4, ... of the item. A handful of parts: a warp to a row. Hundreds (a long sequence): bound by the
+// loads' latency, so the eight warps share a row, each a run of its parts with eight loads on their way, the runs added in order
+// (131,071 positions of two kv heads, 222 parts to a row: 150 us with one warp and one part at a time).
 template <int ROWS, int D>
 __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_constant__ AttnArgs a, int ctas) {
     constexpr int V = D / 32;
@@ -95,59 +95,58 @@ __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_consta
     __shared__ float tops[8];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const AttnMeta own = a.meta[c];
+    const int rows = own.ntok * a.g;
+    if (!own.own || (int)blockIdx.y >= rows) return;
+    const int n = attn_item_end(a.meta, c, ctas) - c + 1;
     const size_t slot = attn_slot_floats(ROWS, D);
-    for (int s0 = blockIdx.x; s0 < ctas * ROWS; s0 += 32 * gridDim.x) {
-        const int mine = s0 + lane * (int)gridDim.x;
-        bool is = mine < ctas * ROWS;
-        if (is) {
-            const AttnMeta &m = a.meta[mine / ROWS];
-            is = m.own && mine % ROWS < m.ntok * a.g;
-        }
-        for (unsigned todo = __ballot_sync(0xffffffffu, is); todo; todo &= todo - 1) {
-            const int pick = s0 + (__ffs(todo) - 1) * (int)gridDim.x, c = pick / ROWS, r = pick % ROWS;
-            const AttnMeta own = a.meta[c];
-            const int n = attn_item_end(a.meta, c, ctas) - c + 1, lo = c + n * warp / 8, hi = c + n * (warp + 1) / 8;
-            auto part_of = [&](int i) { return a.part + ((size_t)i * 2 + (i == c)) * slot; };
-            auto there = [&](int i) { return i == c || a.meta[i].cont; };
-            float M = -INFINITY;
-            for (int i = lo + lane; i < hi; i += 32)
-                if (there(i)) M = fmaxf(M, __ldcg(part_of(i) + ROWS * D + r));
+    const bool together = n > 16;
+    auto part_of = [&](int i) { return a.part + ((size_t)i * 2 + (i == c)) * slot; };
+    auto there = [&](int i) { return i == c || a.meta[i].cont; };
+    for (int r = blockIdx.y + (together ? 0 : 4 * warp); r < rows; r += together ? 4 : 32) {
+        const int lo = together ? c + n * warp / 8 : c, hi = together ? c + n * (warp + 1) / 8 : c + n;
+        float M = -INFINITY;
+        for (int i = lo + lane; i < hi; i += 32)
+            if (there(i)) M = fmaxf(M, __ldcg(part_of(i) + ROWS * D + r));
 #pragma unroll
-            for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        if (together) {
             if (lane == 0) tops[warp] = M;
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 8; ++i) M = fmaxf(M, tops[i]);
-            const float mu = M == -INFINITY ? 0.f : M;
-            float L = 0.f, acc[V] = {};
-            for (int i0 = lo; i0 < hi; i0 += 32) {
-                float w = 0.f, l = 0.f;                           // of part i0 + lane
-                if (i0 + lane < hi && there(i0 + lane)) {
-                    const float *p = part_of(i0 + lane) + ROWS * D + r;
-                    l = __ldcg(p + ROWS);
-                    w = l == 0.f ? 0.f : exp2f(__ldcg(p) - mu);   // a part that holds nothing of the row, perhaps not even numbers
-                }
-                const int cnt = min(32, hi - i0);
-                for (int k0 = 0; k0 < cnt; k0 += 8) {
-                    float v[8][V], wk[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        wk[k] = __shfl_sync(0xffffffffu, w, (k0 + k) & 31);
-                        const float lk = __shfl_sync(0xffffffffu, l, (k0 + k) & 31);
-                        const bool use = k0 + k < cnt && lk != 0.f;
-                        if (use) L = fmaf(wk[k], lk, L);
-                        else wk[k] = 0.f;
-#pragma unroll
-                        for (int x = 0; x < V; ++x) v[k][x] = 0.f;
-                        if (use) attn_merge_load<D>(part_of(i0 + k0 + k) + (size_t)r * D + V * lane, v[k]);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-#pragma unroll
-                        for (int x = 0; x < V; ++x) acc[x] = fmaf(wk[k], v[k][x], acc[x]);
-                }
+        }
+        const float mu = M == -INFINITY ? 0.f : M;
+        float L = 0.f, acc[V] = {};
+        for (int i0 = lo; i0 < hi; i0 += 32) {
+            float w = 0.f, l = 0.f;                               // of part i0 + lane
+            if (i0 + lane < hi && there(i0 + lane)) {
+                const float *p = part_of(i0 + lane) + ROWS * D + r;
+                l = __ldcg(p + ROWS);
+                w = l == 0.f ? 0.f : exp2f(__ldcg(p) - mu);       // a part that holds nothing of the row, perhaps not even numbers
             }
+            const int cnt = min(32, hi - i0);
+            for (int k0 = 0; k0 < cnt; k0 += 8) {
+                float v[8][V], wk[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    wk[k] = __shfl_sync(0xffffffffu, w, (k0 + k) & 31);
+                    const float lk = __shfl_sync(0xffffffffu, l, (k0 + k) & 31);
+                    const bool use = k0 + k < cnt && lk != 0.f;
+                    if (use) L = fmaf(wk[k], lk, L);
+                    else wk[k] = 0.f;
+#pragma unroll
+                    for (int x = 0; x < V; ++x) v[k][x] = 0.f;
+                    if (use) attn_merge_load<D>(part_of(i0 + k0 + k) + (size_t)r * D + V * lane, v[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+#pragma unroll
+                    for (int x = 0; x < V; ++x) acc[x] = fmaf(wk[k], v[k][x], acc[x]);
+            }
+        }
+        if (together) {
 #pragma unroll
             for (int x = 0; x < V; ++x) sums[warp][V * lane + x] = acc[x];
             if (lane == 0) sums[warp][D] = L;
@@ -159,15 +158,15 @@ __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_consta
                     for (int x = 0; x < V; ++x) acc[x] += sums[i][V * lane + x];
                     L += sums[i][D];
                 }
-                attn_merge_store<D>(a, own, r, V * lane, acc, L);
             }
-            __syncthreads();                                      // sums and tops are read
         }
+        if (!together || warp == 0) attn_merge_store<D>(a, own, r, V * lane, acc, L);
+        if (together) __syncthreads();                            // sums and tops are read
     }
 }
 
 int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s) {
-    const dim3 few(ctas * ATTN_FEW_ROWS < ctx->sm_count * 8 ? ctas * ATTN_FEW_ROWS : ctx->sm_count * 8), many(ctas, ATTN_TC_ROWS / 8);
+    const dim3 few(ctas, 4), many(ctas, ATTN_TC_ROWS / 8);
     const cudaError_t e = rows == ATTN_FEW_ROWS
         ? (a.d == 128 ? attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 128>, few, dim3(256), 0, s, a, ctas)
                       : attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 64>, few, dim3(256), 0, s, a, ctas))

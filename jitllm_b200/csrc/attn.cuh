@@ -64,6 +64,10 @@ __host__ __device__ static inline int attn_limit(const AttnSeq &q, int t1) {
 
 struct AttnCut { int seq, blk, head, unit; };     // before `unit` of item (seq, blk, head); seq == nseq: the line's end
 
+// a / b of numbers that are not negative: 64-bit division is a long subroutine, and few calls need it.
+__host__ __device__ static inline long long attn_div(long long a, long long b) {
+    return ((a | b) >> 31) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
 __host__ __device__ static inline long long attn_item_weight(const AttnSeq &q, int blk, int T, int cost) {
     const int t1 = (blk + 1) * T < q.n ? (blk + 1) * T : q.n;
     return (long long)cost + (q.pos0 > 0 ? q.pos0 : 0) + t1;
@@ -89,7 +93,7 @@ __host__ __device__ static inline AttnCut attn_cut_in(const AttnArgs &a, int s, 
     x -= attn_blocks_weight(q, lo, T, cost) * a.hkv;
     const long long w = attn_item_weight(q, lo, T, cost);
     AttnCut c;
-    c.seq = s; c.blk = lo; c.head = (int)(x / w);
+    c.seq = s; c.blk = lo; c.head = (int)attn_div(x, w);
     x -= c.head * w;
     const int t1 = (lo + 1) * T < q.n ? (lo + 1) * T : q.n;
     const int units = (attn_limit(q, t1) + (1 << unit_shift) - 1) >> unit_shift;
@@ -153,12 +157,12 @@ __host__ __device__ static inline long long attn_seq_weight(const AttnArgs &a, c
 // end a cut snaps onto it. False: the CTA has no share.
 __host__ __device__ static inline bool attn_cuts(long long total, int cta, int grid, int unit_shift, int min_units, long long &b0,
                                                  long long &b1, int &snap) {
-    long long ctas = total / ((long long)min_units << unit_shift);
+    long long ctas = attn_div(total, (long long)min_units << unit_shift);
     ctas = ctas < 1 ? 1 : (ctas > grid ? grid : ctas);
     if (total == 0 || cta >= ctas) return false;
-    const long long share = total / ctas, rest = total % ctas;        // total * cta may pass 63 bits
-    b0 = share * cta + rest * cta / ctas;
-    b1 = share * (cta + 1) + rest * (cta + 1) / ctas;
+    const long long share = attn_div(total, ctas), rest = total - share * ctas;       // total * cta may pass 63 bits
+    b0 = share * cta + attn_div(rest * cta, ctas);
+    b1 = share * (cta + 1) + attn_div(rest * (cta + 1), ctas);
     const long long quarter = share >> (unit_shift + 2);
     snap = quarter < ATTN_SNAP ? (int)quarter : ATTN_SNAP;
     return true;

@@ -59,6 +59,24 @@ def _dtype_code(a) -> int:
     raise ValueError(f"unsupported element type {a.dtype}")
 
 
+_TORCH, _CODES = None, {}
+
+
+def _torch():
+    global _TORCH
+    if _TORCH is None:
+        import torch
+        _TORCH = torch
+        _CODES.update({torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16})
+    return _TORCH
+
+
+def _tensor_code(t) -> int:
+    """_dtype_code of a torch tensor, without the text."""
+    code = _CODES.get(t.dtype)
+    return _dtype_code(t) if code is None else code
+
+
 class Weight:
     """A weight (or expert bank) resident on the device: jl_weight."""
 
@@ -179,6 +197,7 @@ class PagedKV:
         self.desc = PagedKVDesc(struct_size=C.sizeof(PagedKVDesc), dtype=code, n_kv=self.n_kv, head_dim=self.head_dim,
                                 page_len=self.page_len, n_pages=self.n_pages, n_seq=self.n_seq, max_pages=self.max_pages, k=_ptr(k),
                                 v=_ptr(v), page_table=_ptr(table))
+        self.ref = C.byref(self.desc)
 
 
 class Device:
@@ -390,22 +409,21 @@ class Device:
         q [total][hq][d], k and v [total][hkv][d], f16 or bf16, views with any token and head stride; query head h reads kv head
         h // (hq // hkv). out [total][hq][d], f32, f16 or bf16; rows behind the last sequence are left as they were. scale: None
         for 1 / sqrt(d)."""
-        total, hq, d = self._heads("q", q)
-        if k.shape != v.shape or self._heads("k", k)[::2] != (total, d) or self._heads("v", v)[::2] != (total, d):
-            raise ValueError("q, k and v must be [total][heads][d] with one total and one d, k and v of one shape")
-        if self._strides(k) != self._strides(v):
-            raise ValueError("k and v must have the same strides")
+        total, hq, d, qt, qh = self._heads("q", q)
+        kn, hkv, kd, kt, kh = self._heads("k", k)
+        if self._heads("v", v) != (total, hkv, d, kt, kh) or kn != total or kd != d:
+            raise ValueError("q, k and v must be [total][heads][d] with one total and one d, k and v of one shape and strides")
         if not q.dtype == k.dtype == v.dtype:
             raise ValueError("q, k and v must be of one type")
         self._seqs("starts", starts)
-        self._out(out, (total, hq, d))
+        self._out(out, q)
         self._on_device(out, q, k, v, starts, scratch)
-        if starts.numel() < 2 or total == 0:
+        nseq = starts.shape[0] - 1
+        if nseq < 1 or total == 0:
             return
-        self._check(self.lib.jl_attn_prompt(self.ctx, _ptr(out), _dtype_code(out), q.data_ptr(), *self._strides(q), k.data_ptr(),
-                                            v.data_ptr(), *self._strides(k), _dtype_code(q), _ptr(starts), starts.numel() - 1,
-                                            total, hq, k.shape[1], d, d ** -0.5 if scale is None else scale, _ptr(scratch),
-                                            _nbytes(scratch), stream))
+        self._check(self.lib.jl_attn_prompt(self.ctx, out.data_ptr(), _tensor_code(out), q.data_ptr(), qt, qh, k.data_ptr(), v.data_ptr(), kt,
+                                            kh, _tensor_code(q), _ptr(starts), nseq, total, hq, hkv, d, d ** -0.5 if scale is None else scale,
+                                            _ptr(scratch), scratch.numel() * scratch.element_size(), stream))
 
     def AttnPaged(self, out, q, kv: PagedKV, starts, lens, scratch, max_new: int | None = None, scale: float | None = None,
                   stream: int = 0) -> None:
@@ -413,63 +431,66 @@ class Device:
         lens[s] - n + i (its key and value are in the cache already: RopeAppend). starts int32 [n_seq + 1] and lens int32 [n_seq] are
         device tensors; q, out, scratch and scale as in AttnPrompt. max_new: the most new rows of any sequence, as far as the caller
         knows; it picks the kernel, not the result (None: all rows may be one sequence's)."""
-        total, hq, d = self._heads("q", q)
+        total, hq, d, qt, qh = self._heads("q", q)
         if d != kv.head_dim or q.dtype != kv.k.dtype:
             raise ValueError("q must have the cache's head size and type")
         self._seqs("starts", starts, kv.n_seq + 1)
         self._seqs("lens", lens, kv.n_seq)
-        self._out(out, (total, hq, d))
+        self._out(out, q)
         self._on_device(out, q, kv.k, starts, lens, scratch)
         if kv.n_seq == 0 or total == 0:
             return
-        self._check(self.lib.jl_attn_paged(self.ctx, _ptr(out), _dtype_code(out), q.data_ptr(), *self._strides(q), C.byref(kv.desc),
-                                           _ptr(starts), _ptr(lens), total, total if max_new is None else max_new, hq,
-                                           d ** -0.5 if scale is None else scale, _ptr(scratch), _nbytes(scratch), stream))
+        self._check(self.lib.jl_attn_paged(self.ctx, out.data_ptr(), _tensor_code(out), q.data_ptr(), qt, qh, kv.ref, _ptr(starts), _ptr(lens),
+                                           total, total if max_new is None else max_new, hq, d ** -0.5 if scale is None else scale,
+                                           _ptr(scratch), scratch.numel() * scratch.element_size(), stream))
 
     def RopeAppend(self, q_out, qkv, kv: PagedKV, starts, lens, cos, sin, stream: int = 0) -> None:
         """The cache's writer: rows of qkv [total][(hq + 2 n_kv) * d] (f32, f16 or bf16) are the sequences' new rows, at the positions
         that AttnPaged gives them. q_out [total][hq][d] of the cache's type gets q rotated; k (rotated) and v go to their pages.
         cos, sin: f32 [positions][d / 2], adjacent-pair rotation. Rows at positions outside the tables are left out."""
-        total, hq, d = self._heads("q_out", q_out)
+        total, hq, d, _, _ = self._heads("q_out", q_out)
         if d != kv.head_dim or q_out.dtype != kv.k.dtype or not q_out.is_contiguous():
             raise ValueError("q_out must be contiguous and have the cache's head size and type")
-        if tuple(qkv.shape) != (total, (hq + 2 * kv.n_kv) * d):
+        if qkv.shape != (total, (hq + 2 * kv.n_kv) * d):
             raise ValueError("qkv must be [total][(hq + 2 n_kv) * d]")
-        for name, tab in (("cos", cos), ("sin", sin)):
-            if tab.dim() != 2 or tab.shape != cos.shape or tab.shape[1] * 2 != d or _dtype_code(tab) != _lib.DT_F32:
-                raise ValueError(f"{name} must be f32 [positions][d / 2]")
+        if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] * 2 != d or _tensor_code(cos) or _tensor_code(sin):
+            raise ValueError("cos and sin must be f32 [positions][d / 2]")
         self._seqs("starts", starts, kv.n_seq + 1)
         self._seqs("lens", lens, kv.n_seq)
         self._on_device(q_out, qkv, kv.k, starts, lens, cos, sin)
         if kv.n_seq == 0 or total == 0:
             return
-        self._check(self.lib.jl_rope_append(self.ctx, _ptr(q_out), _ptr(qkv), _dtype_code(qkv), C.byref(kv.desc), _ptr(starts), _ptr(lens),
-                                            total, hq, _ptr(cos), _ptr(sin), cos.shape[0], stream))
+        self._check(self.lib.jl_rope_append(self.ctx, q_out.data_ptr(), _ptr(qkv), _tensor_code(qkv), kv.ref, _ptr(starts), _ptr(lens), total, hq,
+                                            _ptr(cos), _ptr(sin), cos.shape[0], stream))
 
+    # The checks below run at every call of a decode step: they ask a tensor for as little as they can.
     @staticmethod
     def _heads(name, t):
-        if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
-            raise ValueError(f"{name} must be [total][heads][d], contiguous in d")
-        return tuple(t.shape)
+        """total, heads, d and the token and head strides of a [total][heads][d] view; the stride of a dimension of one, which is
+        never used and may be anything, as if the view were contiguous."""
+        shape = t.shape
+        if len(shape) != 3:
+            raise ValueError(f"{name} must be [total][heads][d]")
+        n, h, d = shape
+        a, b, c = t.stride()
+        if c != 1 and d > 1:
+            raise ValueError(f"{name} must be contiguous in d")
+        return n, h, d, a if n > 1 else h * d, b if h > 1 else d
 
     @staticmethod
-    def _strides(t):
-        """Token and head stride; those of a dimension of one are never used, whatever they say."""
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2], t.stride(1) if t.shape[1] > 1 else t.shape[2]
-
-    @staticmethod
-    def _out(out, shape):
-        if tuple(out.shape) != shape or not out.is_contiguous():
+    def _out(out, q):
+        if out.shape != q.shape or not out.is_contiguous():
             raise ValueError("out must be contiguous [total][hq][d]")
 
     @staticmethod
     def _seqs(name, t, n=None):
-        if t.dim() != 1 or not str(t.dtype).endswith("int32") or (n is not None and t.numel() != n):
+        shape = t.shape
+        if len(shape) != 1 or t.dtype != _torch().int32 or (n is not None and shape[0] != n):
             raise ValueError(f"{name} must be a one-dimensional int32 tensor" + (f" of {n}" if n is not None else ""))
 
     def _on_device(self, *tensors):
         for t in tensors:
-            if t.device.type != "cuda" or t.device.index != self.ordinal:
+            if t.get_device() != self.ordinal:
                 raise ValueError(f"a tensor lies on {t.device}, this Device is GPU {self.ordinal}")
 
     def _check(self, rc: int) -> None:
