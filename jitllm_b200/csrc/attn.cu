@@ -247,14 +247,14 @@ __global__ void __launch_bounds__(256) attn_append_kernel(const __grid_constant_
 namespace {
 // The caller's current device comes back however the call ends.
 struct DeviceGuard {
-    int was;
+    int was, to;
     bool ok;
-    explicit DeviceGuard(int device) : was(-1), ok(false) {
+    explicit DeviceGuard(int device) : was(-1), to(device), ok(false) {
         if (cudaGetDevice(&was) != cudaSuccess) { cudaGetLastError(); was = -1; }
         ok = was == device || cudaSetDevice(device) == cudaSuccess;
         if (!ok) cudaGetLastError();
     }
-    ~DeviceGuard() { if (was >= 0) cudaSetDevice(was); }
+    ~DeviceGuard() { if (was >= 0 && was != to) cudaSetDevice(was); }
 };
 bool off16(const void *p) { return ((uintptr_t)p & 15u) != 0; }
 bool is16(int dtype) { return dtype == JL_DT_F16 || dtype == JL_DT_BF16; }

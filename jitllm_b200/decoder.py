@@ -5,7 +5,8 @@ the steps around them -- RMSNorm, RoPE, the KV cache, attention, SiLU*up, the re
 the greedy argmax -- are neighbours of the path: the prefill runs them as PyTorch ops, a decode
 step runs the library's own short kernels between the matvecs (`decode_step`), and a decode step
 of ONE sequence runs everything as one persistent kernel (`decode_step_block`: the reference's
-LayerDevice seam). Weights are random-init Q4_K blocks of the right shapes (no checkpoint can be fetched);
+LayerDevice seam). Requests of different lengths share a pool of cache pages (`step_paged`), and packed
+prompts are scored without a cache (`score_packed`). Weights are random-init Q4_K blocks of the right shapes (no checkpoint can be fetched);
 q|k|v and gate|up are stored as one row-concatenated matrix each, as the reference's
 `MatVecSegments` fuses them (docs/kernel-inventory.md:83).
 
@@ -186,8 +187,7 @@ class Decoder:
         return of
 
     def _prefill_chain(self, tokens):
-        """The stack over a prompt with one library kernel between two matmuls: the norm and SiLU*up write the GEMM's
-        activation operand where the next matrix takes one (f32 rows otherwise), RoPE fills q and the cache. Returns the last
+        """The stack over a prompt with one library kernel between two matmuls (_chain): RoPE fills q and the cache. Returns the last
         row, or None when a shape has no such form."""
         torch, c, lib = self.torch, self.cfg, self.dev.lib
         import torch.nn.functional as F
@@ -198,47 +198,121 @@ class Decoder:
         if all(op(l[name]) is None for l in self.layers for name in ("qkv", "gu", "down")):
             return None
         st = torch.cuda.current_stream().cuda_stream
+        q = torch.empty(T, self.hq, d, device="cuda", dtype=torch.bfloat16)
 
-        def ok(rc):
-            if rc != 0:
-                raise RuntimeError(f"jl_aux call failed with status {rc}")
+        def attend(li, qkv):
+            kc, vc = self.k_cache[li], self.v_cache[li]
+            self._ok(lib.jl_aux_rope_prefill(q.data_ptr(), qkv.data_ptr(), kc.data_ptr(), vc.data_ptr(), self.cos.data_ptr(),
+                                             self.sin.data_ptr(), T, kc.shape[0], self.hq, self.hkv, d, self.max_len, st))
+            att = F.scaled_dot_product_attention(q.transpose(0, 1)[None], kc[:1, :, :T], vc[:1, :, :T], is_causal=True, enable_gqa=True)
+            return att[0].transpose(0, 1).reshape(T, -1)
+
+        x, delta = self._chain(tokens, op, attend)
+        return x[-1:] + delta[-1:]
+
+    @staticmethod
+    def _ok(rc):
+        if rc != 0:
+            raise RuntimeError(f"jl_aux call failed with status {rc}")
+
+    def _chain(self, tokens, op, attend):
+        """The stack over the rows of `tokens` with one library kernel between two matmuls: the norm and SiLU*up write the GEMM's
+        activation operand where the next matrix takes one (op(w), see _gemm_operands; f32 rows otherwise). attend(li, qkv f32) stores
+        k and v and returns the attention's rows, [n][hq * d] bf16 or f32. Returns the residual rows and what the last block adds to
+        them."""
+        torch, c, lib, ok = self.torch, self.cfg, self.dev.lib, self._ok
+        n = tokens.shape[0]
+        st = torch.cuda.current_stream().cuda_stream
 
         def mm_prepared(w):
-            out = torch.empty(T, w.nrows, device="cuda", dtype=torch.float32)
-            ok(lib.jl_matmul_dev_prepared(self.dev.ctx, out.data_ptr(), 0, w.handle, T, st))
+            out = torch.empty(n, w.nrows, device="cuda", dtype=torch.float32)
+            ok(lib.jl_matmul_dev_prepared(self.dev.ctx, out.data_ptr(), 0, w.handle, n, st))
             return out
 
         def norm_mm(delta, w):
             dp = delta.data_ptr() if delta is not None else None
             if op(w) is not None:
-                ok(lib.jl_aux_add_rmsnorm_gemm(x.data_ptr(), dp, self.norm_w.data_ptr(), c.eps, *op(w), T, c.hidden, st))
+                ok(lib.jl_aux_add_rmsnorm_gemm(x.data_ptr(), dp, self.norm_w.data_ptr(), c.eps, *op(w), n, c.hidden, st))
                 return mm_prepared(w)
             h = torch.empty_like(x)
-            ok(lib.jl_aux_add_rmsnorm(x.data_ptr(), dp, self.norm_w.data_ptr(), c.eps, h.data_ptr(), None, T, c.hidden, st))
+            ok(lib.jl_aux_add_rmsnorm(x.data_ptr(), dp, self.norm_w.data_ptr(), c.eps, h.data_ptr(), None, n, c.hidden, st))
             return self.mm(w, h)
 
         x = self.emb[tokens].float()
-        q = torch.empty(T, self.hq, d, device="cuda", dtype=torch.bfloat16)
         delta = None
         for li, l in enumerate(self.layers):
-            kc, vc = self.k_cache[li], self.v_cache[li]
-            qkv = norm_mm(delta, l["qkv"])
-            ok(lib.jl_aux_rope_prefill(q.data_ptr(), qkv.data_ptr(), kc.data_ptr(), vc.data_ptr(), self.cos.data_ptr(),
-                                       self.sin.data_ptr(), T, kc.shape[0], self.hq, self.hkv, d, self.max_len, st))
-            att = F.scaled_dot_product_attention(q.transpose(0, 1)[None], kc[:1, :, :T], vc[:1, :, :T], is_causal=True, enable_gqa=True)
-            att = att[0].transpose(0, 1).reshape(T, -1)
+            att = attend(li, norm_mm(delta, l["qkv"]))
             # the GEMM takes the attention's bf16 rows as they are (each is its own high half: the low half of the f32 form is
             # zero); the row kernels take f32
             delta = self._allreduce(self.mm(l["o"], att if op(l["o"]) is not None else att.float()))
             gu = norm_mm(delta, l["gu"])
             if op(l["down"]) is not None:
-                ok(lib.jl_aux_silu_mul_gemm(*op(l["down"]), gu.data_ptr(), T, self.ffn_l, st))
+                ok(lib.jl_aux_silu_mul_gemm(*op(l["down"]), gu.data_ptr(), n, self.ffn_l, st))
                 delta = self._allreduce(mm_prepared(l["down"]))
             else:
-                a = torch.empty(T, self.ffn_l, device="cuda", dtype=torch.float32)
-                ok(lib.jl_aux_silu_mul(a.data_ptr(), None, gu.data_ptr(), T, self.ffn_l, st))
+                a = torch.empty(n, self.ffn_l, device="cuda", dtype=torch.float32)
+                ok(lib.jl_aux_silu_mul(a.data_ptr(), None, gu.data_ptr(), n, self.ffn_l, st))
                 delta = self._allreduce(self.mm(l["down"], a))
-        return x[-1:] + delta[-1:]
+        return x, delta
+
+    # -- several requests at once ---------------------------------------------------
+    def open_pool(self, n_pages: int, page_len: int) -> None:
+        """A pool of cache pages for step_paged, beside the per-sequence caches: every layer has its own pages under the same numbers,
+        so that one page table serves the whole stack. Pages hold a power of two from 16 to 1024 positions."""
+        torch, c = self.torch, self.cfg
+        self.k_pool = torch.zeros(c.n_layer, n_pages, self.hkv, page_len, c.head_dim, device="cuda", dtype=torch.bfloat16)
+        self.v_pool = torch.zeros_like(self.k_pool)
+        self._paged_scratch = torch.empty(self.dev.AttnScratchBytes(), device="cuda", dtype=torch.uint8)
+
+    def _attn_scratch(self):
+        if getattr(self, "_paged_scratch", None) is None:
+            self._paged_scratch = self.torch.empty(self.dev.AttnScratchBytes(), device="cuda", dtype=self.torch.uint8)
+        return self._paged_scratch
+
+    def step_paged(self, tokens, starts, lens, table, max_new: int):
+        """One step of several requests over the pool: prompts, chunks of prompts and single tokens in any mixture. tokens [N] int64:
+        rows starts[s] .. starts[s + 1] - 1 are sequence s's new tokens; lens[s] its positions with them; table [n_seq][max_pages] its
+        pages (int32 device tensors; the caller hands out pages for the new positions beforehand). max_new: the most new tokens of any
+        sequence. Returns the next token of every sequence [n_seq]; that of a sequence without new tokens has no meaning. Allocates
+        nothing but tensors, so that a step of fixed N can be captured and replayed on other lengths and tables."""
+        from .device import PagedKV
+        torch, c = self.torch, self.cfg
+        n, d = tokens.shape[0], c.head_dim
+        st = torch.cuda.current_stream().cuda_stream
+        operands = self._gemm_operands(n)
+        op = operands if n >= 9 and self.ffn_l <= 50 * 1024 else lambda w: None
+        q = torch.empty(n, self.hq, d, device="cuda", dtype=torch.bfloat16)
+        out = torch.empty(n, self.hq, d, device="cuda", dtype=torch.bfloat16 if n >= 9 else torch.float32)
+        scratch = self._attn_scratch()
+
+        def attend(li, qkv):
+            kv = PagedKV(self.k_pool[li], self.v_pool[li], table)
+            self.dev.RopeAppend(q, qkv, kv, starts, lens, self.cos, self.sin, stream=st)
+            self.dev.AttnPaged(out, q, kv, starts, lens, scratch, max_new=max_new, stream=st)
+            return out.view(n, -1)
+
+        x, delta = self._chain(tokens, op, attend)
+        last = (starts[1:] - 1).clamp_min(0).long()
+        return self._argmax((x + delta)[last])
+
+    def score_packed(self, tokens, starts):
+        """The next token after each of several packed prompts, without a cache: tokens [N] int64, prompt s is rows starts[s] ..
+        starts[s + 1] - 1 (int32 device tensor). Returns [n_seq]; that of an empty prompt has no meaning."""
+        torch, c = self.torch, self.cfg
+        n, d = tokens.shape[0], c.head_dim
+        st = torch.cuda.current_stream().cuda_stream
+        row = torch.arange(n, device="cuda", dtype=torch.int32)
+        seq = torch.searchsorted(starts[1:].contiguous(), row, right=True).clamp_max(starts.shape[0] - 2)
+        pos = (row - starts[seq]).long()
+        out = torch.empty(n, self.hq, d, device="cuda", dtype=torch.bfloat16)
+        scratch = self._attn_scratch()
+
+        def attend(li, q, k, v):
+            self.dev.AttnPrompt(out, q, k, v, starts, scratch, stream=st)
+            return out.view(n, -1)
+
+        x = self._layers(self.emb[tokens].float(), pos, attend)
+        return self._argmax(x[(starts[1:] - 1).clamp_min(0).long()])
 
     def decode_step(self, tokens, pos_dev):
         """tokens [B] int64, one per sequence, all at position pos_dev (a 1-element int64 DEVICE tensor,
