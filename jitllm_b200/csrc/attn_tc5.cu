@@ -602,14 +602,20 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     }
                 }
                 if (slow) {
-                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                    for (int x = 0; x < 4; ++x) {
-                        uint32_t v[32];
-                        tc5_ld32(S + 32 * x, v);
-                        ta_wait_ld(v);
+                    uint32_t s[4][32];
 #pragma unroll
-                        for (int y = 0; y < 32; ++y) tops[y & 3] = ta_max(tops[y & 3], 32 * x + y < n ? __uint_as_float(v[y]) : -INFINITY);
+                    for (int x = 0; x < 4; ++x) tc5_ld32(S + 32 * x, s[x]);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) ta_wait_ld(s[x]);
+                    float tops[4];
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+#pragma unroll
+                        for (int y = 0; y < 32; ++y)
+                            if (32 * x + y >= n) s[x][y] = 0xFF800000u;
+                        tops[x] = __uint_as_float(s[x][0]);
+#pragma unroll
+                        for (int y = 1; y < 32; ++y) tops[x] = ta_max(tops[x], __uint_as_float(s[x][y]));
                     }
                     const float top = ta_max(ta_max(tops[0], tops[1]), ta_max(tops[2], tops[3]));      // of the row; m, l and O go up to it
                     const float next = ta_max(m, top);               // NaN stays
@@ -629,15 +635,10 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     }
                     const float mc = m == -INFINITY ? 0.f : -m * c;
                     float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-#pragma unroll 1
-                    for (int x = 0; x < 4; ++x) {
-                        uint32_t v[32], hi[16], lo[16];
-                        tc5_ld32(S + 32 * x, v);
-                        ta_wait_ld(v);
 #pragma unroll
-                        for (int y = 0; y < 32; ++y)
-                            if (32 * x + y >= n) v[y] = 0xFF800000u;
-                        weights(v, mc, sum, hi, lo);
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t hi[16], lo[16];
+                        weights(s[x], mc, sum, hi, lo);
                         ta_st16(S + 32 * x, hi);
                         if constexpr (HILO) ta_st16(S + 32 * x + 16, lo);
                     }
