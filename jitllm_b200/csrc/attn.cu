@@ -46,8 +46,8 @@ __device__ __forceinline__ void attn_merge_load(const float *p, float (&v)[D / 3
 
 // Many rows and, as a rule, few parts: block (c, y) takes eight rows, a warp each. Bound by the parts' bytes, which come from L2: small
 // warps, many of them.
-template <int ROWS, int D>
-__global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_constant__ AttnArgs a, int ctas) {
+template <int D>
+__global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_constant__ AttnArgs a, int ctas, int slot_rows) {
     constexpr int V = D / 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -55,10 +55,10 @@ __global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_const
     const AttnMeta own = a.meta[c];
     if (!own.own || r >= own.ntok * a.g) return;
     const int end = attn_item_end(a.meta, c, ctas);
-    const size_t slot = attn_slot_floats(ROWS, D);
+    const size_t slot = attn_slot_floats(slot_rows, D);
     float M = -INFINITY;
     for (int i = c + lane; i <= end; i += 32)
-        if (i == c || a.meta[i].cont) M = fmaxf(M, __ldcg(a.part + ((size_t)i * 2 + (i == c)) * slot + ROWS * D + r));
+        if (i == c || a.meta[i].cont) M = fmaxf(M, __ldcg(a.part + ((size_t)i * 2 + (i == c)) * slot + slot_rows * D + r));
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float mu = M == -INFINITY ? 0.f : M;
@@ -66,9 +66,9 @@ __global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_const
     for (int i0 = c; i0 <= end; i0 += 32) {
         float w = 0.f, l = 0.f;                                   // of part i0 + lane
         if (i0 + lane <= end && (i0 + lane == c || a.meta[i0 + lane].cont)) {
-            const float *p = a.part + ((size_t)(i0 + lane) * 2 + (i0 + lane == c)) * slot + ROWS * D + r;
+            const float *p = a.part + ((size_t)(i0 + lane) * 2 + (i0 + lane == c)) * slot + slot_rows * D + r;
             w = exp2f(__ldcg(p) - mu);
-            l = __ldcg(p + ROWS);
+            l = __ldcg(p + slot_rows);
         }
         const int cnt = min(32, end - i0 + 1);
 #pragma unroll 4
@@ -166,12 +166,12 @@ __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_consta
 }
 
 int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s) {
-    const dim3 few(ctas, 4), many(ctas, ATTN_TC_ROWS / 8);
+    const dim3 few(ctas, 4), many(ctas, rows / 8);
     const cudaError_t e = rows == ATTN_FEW_ROWS
         ? (a.d == 128 ? attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 128>, few, dim3(256), 0, s, a, ctas)
                       : attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 64>, few, dim3(256), 0, s, a, ctas))
-        : (a.d == 128 ? attn_launch_pdl(attn_merge_many_kernel<ATTN_TC_ROWS, 128>, many, dim3(256), 0, s, a, ctas)
-                      : attn_launch_pdl(attn_merge_many_kernel<ATTN_TC_ROWS, 64>, many, dim3(256), 0, s, a, ctas));
+        : (a.d == 128 ? attn_launch_pdl(attn_merge_many_kernel<128>, many, dim3(256), 0, s, a, ctas, rows)
+                      : attn_launch_pdl(attn_merge_many_kernel<64>, many, dim3(256), 0, s, a, ctas, rows));
     JL_CUDA(ctx, e);
     ctx->st.launches++;
     return JL_OK;
@@ -293,7 +293,7 @@ int attn_launch(jl_ctx *ctx, AttnArgs a, int dtype, long long max_new, bool mixe
         a.row_lo = a.row_hi;
         a.row_hi = INT_MAX;
     }
-    const int rc = attn_launch_tc5(ctx, a, dtype, s);
+    const int rc = attn_launch_tc5(ctx, a, dtype, max_new * a.g, s);
     return rc == JL_DECLINED ? attn_launch_few(ctx, a, dtype, s) : rc;
 }
 
@@ -418,7 +418,7 @@ JL_EXPORT int jl_test_attn_share(const int32_t *starts, const int32_t *lens, int
     a.starts = starts; a.lens = lens; a.nseq = nseq; a.total = total; a.hkv = hkv; a.tok_item = tok_item;
     a.table = max_pages > 0 ? starts : nullptr;       // only its presence matters here
     a.page_shift = page_shift; a.max_pages = max_pages;
-    a.g = 1; a.row_hi = INT_MAX; a.item_cost = 1;
+    a.g = 1; a.row_hi = INT_MAX; a.item_cost = 1; a.snap = 2;
     AttnCut first, last;
     attn_share_host(a, cta, grid, unit_shift, min_units, first, last);
     AttnWalk w;

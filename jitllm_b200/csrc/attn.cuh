@@ -21,7 +21,7 @@ struct AttnArgs {
     int page_shift, n_pages, max_pages;
     int row_lo, row_hi;          // the launch takes the sequences with row_lo < new rows * g <= row_hi
     int tok_item;                // tokens of one item
-    int item_cost;               // what an item's start and end take, in units
+    int item_cost, snap;         // units: what an item's start and end take; cuts nearer than this to its end move onto it
     int out_dtype;
     float scale_log2;            // scale * log2(e): softmax is taken to the base 2
 };
@@ -60,7 +60,6 @@ __host__ __device__ static inline int attn_limit(const AttnSeq &q, int t1) {
 // the cuts rounded to whole units of positions inside an item; an item that a cut divides leaves a partial result in each CTA,
 // and attn_merge_kernel joins them in ascending order of positions. A few long sequences thus fill the GPU as well as many short
 // ones, whatever the lengths, which only the device knows; results depend on the cuts in their rounding and on nothing else.
-#define ATTN_SNAP 2              // units: cuts nearer than this to an item's end move onto it, if the shares are long
 
 struct AttnCut { int seq, blk, head, unit; };     // before `unit` of item (seq, blk, head); seq == nseq: the line's end
 
@@ -155,7 +154,7 @@ __host__ __device__ static inline long long attn_seq_weight(const AttnArgs &a, c
 }
 // The shares of a line of `total`: how many there are (each min_units units at least), where share `cta` lies, and how near an item's
 // end a cut snaps onto it. False: the CTA has no share.
-__host__ __device__ static inline bool attn_cuts(long long total, int cta, int grid, int unit_shift, int min_units, long long &b0,
+__host__ __device__ static inline bool attn_cuts(long long total, int cta, int grid, int unit_shift, int min_units, int most, long long &b0,
                                                  long long &b1, int &snap) {
     long long ctas = attn_div(total, (long long)min_units << unit_shift);
     ctas = ctas < 1 ? 1 : (ctas > grid ? grid : ctas);
@@ -164,7 +163,7 @@ __host__ __device__ static inline bool attn_cuts(long long total, int cta, int g
     b0 = share * cta + attn_div(rest * cta, ctas);
     b1 = share * (cta + 1) + attn_div(rest * (cta + 1), ctas);
     const long long quarter = share >> (unit_shift + 2);
-    snap = quarter < ATTN_SNAP ? (int)quarter : ATTN_SNAP;
+    snap = quarter < most ? (int)quarter : most;
     return true;
 }
 static inline void attn_share_host(const AttnArgs &a, int cta, int grid, int unit_shift, int min_units, AttnCut &first, AttnCut &last) {
@@ -172,7 +171,7 @@ static inline void attn_share_host(const AttnArgs &a, int cta, int grid, int uni
     int snap;
     for (int s = 0; s < a.nseq; ++s) total += attn_seq_weight(a, attn_seq(a, s), unit_shift);
     first = last = AttnCut{a.nseq, 0, 0, 0};
-    if (!attn_cuts(total, cta, grid, unit_shift, min_units, b0, b1, snap)) return;
+    if (!attn_cuts(total, cta, grid, unit_shift, min_units, a.snap, b0, b1, snap)) return;
     for (int s = 0; s < a.nseq; ++s) {
         const AttnSeq q = attn_seq(a, s);
         const long long w = attn_seq_weight(a, q, unit_shift);
@@ -205,7 +204,7 @@ __device__ static inline void attn_share(const AttnArgs &a, int cta, int grid, i
     first.blk = first.head = first.unit = last.blk = last.head = last.unit = 0;
     long long b0, b1, base = 0;
     int snap;
-    if (!attn_cuts(total, cta, grid, unit_shift, min_units, b0, b1, snap)) return;
+    if (!attn_cuts(total, cta, grid, unit_shift, min_units, a.snap, b0, b1, snap)) return;
     auto look = [&](int s0, const AttnSeq &q, long long w) {
         long long upto = w;
 #pragma unroll
@@ -264,7 +263,7 @@ __device__ __forceinline__ void attn_store4(void *out, int dtype, size_t at, flo
 __host__ __device__ static inline size_t attn_slot_floats(int rows, int d) { return (size_t)rows * (d + 2); }
 #define ATTN_FEW_ROWS 16
 #define ATTN_FEW_CTAS 3          // to an SM
-#define ATTN_TC_ROWS 256
+#define ATTN_TC_ROWS 256         // or 128, and twice the CTAs
 
 // Launched so that the next kernel of the stream may be put in place while this one drains.
 template <typename... P, typename... Args>
@@ -279,5 +278,6 @@ static cudaError_t attn_launch_pdl(void (*kern)(P...), dim3 grid, dim3 block, in
 
 // attn_few.cu, attn_tc5.cu, attn.cu
 int attn_launch_few(jl_ctx *ctx, const AttnArgs &a, int dtype, cudaStream_t s);
-int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &a, int dtype, cudaStream_t s);    // JL_DECLINED: no tensor map for these strides
+// max_rows: query rows of a sequence and kv head, at most. JL_DECLINED: no tensor map for these strides
+int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &a, int dtype, long long max_rows, cudaStream_t s);
 int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s);

@@ -11,9 +11,8 @@
 #define FEW_UNIT_SHIFT 6
 #define FEW_STAGES 2
 #define FEW_ITEM_COST 4          // an item's start and end against a unit: 3.7 us, 0.8 us with the GPU full
-#ifndef FEW_MIN_UNITS
+#define FEW_SNAP 2
 #define FEW_MIN_UNITS 2
-#endif
 
 template <int D> struct FewTile {
     static constexpr int ROW = 2 * D + 16;            // bytes of a staged row: padded, so that rows start in different banks
@@ -344,6 +343,7 @@ int attn_launch_few(jl_ctx *ctx, const AttnArgs &args, int dtype, cudaStream_t s
     AttnArgs a = args;
     a.tok_item = ATTN_FEW_ROWS / a.g;
     a.item_cost = FEW_ITEM_COST;
+    a.snap = FEW_SNAP;
     if (a.d == 128) return dtype == JL_DT_BF16 ? few_go<128, true>(ctx, a, s) : few_go<128, false>(ctx, a, s);
     return dtype == JL_DT_BF16 ? few_go<64, true>(ctx, a, s) : few_go<64, false>(ctx, a, s);
 }

@@ -19,17 +19,21 @@
 
 #define TA_UNIT_SHIFT 7
 #define TA_KV 128                        // positions of a unit
-#define TA_WARPS 12                      // 0-3, 4-7 softmax of tile 0, 1; then
-#define TA_MMA 8
-#define TA_PRODUCER 9
-#define TA_EDGES 10
-#define TA_WALK 11
-// Registers: launched with 168 a thread (384 threads: 64512); the softmax warpgroups, whose rows of S and P live in registers, go up by 40
-// a thread (256 threads: 10240), the others go down by 80 (128 threads: 10240).
-#define TA_REGS_SOFTMAX 208
-#define TA_REGS_OTHER 88
+// A CTA's warps: four to a tile of 128 rows for the softmax, then one each for the products, the loads, the edges and the walk. Two tiles
+// to a CTA and an SM where there are rows enough (they share K and V); else one tile, and two CTAs to an SM: a tile's softmax and products
+// follow one another, and only another tile's work fills the gaps.
+template <int TILES> struct TaRoles {
+    static constexpr int SOFT = 4 * TILES, MMA = SOFT, PRODUCER = SOFT + 1, EDGES = SOFT + 2, WALK = SOFT + 3, WARPS = SOFT + 4;
+    static constexpr int CTAS = TILES == 1 ? 2 : 1, ROWS = 128 * TILES;
+    // Registers a thread: launched with 168 (384 threads) or 128 (256); the softmax warpgroups, whose rows of S and P live in registers, go
+    // up by 40 (256 threads: 10240) or 72 (128 threads: 9216), the last one goes down by 80 or 72 (128 threads).
+    static constexpr int REGS_SOFT = TILES == 1 ? 200 : 208, REGS_OTHER = TILES == 1 ? 56 : 88;
+};
 #define TA_STATUS_CODE 7
 #define TA_ITEM_COST 4
+#define TA_ITEM_COST_ONE 2
+#define TA_SNAP 2
+#define TA_ONE_TILE_ROWS 128
 #define TA_LIMIT 16384.f                 // of a tile's sum of weights: f16 holds each
 
 
@@ -174,9 +178,9 @@ struct __align__(16) TaSeg {
     int row, n, len, pos0, over; // of the sequence
 };
 #define TA_SEGS 4
-#define TA_SEG_USERS 11          // warps that read it
+template <int TILES>
 __device__ __forceinline__ void ta_seg(const AttnArgs &a, const AttnSeg &g, volatile TaSeg *t) {
-    const int tq = a.tok_item >> 1, tok0 = g.blk * a.tok_item;
+    const int tq = a.tok_item / TILES, tok0 = g.blk * a.tok_item;
     t->seq = g.seq; t->head = g.head; t->u0 = g.u0; t->u1 = g.u1;
     t->whole = g.u0 == 0 && g.u1 == g.units;
     t->ends = g.u1 == g.units;
@@ -185,7 +189,7 @@ __device__ __forceinline__ void ta_seg(const AttnArgs &a, const AttnSeg &g, vola
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int first = tok0 + i * tq;
-        const int units = first < g.q.n ? (attn_limit(g.q, min(first + tq, g.q.n)) + TA_KV - 1) >> TA_UNIT_SHIFT : 0;
+        const int units = i < TILES && first < g.q.n ? (attn_limit(g.q, min(first + tq, g.q.n)) + TA_KV - 1) >> TA_UNIT_SHIFT : 0;
         t->e[i] = max(0, min(units, g.u1) - g.u0);
     }
     t->edge = min(attn_limit(g.q, tok0 + 1), g.q.len) >> TA_UNIT_SHIFT;
@@ -195,12 +199,13 @@ __device__ __forceinline__ int ta_seen(const volatile TaSeg *t, int tok1) {     
     return max(0, min(t->pos0 + tok1, t->len));
 }
 
-template <int D> struct TaSmem {
+template <int D, int TILES> struct TaSmem {
     static constexpr int NH = D / 64;                         // 64-column halves: 128 bytes of a row, the swizzle's width
     static constexpr int HALF = 128 * 128;                    // bytes of 128 rows of one
     static constexpr int TILE = NH * HALF;
-    static constexpr int STAGES = D == 128 ? 4 : 8;
-    static constexpr int Q = 0, KV = 2 * TILE, OUT = KV + STAGES * TILE, BARS = OUT + 8 * 4096;      // OUT: a softmax warp's 32 rows of 128 bytes
+    static constexpr int STAGES = (D == 128 ? 2 : 4) * TILES;
+    static constexpr int PASS = D == 128 && TILES == 1 ? 64 : 128;       // bytes of a row that leave at a time
+    static constexpr int Q = 0, KV = TILES * TILE, OUT = KV + STAGES * TILE, BARS = OUT + 4 * TILES * 32 * PASS;     // OUT: 32 rows of PASS bytes to a softmax warp
     // barriers: kv_full[STAGES], kv_empty[STAGES], q_full, q_empty, s_full[2], p_full[2], o_full[2], drain, v_ok[OKS], e_full[OKS], g_full[TA_SEGS], g_empty[TA_SEGS]
     static constexpr int OKS = D == 128 ? 4 : 8;              // more than the V tiles that the ring can hold
     static constexpr int NBARS = 2 * STAGES + 9 + 2 * OKS + 2 * TA_SEGS;
@@ -243,11 +248,13 @@ __device__ __noinline__ void ta_odd(const AttnArgs *a, int seq, int head, int ro
     }
 }
 
-template <int D, bool BF16, bool HILO>
-__global__ void __launch_bounds__(TA_WARPS * 32, 1)
+template <int D, int TILES, bool BF16, bool HILO>
+__global__ void __launch_bounds__(TaRoles<TILES>::WARPS * 32, TaRoles<TILES>::CTAS)
 attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                 const __grid_constant__ CUtensorMap vmap, int box_rows, int min_units) {
-    using L = TaSmem<D>;
+    using L = TaSmem<D, TILES>;
+    using R = TaRoles<TILES>;
+    constexpr int TM_O = TILES * 128;                       // O's columns in TMEM, behind S's
     extern __shared__ uint8_t raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sbase = smem_u32(smem), bars = sbase + L::BARS;
@@ -258,7 +265,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::MISC + 4);        // [0] flag, [1] limit
     volatile int *seg_bad = reinterpret_cast<volatile int *>(smem + L::MISC + 16), *seg_odd = seg_bad + 4;
     const int warp = tc5_uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int tq = a.tok_item >> 1;
+    const int tq = a.tok_item / TILES;
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::STAGES; ++s) { mbar_init(kv_full + 8 * s, 1); mbar_init(kv_empty + 8 * s, 1); }
         mbar_init(q_full, 1);
@@ -269,20 +276,20 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             mbar_init(o_full + 8 * i, 1);
         }
         for (int i = 0; i < 2 * L::OKS; ++i) mbar_init(v_ok + 8 * i, 1);       // and e_full
-        for (int i = 0; i < TA_SEGS; ++i) { mbar_init(g_full + 8 * i, 1); mbar_init(g_empty + 8 * i, TA_SEG_USERS); }
+        for (int i = 0; i < TA_SEGS; ++i) { mbar_init(g_full + 8 * i, 1); mbar_init(g_empty + 8 * i, R::SOFT + 3); }     // all but the walk
         mbar_init(drain, 1);
         for (int i = 0; i < 4; ++i) seg_bad[i] = seg_odd[i] = 0;
         abort_flag[0] = 0;
         abort_flag[1] = a.status[1];
         mbar_init_fence();
     }
-    if (warp == TA_MMA) tc5_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), 512);
+    if (warp == R::MMA) tc5_alloc(smem_u32(const_cast<uint32_t *>(tmem_slot)), 256 * TILES);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     tc5_fence_before();
     __syncthreads();
     tc5_fence_after();
-    const uint32_t tmem = *tmem_slot;                       // S of the tiles at columns 0, 128; O at 256, 384
+    const uint32_t tmem = *tmem_slot;                       // S of the tiles at columns 0, 128; O behind them
     volatile TaSeg *const ring = reinterpret_cast<volatile TaSeg *>(smem + L::SEGS);
     bool ok = true;
     uint32_t gi = 0;                                        // segments seen
@@ -299,8 +306,8 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     };
 #define TA_REGS(how, n) asm volatile("setmaxnreg." how ".sync.aligned.u32 %0;" ::"n"(n))
 
-    if (warp == TA_PRODUCER) {
-        TA_REGS("dec", TA_REGS_OTHER);
+    if (warp == R::PRODUCER) {
+        TA_REGS("dec", R::REGS_OTHER);
         // ------------------------------------------------ producer: the ring's tiles are K's and V's in turn
         const uint32_t sb = (uint32_t)tc5_uniform((int)sbase);
         uint32_t it = 0, segs = 0, edges = 0;               // tiles issued, segments with work, edge tiles of V
@@ -373,8 +380,8 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             for (uint32_t i = edges > (uint32_t)L::OKS ? edges - L::OKS : 0; i < edges; ++i)
                 mbar_wait_ns(e_full + 8 * (i % L::OKS), (i / L::OKS) & 1, limit);
         }
-    } else if (warp == TA_MMA) {
-        TA_REGS("dec", TA_REGS_OTHER);
+    } else if (warp == R::MMA) {
+        TA_REGS("dec", R::REGS_OTHER);
         // ------------------------------------------------ products
         constexpr uint32_t type = BF16 ? (1u << 7) | (1u << 10) : 0u;
         constexpr uint32_t id_s = tc5_idesc(128, 128) | type, id_o = tc5_idesc(128, D) | type | (1u << 16);   // V: N contiguous
@@ -416,7 +423,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 }
                 if (ok && j + 1 < E) ok = __all_sync(0xffffffffu, ta_wait(kv_full + 8 * sk, ((it + 1) / L::STAGES) & 1, abort_flag));
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < TILES; ++i) {
                     const int e = i ? e1 : e0;
                     if (!ok || j >= e) continue;
                     ok = __all_sync(0xffffffffu, ta_wait(p_full + 8 * i, done[i] & 1, abort_flag));
@@ -424,7 +431,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     tc5_fence_after();
                     if (leader) {
                         const uint64_t v = vd + sv * (L::TILE >> 4);
-                        const uint32_t p = tm + i * 128, o = tm + 256 + i * 128;
+                        const uint32_t p = tm + i * 128, o = tm + TM_O + i * 128;
 #pragma unroll
                         for (int x = 0; x < TA_KV / 16; ++x) {
                             ta_mma_ts(o, p + 32 * (x >> 1) + 8 * (x & 1), v + x * (2048 >> 4), id_o, j != 0 || x != 0);
@@ -448,8 +455,8 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         if (leader) tc5_commit(drain);                               // nothing of the tensor core's is left when TMEM is given back
         __syncwarp();
         if (!mbar_wait_ns(drain, 0, tc5_limit_ns(abort_flag))) *abort_flag = 1;
-    } else if (warp == TA_EDGES) {
-        TA_REGS("dec", TA_REGS_OTHER);
+    } else if (warp == R::EDGES) {
+        TA_REGS("dec", R::REGS_OTHER);
         // ------------------------------------------------ edges
         // V tiles at the edge of what the item's rows see. Positions behind the sequence's end become zeros (another sequence's rows,
         // or what was in the stage before), and so does what is infinite or NaN: its weight is zero for the rows that do not see it,
@@ -503,8 +510,8 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             segs++;
             seg_done();
         }
-    } else if (warp == TA_WALK) {
-        TA_REGS("dec", TA_REGS_OTHER);
+    } else if (warp == R::WALK) {
+        TA_REGS("dec", R::REGS_OTHER);
         // ------------------------------------------------ the walk
         AttnCut first, last;
         attn_share(a, blockIdx.x, gridDim.x, TA_UNIT_SHIFT, min_units, first, last);
@@ -516,13 +523,13 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             if (!ok) break;
             more = walk.next(a, TA_UNIT_SHIFT, g);
             if (lane == 0) {
-                if (more) ta_seg(a, g, ring + gi % TA_SEGS);
+                if (more) ta_seg<TILES>(a, g, ring + gi % TA_SEGS);
                 else ring[gi % TA_SEGS].seq = -1;
                 mbar_arrive(g_full + 8 * (gi % TA_SEGS));
             }
         }
     } else {
-        TA_REGS("inc", TA_REGS_SOFTMAX);
+        TA_REGS("inc", R::REGS_SOFT);
         // ------------------------------------------------ softmax: warpgroup i owns tile i, a thread one of its rows
         // The weights of a tile are taken to the maximum of the tiles before it, without looking for the tile's own first: nothing is
         // lost as long as they stay in range, and their sum, which is taken anyway, says whether they do. Only where it passes TA_LIMIT
@@ -530,7 +537,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         // P is written over it at the end. The sums and products are f32, so scaled by up to TA_LIMIT they lose nothing.
         const int i = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // 32 lanes a warp, in bits 16 and up of a TMEM address
-        const uint32_t S = tmem + i * 128 + lanes, O = tmem + 256 + i * 128 + lanes;
+        const uint32_t S = tmem + i * 128 + lanes, O = tmem + TM_O + i * 128 + lanes;
         const float c = a.scale_log2;
         uint32_t tiles = 0, parts = 0, segs = 0;
         AttnMeta *const meta = a.meta + blockIdx.x;
@@ -665,61 +672,64 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             float *slot = nullptr;
             if (!whole) {
                 const int which = t->u0 > 0 ? 0 : 1;
-                slot = a.part + ((size_t)blockIdx.x * 2 + which) * attn_slot_floats(ATTN_TC_ROWS, D);
+                slot = a.part + ((size_t)blockIdx.x * 2 + which) * attn_slot_floats(R::ROWS, D);
                 if (threadIdx.x == 0) {
                     if (which == 0) { meta->cont = 1; meta->ends = t->ends; }
                     else { meta->own = 1; meta->row = t->row + t->tok0; meta->ntok = t->ntok; meta->head = t->head; }
                 }
                 if (live) {
-                    slot[ATTN_TC_ROWS * D + row] = m * c;
-                    slot[ATTN_TC_ROWS * D + ATTN_TC_ROWS + row] = l;
+                    slot[R::ROWS * D + row] = m * c;
+                    slot[R::ROWS * D + R::ROWS + row] = l;
                 }
             }
             const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-            // Rows leave through shared memory, 128 bytes of each at a time: a thread has a row, and its own stores would touch 32 lines
+            // Rows leave through shared memory, PASS bytes of each at a time: a thread has a row, and its own stores would touch 32 lines
             // an instruction (8 us of an item's time). Where the row goes; negative: nowhere.
+            constexpr int PB = L::PASS, GR = PB / 4, PP = PB / 16;   // columns fetched at a time; 16-byte pieces of a row's pass
             const bool f32 = !whole || a.out_dtype == JL_DT_F32;
             uint8_t *const dst = whole ? static_cast<uint8_t *>(a.out) : reinterpret_cast<uint8_t *>(slot);
             const long long at = !live || (!whole && E == 0) ? -1
                                  : (whole ? (long long)(t->row + t->tok0 + tok) * a.hq + t->head * a.g + r % a.g : (long long)row) * (f32 ? 4 : 2) * D;
-            const uint32_t stage = sbase + L::OUT + warp * 4096;
-            uint32_t w[32];                                          // the 128 bytes
+            const uint32_t stage = sbase + L::OUT + warp * 32 * PB;
+            auto swizzle = [](int row, int piece) { return PP == 8 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3); };
+            uint32_t w[GR];                                          // the pass
 #pragma unroll 1
-            for (int x = 0; x < D / 32 && !idle; ++x) {
-                uint32_t o[32];
+            for (int x = 0; x < D / GR && !idle; ++x) {
+                uint32_t o[GR];
                 if (E > 0) {
-                    tc5_ld32(O + 32 * x, o);
+                    if constexpr (GR == 32) tc5_ld32(O + GR * x, o);
+                    else tc5_ld16(O + GR * x, o);
                     ta_wait_ld(o);
                 } else {
 #pragma unroll
-                    for (int y = 0; y < 32; ++y) o[y] = 0u;
+                    for (int y = 0; y < GR; ++y) o[y] = 0u;
                 }
                 if (f32) {
 #pragma unroll
-                    for (int y = 0; y < 32; ++y) w[y] = __float_as_uint(__uint_as_float(o[y]) * inv);
+                    for (int y = 0; y < GR; ++y) w[y] = __float_as_uint(__uint_as_float(o[y]) * inv);
                 } else {
 #pragma unroll
-                    for (int y = 0; y < 16; ++y) {
+                    for (int y = 0; y < GR / 2; ++y) {
                         const float u = __uint_as_float(o[2 * y]) * inv, v = __uint_as_float(o[2 * y + 1]) * inv;
                         const uint32_t p = a.out_dtype == JL_DT_BF16 ? ta_pack<true>(u, v) : ta_pack<false>(u, v);
-                        if (x & 1) w[16 + y] = p; else w[y] = p;
+                        if (x & 1) w[GR / 2 + y] = p; else w[y] = p;
                     }
                     if (!(x & 1)) continue;
                 }
                 __syncwarp();                                        // the last pass's rows have been read
 #pragma unroll
-                for (int y = 0; y < 8; ++y)
-                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * 128 + ((y ^ (lane & 7)) << 4)), "r"(w[4 * y]),
+                for (int y = 0; y < PP; ++y)
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * PB + (swizzle(lane, y) << 4)), "r"(w[4 * y]),
                                  "r"(w[4 * y + 1]), "r"(w[4 * y + 2]), "r"(w[4 * y + 3]) : "memory");
                 __syncwarp();
-                const int col = f32 ? 128 * x : 64 * (x - 1);        // in bytes
+                const int col = f32 ? PB * x : PB / 2 * (x - 1);     // in bytes
 #pragma unroll
-                for (int y = 0; y < 8; ++y) {
-                    const int rr = 4 * y + (lane >> 3), pc = lane & 7;
+                for (int y = 0; y < PP; ++y) {
+                    const int rr = y * (32 / PP) + lane / PP, pc = lane % PP;
                     const long long to = __shfl_sync(0xffffffffu, at, rr);
                     uint4 v;
                     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                 : "r"(stage + rr * 128 + ((pc ^ (rr & 7)) << 4)));
+                                 : "r"(stage + rr * PB + (swizzle(rr, pc) << 4)));
                     if (to >= 0) *reinterpret_cast<uint4 *>(dst + to + col + 16 * pc) = v;
                 }
             }
@@ -734,7 +744,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     __syncthreads();
     tc5_fence_after();
     if (threadIdx.x == 0 && *abort_flag) atomicExch(a.status, TA_STATUS_CODE);
-    if (warp == TA_MMA) tc5_dealloc(tmem, 512);
+    if (warp == R::MMA) tc5_dealloc(tmem, 256 * TILES);
 }
 
 static bool ta_map(CUtensorMap *map, const void *base, bool bf16, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
@@ -746,23 +756,32 @@ static bool ta_map(CUtensorMap *map, const void *base, bool bf16, int rank, cons
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, bool BF16, bool HILO>
+template <int D, int TILES, bool BF16, bool HILO>
 static int ta_go(jl_ctx *ctx, const AttnArgs &a, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, int box_rows, cudaStream_t s) {
-    auto kern = attn_tc5_kernel<D, BF16, HILO>;
-    const int smem = TaSmem<D>::TOTAL, grid = ctx->sm_count;
+    using R = TaRoles<TILES>;
+    auto kern = attn_tc5_kernel<D, TILES, BF16, HILO>;
+    const int smem = TaSmem<D, TILES>::TOTAL, grid = ctx->sm_count * R::CTAS;
     JL_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const cudaError_t e = attn_launch_pdl(kern, dim3(grid), dim3(TA_WARPS * 32), smem, s, a, q, k, v, box_rows, 2);
+    const cudaError_t e = attn_launch_pdl(kern, dim3(grid), dim3(R::WARPS * 32), smem, s, a, q, k, v, box_rows, 2);
     JL_CUDA(ctx, e);
     ctx->st.launches++;
-    return attn_launch_merge(ctx, a, ATTN_TC_ROWS, grid, s);
+    return attn_launch_merge(ctx, a, R::ROWS, grid, s);
 }
 
-int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &args, int dtype, cudaStream_t s) {
+template <int D, int TILES>
+static int ta_type(jl_ctx *ctx, const AttnArgs &a, bool bf16, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, int box_rows, cudaStream_t s) {
+    if (a.out_dtype == JL_DT_F32)
+        return bf16 ? ta_go<D, TILES, true, true>(ctx, a, q, k, v, box_rows, s) : ta_go<D, TILES, false, true>(ctx, a, q, k, v, box_rows, s);
+    return bf16 ? ta_go<D, TILES, true, false>(ctx, a, q, k, v, box_rows, s) : ta_go<D, TILES, false, false>(ctx, a, q, k, v, box_rows, s);
+}
+
+int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &args, int dtype, long long max_rows, cudaStream_t s) {
     AttnArgs a = args;
-    const int tq = 128 / a.g;
-    a.tok_item = 2 * tq;
-    a.item_cost = TA_ITEM_COST;
-    const bool bf16 = dtype == JL_DT_BF16, hilo = a.out_dtype == JL_DT_F32;
+    const int tq = 128 / a.g, tiles = max_rows <= TA_ONE_TILE_ROWS ? 1 : 2;
+    a.tok_item = tiles * tq;
+    a.item_cost = tiles == 1 ? TA_ITEM_COST_ONE : TA_ITEM_COST;
+    a.snap = TA_SNAP;
+    const bool bf16 = dtype == JL_DT_BF16;
     CUtensorMap q, k, v;
     const cuuint64_t d = a.d;
     const cuuint64_t qd[3] = {d, (cuuint64_t)a.hq, (cuuint64_t)a.total}, qs[2] = {(cuuint64_t)a.q_head * 2, (cuuint64_t)a.q_tok * 2};
@@ -774,8 +793,6 @@ int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &args, int dtype, cudaStream_t s
     const cuuint32_t kb[4] = {64, (cuuint32_t)box_rows, 1, 1};
     if (!ta_map(&q, a.q, bf16, 3, qd, qs, qb) || !ta_map(&k, a.k, bf16, 4, kd, ks, kb) || !ta_map(&v, a.v, bf16, 4, kd, ks, kb))
         return JL_DECLINED;
-#define TA_GO(D) (bf16 ? (hilo ? ta_go<D, true, true>(ctx, a, q, k, v, box_rows, s) : ta_go<D, true, false>(ctx, a, q, k, v, box_rows, s)) \
-                       : (hilo ? ta_go<D, false, true>(ctx, a, q, k, v, box_rows, s) : ta_go<D, false, false>(ctx, a, q, k, v, box_rows, s)))
-    return a.d == 128 ? TA_GO(128) : TA_GO(64);
-#undef TA_GO
+    if (tiles == 1) return a.d == 128 ? ta_type<128, 1>(ctx, a, bf16, q, k, v, box_rows, s) : ta_type<64, 1>(ctx, a, bf16, q, k, v, box_rows, s);
+    return a.d == 128 ? ta_type<128, 2>(ctx, a, bf16, q, k, v, box_rows, s) : ta_type<64, 2>(ctx, a, bf16, q, k, v, box_rows, s);
 }
