@@ -687,11 +687,16 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             // an instruction (8 us of an item's time). Where the row goes; negative: nowhere.
             constexpr int PB = L::PASS, GR = PB / 4, PP = PB / 16;   // columns fetched at a time; 16-byte pieces of a row's pass
             const bool f32 = !whole || a.out_dtype == JL_DT_F32;
-            uint8_t *const dst = whole ? static_cast<uint8_t *>(a.out) : reinterpret_cast<uint8_t *>(slot);
-            const long long at = !live || (!whole && E == 0) ? -1
-                                 : (whole ? (long long)(t->row + t->tok0 + tok) * a.hq + t->head * a.g + r % a.g : (long long)row) * (f32 ? 4 : 2) * D;
+            const int size = f32 ? 4 : 2;
+            uint8_t *const dst = whole ? static_cast<uint8_t *>(a.out) + ((long long)(t->row + t->tok0) * a.hq + t->head * a.g) * size * D
+                                       : reinterpret_cast<uint8_t *>(slot);      // of the item
+            const int at = !live || (!whole && E == 0) ? -1 : (whole ? tok * a.hq + r % a.g : row) * size * D;
             const uint32_t stage = sbase + L::OUT + warp * 32 * PB;
             auto swizzle = [](int row, int piece) { return PP == 8 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3); };
+            const int first = lane / PP, pc = lane % PP;             // of the rows and pieces that this thread stores: rows first + y 32 / PP
+            int to[PP];
+#pragma unroll
+            for (int y = 0; y < PP; ++y) to[y] = __shfl_sync(0xffffffffu, at, y * (32 / PP) + first);
             uint32_t w[GR];                                          // the pass
 #pragma unroll 1
             for (int x = 0; x < D / GR && !idle; ++x) {
@@ -725,12 +730,11 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 const int col = f32 ? PB * x : PB / 2 * (x - 1);     // in bytes
 #pragma unroll
                 for (int y = 0; y < PP; ++y) {
-                    const int rr = y * (32 / PP) + lane / PP, pc = lane % PP;
-                    const long long to = __shfl_sync(0xffffffffu, at, rr);
+                    const int rr = y * (32 / PP) + first;
                     uint4 v;
                     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                                  : "r"(stage + rr * PB + (swizzle(rr, pc) << 4)));
-                    if (to >= 0) *reinterpret_cast<uint4 *>(dst + to + col + 16 * pc) = v;
+                    if (to[y] >= 0) *reinterpret_cast<uint4 *>(dst + to[y] + col + 16 * pc) = v;
                 }
             }
             __syncwarp();
