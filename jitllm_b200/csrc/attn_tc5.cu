@@ -2,18 +2,22 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale log2(e) q.k_j - m),  m a maximum of the exponents so far
 //
-// An item is 256 query rows of one kv head in two tiles of 128: (new token, query head of the group), token-major, so that grouped
-// heads share the tile's keys and a causal edge is 128 / g tokens wide. Per 128 positions a tile takes two 128 x 128 x d products
-// (tcgen05.mma, kind::f16: S = Q K^T out of shared memory, O += P V with P out of TMEM) and 128 x 128 exponentials: 1024 clocks each at
-// d = 128, so the two tiles alternate -- the tensor core works on one while the other's softmax runs.
+// An item is 256 query rows of one kv head in two tiles of 128 (or one tile: TaRoles): (new token, query head of the group),
+// token-major, so that grouped heads share the tile's keys and a causal edge is 128 / g tokens wide. Per 128 positions a tile takes two
+// 128 x 128 x d products (tcgen05.mma, kind::f16: S = Q K^T out of shared memory, O += P V with P out of TMEM; 512 clocks each at d = 128)
+// and 128 x 128 exponentials (1024 clocks of the exponential unit). TMEM holds S and O of both tiles and nothing else, P goes over S: so a
+// tile's softmax and products follow one another, and the two tiles alternate, one on the tensor core while the other's softmax runs.
 //
-// Roles of a CTA (one to an SM): two softmax warpgroups, one a tile (a thread owns a row: S comes to its registers, P goes back over
-// S's columns, 16 bits), an MMA warp, a TMA producer, and a warp that looks over the V tiles at a sequence's edge. K and V tiles of 128
-// positions come through one ring by TMA (a box to a page and 64 columns), Q once an item.
+// Roles of a CTA: a softmax warpgroup to a tile (a thread owns a row: S comes to its registers, P goes back over S's columns, 16 bits);
+// a warp each that issues the products, that loads (K and V tiles of 128 positions through one ring by TMA, a box to a page and 64
+// columns; Q once an item), that looks over the V tiles at a sequence's edge, and that walks the CTA's share.
 //
-// O is rescaled only when a row's maximum has grown by more than 2^8 since it was last (P is then at most 2^8: no overflow, the
-// same relative rounding, and the sum of P carries the same factor); by the softmax warpgroup itself, which S's arrival tells that
-// the product before it is complete.
+// What bounds it: a tile's round of 128 positions, 1450 clocks of softmax (1290 of a loop of nothing else, of them 1024 exponentials), 300
+// for S, P and the barriers to change hands, 1024 of products: 3250 clocks as counted with two tiles at work, where the tensor core
+// alone would need 2048. Tried and not kept: exponentials on the FMA pipe by a polynomial (it costs the scheduler what it saves the other
+// unit), rows split over two warps (the exchange of their maxima costs as much), S in halves of 64 positions with columns of their own
+// (the products S = Q K^T then read Q twice as often and take 1.5 times as long), an MMA warp to a tile (their products run side by side
+// and the tiles fall into step). A 16,384-token prompt of 32 heads over 8: 1.99 ms, 1.10 PFLOP/s, at the clock that the power limit leaves.
 #include "attn.cuh"
 #include "tc5.cuh"
 
@@ -30,12 +34,15 @@ template <int TILES> struct TaRoles {
     static constexpr int REGS_SOFT = TILES == 1 ? 200 : 208, REGS_OTHER = TILES == 1 ? 56 : 88;
 };
 #define TA_STATUS_CODE 7
+// What an item's start and end take against a unit: Q's arrival, the first S, the last product, the rows' way out; 10,000 clocks beside
+// 3250 of two tiles, 6000 beside 2900 of one.
 #define TA_ITEM_COST 4
 #define TA_ITEM_COST_ONE 2
 #define TA_SNAP 2
+// One tile up to as many rows as it has (five tokens of 8 heads: 50 us against 62 with a second tile idle); beyond, two: a 1531-token
+// prompt takes 52 us so and 60 as single tiles, whose CTAs load K and V each for itself.
 #define TA_ONE_TILE_ROWS 128
 #define TA_LIMIT 16384.f                 // of a tile's sum of weights: f16 holds each
-
 
 // The bounded wait of this kernel's roles. A try that may sleep for up to 20 us: the warps that wait are many, and their polling would take
 // the issue slots of those that work.
@@ -531,10 +538,12 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     } else {
         TA_REGS("inc", R::REGS_SOFT);
         // ------------------------------------------------ softmax: warpgroup i owns tile i, a thread one of its rows
-        // The weights of a tile are taken to the maximum of the tiles before it, without looking for the tile's own first: nothing is
-        // lost as long as they stay in range, and their sum, which is taken anyway, says whether they do. Only where it passes TA_LIMIT
-        // (or is NaN), and at a row's first tile, S is read for its maximum, O rescaled and the weights taken again: S stays whole until
-        // P is written over it at the end. The sums and products are f32, so scaled by up to TA_LIMIT they lose nothing.
+        // The weights of a tile are taken to a reference of the tiles before it, without looking for the tile's own maximum first (250
+        // clocks): nothing is lost as long as they stay in range, and their sum, which is taken anyway, says whether they do. A row's
+        // first reference is the largest of its first 16 scores. Where the sum passes TA_LIMIT (or is NaN), and in masked tiles, S is
+        // read for its maximum, O rescaled -- S's arrival tells that the product before it is complete -- and the weights taken to that:
+        // S stays whole until P is written over it. The sums and products are f32, so scaled by up to TA_LIMIT they lose nothing. The two
+        // ways are kept apart: a loop around one of them, or masks in it, cost 100 to 470 clocks a tile.
         const int i = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // 32 lanes a warp, in bits 16 and up of a TMEM address
         const uint32_t S = tmem + i * 128 + lanes, O = tmem + TM_O + i * 128 + lanes;
@@ -549,7 +558,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             const int seen = ta_seen(t, t->tok0 + min(tok, t->ntok - 1) + 1) - p_first;      // positions of the segment that the row sees
             const int all_seen = ta_seen(t, t->tok0 + i * tq + 1) - p_first;                 // by the tile's first token: below it nothing is masked
             const bool idle = !__any_sync(0xffffffffu, live);        // no row of the warp is used: its columns of P stay as they are
-            float m = -INFINITY, l = 0.f;                            // m: the maximum that O and l are scaled to (of S, unscaled)
+            float m = -INFINITY, l = 0.f;                            // m: the reference that O and l are scaled to (of S, unscaled)
             for (int j = 0; j < E; ++j, ++tiles) {
                 ok = __all_sync(0xffffffffu, ta_wait(s_full + 8 * i, tiles & 1, abort_flag));
                 if (!ok) break;
