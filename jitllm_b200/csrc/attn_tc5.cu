@@ -46,7 +46,9 @@ template <int TILES> struct TaRoles {
 
 // The bounded wait of this kernel's roles. A try that may sleep for up to 20 us: the warps that wait are many, and their polling would take
 // the issue slots of those that work.
-__device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+// patience: by how much the limit is longer for a role whose wait spans others' whole work (they give up first, and end it).
+#define TA_PATIENCE 4096u
+__device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, uint32_t patience = 1) {
     uint64_t t0 = 0;
     for (;;) {
         uint32_t done;
@@ -61,7 +63,7 @@ __device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity, volatile 
         if (*abort_flag) return false;
         const uint64_t t = jl_gtime_ns();
         if (!t0) t0 = t;
-        else if (t - t0 > tc5_limit_ns(abort_flag)) break;
+        else if (t - t0 > tc5_limit_ns(abort_flag) * patience) break;
     }
     *abort_flag = 1;
     return false;
@@ -478,7 +480,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             for (int j = 0; j < E && ok; ++j, it += 2) {
                 if (j < edge) continue;
                 const uint32_t s = (it + 1) % L::STAGES;
-                ok = __all_sync(0xffffffffu, ta_wait(e_full + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag));
+                ok = __all_sync(0xffffffffu, ta_wait(e_full + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag, TA_PATIENCE));
                 if (!ok) break;
                 const int rows = left - j * TA_KV;       // of the sequence
                 const uint32_t v = sbase + L::KV + s * L::TILE;
@@ -526,7 +528,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         walk.begin(first, last);
         AttnSeg g;
         for (bool more = true; more && ok; ++gi) {
-            if (gi >= TA_SEGS) ok = __all_sync(0xffffffffu, ta_wait(g_empty + 8 * (gi % TA_SEGS), (gi / TA_SEGS + 1) & 1, abort_flag));
+            if (gi >= TA_SEGS) ok = __all_sync(0xffffffffu, ta_wait(g_empty + 8 * (gi % TA_SEGS), (gi / TA_SEGS + 1) & 1, abort_flag, TA_PATIENCE));
             if (!ok) break;
             more = walk.next(a, TA_UNIT_SHIFT, g);
             if (lane == 0) {

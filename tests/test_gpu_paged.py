@@ -201,7 +201,7 @@ def test_bad_pages_are_not_followed(dev, max_new):
     assert bool(out[6:].isnan().all())
 
 
-@pytest.mark.parametrize("max_new", [4, None])
+@pytest.mark.parametrize("max_new", [4, 20, None])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
 def test_what_a_row_does_not_see_does_not_reach_it(dev, max_new, value):
     """Infinite or NaN keys and values at a sequence's own later positions leave its earlier rows alone."""
@@ -222,6 +222,44 @@ def test_what_a_row_does_not_see_does_not_reach_it(dev, max_new, value):
         ref, mag, size = _reference(q[a:a + n], *pool.rows[s], lens[s] - new[s], 128 ** -0.5)
         _check(out[a:a + n], ref, mag, size, _dt("bf16"), 300, 128)
     assert not bool(out[54:].isfinite().all(-1).any())                   # the rows that see them do
+
+
+@pytest.mark.parametrize("new", [1, 6, 40])
+def test_many_sequences(dev, new):
+    """More than a warp looks over at once, of all lengths, some idle or empty."""
+    lens = [(37 * s * s) % 700 for s in range(300)]
+    n = [0 if s % 7 == 3 else min(new, lens[s]) for s in range(300)]
+    _paged_case(dev, n, lens, 8, 2, 64, 32, _dt("bf16"), _dt("bf16"), 9, max_new=new)
+
+
+@pytest.mark.parametrize("max_new", [1, 24, None])
+def test_pages_behind_32_bits_of_elements(dev, max_new):
+    """A pool of 2.7e9 elements, its last pages in use: the writer and the attention reach them."""
+    import torch
+    from jitllm_b200 import PagedKV
+    hkv, d, page_len, pages = 8, 128, 64, 41000
+    k = torch.zeros(pages, hkv, page_len, d, device="cuda", dtype=torch.bfloat16)
+    v = torch.zeros_like(k)
+    n = {1: 1, 24: 24, None: 70}[max_new]
+    table = torch.tensor([[pages - 1, 3, pages - 2, 32768]], dtype=torch.int32, device="cuda")
+    kv, cos, sin = PagedKV(k, v, table), *_tables(256, d)
+    qkv = torch.randn(200, (16 + 2 * hkv) * d, device="cuda")
+    st, scratch = torch.cuda.current_stream().cuda_stream, _scratch(dev)
+    q = torch.empty(200, 16, d, device="cuda", dtype=torch.bfloat16)
+    dev.RopeAppend(q, qkv, kv, _starts([200]), torch.tensor([200], dtype=torch.int32, device="cuda"), cos, sin, stream=st)
+    out = torch.empty(n, 16, d, device="cuda")
+    dev.AttnPaged(out, q[200 - n:].contiguous(), kv, _starts([n]), torch.tensor([200], dtype=torch.int32, device="cuda"), scratch, max_new=max_new,
+                  stream=st)
+    torch.cuda.synchronize()
+    x = qkv.view(200, 16 + 2 * hkv, d)
+    vv = x[:, 16 + hkv:].to(torch.bfloat16)
+    for p in (0, 63, 64, 128, 199):
+        assert torch.equal(v[int(table[0, p // 64]), :, p % 64], vv[p])
+    used = sorted(table[0].tolist())
+    assert int((v.view(pages, -1).any(1)).sum()) == 4 and v.view(pages, -1).any(1).nonzero().flatten().tolist() == used
+    kk = k[table[0].long()].transpose(1, 2).reshape(-1, hkv, d)[:200]                     # as the writer rounded them
+    ref, mag, size = _reference(q[200 - n:], kk, vv, 200 - n, d ** -0.5)
+    _check(out, ref, mag, size, torch.bfloat16, 200, d)
 
 
 def test_sequences_may_share_pages(dev):
