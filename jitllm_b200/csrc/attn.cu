@@ -9,25 +9,40 @@
 // The item that CTA c began, and the CTAs behind it continued: the softmax weights of the parts are 2^(their maximum - the largest), the
 // parts added in ascending order of positions.
 
-// The CTA that holds the item's last part; eight of a lane's looks on their way at a time.
-__device__ __forceinline__ int attn_item_end(const AttnMeta *meta, int c, int ctas) {
+// What a warp knows of it after one round of loads: meta of CTA c + lane, and the item's parts, c to c + n - 1 (a CTA among them whose
+// share came out empty has none).
+struct AttnItem { int flags, row, ntok, head, n; };
+__device__ __forceinline__ AttnItem attn_item(const AttnMeta *meta, int c, int ctas) {
     const int lane = threadIdx.x & 31;
-    for (int at = c + 1;; at += 256) {
-        unsigned m[8];
+    const int4 m = *reinterpret_cast<const int4 *>(meta + min(c + lane, ctas - 1));
+    AttnItem it;
+    it.flags = lane == 0 || (m.x & ATTN_CONT);                    // does CTA c + lane hold a part?
+    it.row = __shfl_sync(0xffffffffu, m.y, 0); it.ntok = __shfl_sync(0xffffffffu, m.z, 0); it.head = __shfl_sync(0xffffffffu, m.w, 0);
+    it.n = 0;
+    if (!(__shfl_sync(0xffffffffu, m.x, 0) & ATTN_OWN)) return it;
+    unsigned b = __ballot_sync(0xffffffffu, lane > 0 && (c + lane >= ctas - 1 || (m.x & ATTN_ENDS)));
+    int at = c;
+    while (!b) {                                                  // eight of a lane's looks on their way at a time
+        unsigned e[8];
+        at += 32;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const int i = min(at + 32 * k + lane, ctas - 1);
-            m[k] = i == ctas - 1 || (meta[i].cont && meta[i].ends);
+            e[k] = i == ctas - 1 || (meta[i].flags & ATTN_ENDS);
         }
+        int to = at;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const unsigned b = __ballot_sync(0xffffffffu, m[k]);
-            if (b) return min(at + 32 * k + __ffs(b) - 1, ctas - 1);
+            const unsigned x = __ballot_sync(0xffffffffu, e[k]);
+            if (x && !b) { b = x; to = at + 32 * k; }
         }
+        at = b ? to : at + 224;
     }
+    it.n = min(at + __ffs(b) - 1, ctas - 1) - c + 1;
+    return it;
 }
 template <int D>
-__device__ __forceinline__ void attn_merge_store(const AttnArgs &a, const AttnMeta &own, int r, int col, const float (&acc)[D / 32], float L) {
+__device__ __forceinline__ void attn_merge_store(const AttnArgs &a, const AttnItem &own, int r, int col, const float (&acc)[D / 32], float L) {
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const size_t at = ((size_t)(own.row + r / a.g) * a.hq + own.head * a.g + r % a.g) * D + col;
     if constexpr (D == 128) attn_store4(a.out, a.out_dtype, at, make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv));
@@ -44,71 +59,89 @@ __device__ __forceinline__ void attn_merge_load(const float *p, float (&v)[D / 3
     }
 }
 
-// Many rows and, as a rule, few parts: block (c, y) takes eight rows, a warp each. Bound by the parts' bytes, which come from L2: small
-// warps, many of them.
+// Bound by the latency of loads that follow one another, 0.7 us each beside parts of a few MB that L2 serves: so everything whose address
+// is known is asked for at once, the maxima, the sums and the first parts' rows, and weighed once it is there.
+
+// Many rows and, as a rule, few parts: block (c, y) takes eight rows, a warp each.
 template <int D>
 __global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_constant__ AttnArgs a, int ctas, int slot_rows) {
-    constexpr int V = D / 32;
+    constexpr int V = D / 32, B = 4;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int c = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const AttnMeta own = a.meta[c];
-    if (!own.own || r >= own.ntok * a.g) return;
-    const int end = attn_item_end(a.meta, c, ctas);
+    const AttnItem it = attn_item(a.meta, c, ctas);
+    if (r >= it.ntok * a.g || !it.n) return;
     const size_t slot = attn_slot_floats(slot_rows, D);
-    float M = -INFINITY;
-    for (int i = c + lane; i <= end; i += 32)
-        if (i == c || a.meta[i].cont) M = fmaxf(M, __ldcg(a.part + ((size_t)i * 2 + (i == c)) * slot + slot_rows * D + r));
+    auto part_of = [&](int k) { return a.part + ((size_t)(c + k) * 2 + (k == 0)) * slot; };
+    auto there = [&](int k) { return k < it.n && (k < 32 ? it.flags : a.meta[c + k].flags & ATTN_CONT) != 0; };      // k % 32 == lane
+    auto top_of = [&](int k) { return there(k) ? __ldcg(part_of(k) + slot_rows * D + r) : -INFINITY; };
+    auto sum_of = [&](int k) { return there(k) ? __ldcg(part_of(k) + slot_rows * D + slot_rows + r) : 0.f; };
+    float v[B][V], m = top_of(lane), l = sum_of(lane), M = m;
+    auto rows_of = [&](int k0) {
+#pragma unroll
+        for (int k = 0; k < B; ++k)
+            if (k0 + k < it.n) attn_merge_load<D>(part_of(k0 + k) + (size_t)r * D + V * lane, v[k]);
+    };
+    rows_of(0);
+    for (int k = 32 + lane; k < it.n; k += 32) M = fmaxf(M, top_of(k));
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float mu = M == -INFINITY ? 0.f : M;
     float L = 0.f, acc[V] = {};
-    for (int i0 = c; i0 <= end; i0 += 32) {
-        float w = 0.f, l = 0.f;                                   // of part i0 + lane
-        if (i0 + lane <= end && (i0 + lane == c || a.meta[i0 + lane].cont)) {
-            const float *p = a.part + ((size_t)(i0 + lane) * 2 + (i0 + lane == c)) * slot + slot_rows * D + r;
-            w = exp2f(__ldcg(p) - mu);
-            l = __ldcg(p + slot_rows);
-        }
-        const int cnt = min(32, end - i0 + 1);
-#pragma unroll 4
-        for (int k = 0; k < cnt; ++k) {
-            const float wk = __shfl_sync(0xffffffffu, w, k), lk = __shfl_sync(0xffffffffu, l, k);
-            if (lk == 0.f) continue;                              // the part holds nothing of this row, perhaps not even numbers
-            float v[V];
-            attn_merge_load<D>(a.part + ((size_t)(i0 + k) * 2 + (i0 + k == c)) * slot + (size_t)r * D + V * lane, v);
+    for (int k0 = 0; k0 < it.n; k0 += B) {
+        if (k0 && !(k0 & 31)) { m = top_of(k0 + lane); l = sum_of(k0 + lane); }
+        if (k0) rows_of(k0);
+        const float w = exp2f(m - mu);
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+            const float wk = __shfl_sync(0xffffffffu, w, (k0 + k) & 31), lk = __shfl_sync(0xffffffffu, l, (k0 + k) & 31);
+            if (k0 + k >= it.n || lk == 0.f) continue;            // the part holds nothing of this row, perhaps not even numbers
             L = fmaf(wk, lk, L);
 #pragma unroll
-            for (int x = 0; x < V; ++x) acc[x] = fmaf(wk, v[x], acc[x]);
+            for (int x = 0; x < V; ++x) acc[x] = fmaf(wk, v[k][x], acc[x]);
         }
     }
-    attn_merge_store<D>(a, own, r, V * lane, acc, L);
+    attn_merge_store<D>(a, it, r, V * lane, acc, L);
 }
 
-// Few rows: block (c, y) takes rows y, y + 4, ... of the item. A handful of parts: a warp to a row. Hundreds (a long sequence): bound by the
-// loads' latency, so the eight warps share a row, each a run of its parts with eight loads on their way, the runs added in order
-// (131,071 positions of two kv heads, 222 parts to a row: 150 us with one warp and one part at a time).
+// Few rows: block (c, y) takes rows y, y + 8, ... of the item. A handful of parts: a warp to a row. Hundreds (a long sequence): the eight
+// warps share a row, each a run of its parts, the runs added in order (131,071 positions of two kv heads, 222 parts to a row: 150 us with
+// one warp and one part at a time; 52.9 in all with four blocks to an item, 48.4 with eight).
+#define ATTN_MERGE_BLOCKS 8
 template <int ROWS, int D>
 __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_constant__ AttnArgs a, int ctas) {
-    constexpr int V = D / 32;
+    constexpr int V = D / 32, B = 8;
     __shared__ float sums[8][D + 1];                              // a warp's weighted sums, and its sum of weights
     __shared__ float tops[8];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const AttnMeta own = a.meta[c];
-    const int rows = own.ntok * a.g;
-    if (!own.own || (int)blockIdx.y >= rows) return;
-    const int n = attn_item_end(a.meta, c, ctas) - c + 1;
+    const AttnItem it = attn_item(a.meta, c, ctas);
+    const int rows = it.ntok * a.g;
+    if (!it.n || (int)blockIdx.y >= rows) return;
     const size_t slot = attn_slot_floats(ROWS, D);
-    const bool together = n > 16;
-    auto part_of = [&](int i) { return a.part + ((size_t)i * 2 + (i == c)) * slot; };
-    auto there = [&](int i) { return i == c || a.meta[i].cont; };
-    for (int r = blockIdx.y + (together ? 0 : 4 * warp); r < rows; r += together ? 4 : 32) {
-        const int lo = together ? c + n * warp / 8 : c, hi = together ? c + n * (warp + 1) / 8 : c + n;
-        float M = -INFINITY;
-        for (int i = lo + lane; i < hi; i += 32)
-            if (there(i)) M = fmaxf(M, __ldcg(part_of(i) + ROWS * D + r));
+    const bool together = it.n > 16;
+    const int lo = together ? it.n * warp / 8 : 0, hi = together ? it.n * (warp + 1) / 8 : it.n;
+    auto part_of = [&](int k) { return a.part + ((size_t)(c + k) * 2 + (k == 0)) * slot; };
+    // of the lane's parts lo + lane and lo + 32 + lane; a run has no more than 64 (ATTN_FEW_MAX)
+    bool has[2];
+    has[0] = lo + lane < hi && (together ? lo + lane == 0 || (a.meta[c + lo + lane].flags & ATTN_CONT) : it.flags != 0);
+    has[1] = lo + 32 + lane < hi && (a.meta[c + lo + 32 + lane].flags & ATTN_CONT);
+    for (int r = blockIdx.y + (together ? 0 : ATTN_MERGE_BLOCKS * warp); r < rows; r += ATTN_MERGE_BLOCKS * (together ? 1 : 8)) {
+        float m[2], l[2], v[B][V];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float *p = part_of(lo + 32 * h + lane) + ROWS * D + r;
+            m[h] = has[h] ? __ldcg(p) : -INFINITY;
+            l[h] = has[h] ? __ldcg(p + ROWS) : 0.f;
+        }
+        auto rows_of = [&](int k0) {
+#pragma unroll
+            for (int k = 0; k < B; ++k)
+                if (k0 + k < hi) attn_merge_load<D>(part_of(k0 + k) + (size_t)r * D + V * lane, v[k]);
+        };
+        rows_of(lo);
+        float M = fmaxf(m[0], m[1]);
 #pragma unroll
         for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         if (together) {
@@ -118,32 +151,18 @@ __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_consta
             for (int i = 0; i < 8; ++i) M = fmaxf(M, tops[i]);
         }
         const float mu = M == -INFINITY ? 0.f : M;
+        const float w0 = exp2f(m[0] - mu), w1 = exp2f(m[1] - mu);
         float L = 0.f, acc[V] = {};
-        for (int i0 = lo; i0 < hi; i0 += 32) {
-            float w = 0.f, l = 0.f;                               // of part i0 + lane
-            if (i0 + lane < hi && there(i0 + lane)) {
-                const float *p = part_of(i0 + lane) + ROWS * D + r;
-                l = __ldcg(p + ROWS);
-                w = l == 0.f ? 0.f : exp2f(__ldcg(p) - mu);       // a part that holds nothing of the row, perhaps not even numbers
-            }
-            const int cnt = min(32, hi - i0);
-            for (int k0 = 0; k0 < cnt; k0 += 8) {
-                float v[8][V], wk[8];
+        for (int k0 = 0; lo + k0 < hi; k0 += B) {
+            if (k0) rows_of(lo + k0);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    wk[k] = __shfl_sync(0xffffffffu, w, (k0 + k) & 31);
-                    const float lk = __shfl_sync(0xffffffffu, l, (k0 + k) & 31);
-                    const bool use = k0 + k < cnt && lk != 0.f;
-                    if (use) L = fmaf(wk[k], lk, L);
-                    else wk[k] = 0.f;
+            for (int k = 0; k < B; ++k) {
+                const float wk = __shfl_sync(0xffffffffu, k0 < 32 ? w0 : w1, (k0 + k) & 31);
+                const float lk = __shfl_sync(0xffffffffu, k0 < 32 ? l[0] : l[1], (k0 + k) & 31);
+                if (lo + k0 + k >= hi || lk == 0.f) continue;     // the part holds nothing of the row, perhaps not even numbers
+                L = fmaf(wk, lk, L);
 #pragma unroll
-                    for (int x = 0; x < V; ++x) v[k][x] = 0.f;
-                    if (use) attn_merge_load<D>(part_of(i0 + k0 + k) + (size_t)r * D + V * lane, v[k]);
-                }
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-#pragma unroll
-                    for (int x = 0; x < V; ++x) acc[x] = fmaf(wk[k], v[k][x], acc[x]);
+                for (int x = 0; x < V; ++x) acc[x] = fmaf(wk, v[k][x], acc[x]);
             }
         }
         if (together) {
@@ -160,13 +179,15 @@ __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_consta
                 }
             }
         }
-        if (!together || warp == 0) attn_merge_store<D>(a, own, r, V * lane, acc, L);
+        if (!together || warp == 0) attn_merge_store<D>(a, it, r, V * lane, acc, L);
         if (together) __syncthreads();                            // sums and tops are read
     }
 }
 
-int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s) {
-    const dim3 few(ctas, 4), many(ctas, rows / 8);
+int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, int unit, cudaStream_t s) {
+    // Sequences that can be no longer than a unit leave no parts: 11 us instead of 16 for a prompt of seven tokens.
+    if ((a.table ? (long long)a.max_pages << a.page_shift : (long long)a.total) <= unit) return JL_OK;
+    const dim3 few(ctas, ATTN_MERGE_BLOCKS), many(ctas, rows / 8);
     const cudaError_t e = rows == ATTN_FEW_ROWS
         ? (a.d == 128 ? attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 128>, few, dim3(256), 0, s, a, ctas)
                       : attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 64>, few, dim3(256), 0, s, a, ctas))
@@ -317,7 +338,7 @@ int check_pages(jl_ctx *ctx, const char *name, const jl_paged_kv *kv, jl_paged_k
 
 JL_EXPORT size_t jl_attn_scratch_bytes(jl_ctx *ctx) {
     if (!ctx) return 0;
-    const int few = ctx->sm_count * ATTN_FEW_CTAS;
+    const int few = attn_few_grid(ctx);
     const size_t f = (size_t)few * 2 * attn_slot_floats(ATTN_FEW_ROWS, 128), t = (size_t)ctx->sm_count * 2 * attn_slot_floats(ATTN_TC_ROWS, 128);
     return attn_meta_bytes(few) + (f > t ? f : t) * sizeof(float);
 }
@@ -343,7 +364,7 @@ JL_EXPORT int jl_attn_prompt(jl_ctx *ctx, void *out, int out_dtype, const void *
     a.nseq = nseq; a.total = total; a.hq = hq; a.hkv = hkv; a.g = hq / hkv; a.d = d;
     a.out_dtype = out_dtype; a.scale_log2 = scale * 1.4426950408889634f; a.status = ctx->dev_status;
     a.meta = static_cast<AttnMeta *>(scratch);
-    a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + attn_meta_bytes(ctx->sm_count * ATTN_FEW_CTAS));
+    a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + attn_meta_bytes(attn_few_grid(ctx)));
     rc = attn_launch(ctx, a, dtype, total, false, (cudaStream_t)stream);
     if (rc == JL_OK) ctx->st.served++;
     return rc;
@@ -373,7 +394,7 @@ JL_EXPORT int jl_attn_paged(jl_ctx *ctx, void *out, int out_dtype, const void *q
     a.page_shift = shift; a.n_pages = c.n_pages; a.max_pages = c.max_pages;
     a.out_dtype = out_dtype; a.scale_log2 = scale * 1.4426950408889634f; a.status = ctx->dev_status;
     a.meta = static_cast<AttnMeta *>(scratch);
-    a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + attn_meta_bytes(ctx->sm_count * ATTN_FEW_CTAS));
+    a.part = reinterpret_cast<float *>(static_cast<uint8_t *>(scratch) + attn_meta_bytes(attn_few_grid(ctx)));
     rc = attn_launch(ctx, a, c.dtype, max_new, c.n_seq > 1 && total < (long long)max_new * c.n_seq, (cudaStream_t)stream);
     if (rc == JL_OK) ctx->st.served++;
     return rc;

@@ -105,10 +105,12 @@ __host__ __device__ static inline AttnCut attn_cut_in(const AttnArgs &a, int s, 
 
 // What each CTA left in scratch. A CTA has at most two partial results: slot 0 continues an item that a CTA in front began,
 // slot 1 begins an item that the next one continues.
-struct AttnMeta {
-    int cont, ends;              // slot 0 holds a part; the item of slot 0 ends in this CTA
-    int own;                     // slot 1 holds the first part of an item
-    int row, ntok, head;         // of that item: its first row, its tokens, its kv head
+#define ATTN_CONT 1                  // slot 0 holds a part,
+#define ATTN_ENDS 2                  // and its item ends in this CTA
+#define ATTN_OWN 4                   // slot 1 holds the first part of an item
+struct __align__(16) AttnMeta {
+    int flags;
+    int row, ntok, head;             // of slot 1's item: its first row, its tokens, its kv head
 };
 __host__ __device__ static inline size_t attn_meta_bytes(int ctas) { return ((size_t)ctas * sizeof(AttnMeta) + 255) & ~(size_t)255; }
 
@@ -263,6 +265,7 @@ __device__ __forceinline__ void attn_store4(void *out, int dtype, size_t at, flo
 __host__ __device__ static inline size_t attn_slot_floats(int rows, int d) { return (size_t)rows * (d + 2); }
 #define ATTN_FEW_ROWS 16
 #define ATTN_FEW_CTAS 3          // to an SM
+#define ATTN_FEW_MAX 512         // in all: the join keeps 64 parts to each of eight warps
 #define ATTN_TC_ROWS 256         // or 128, and twice the CTAs
 
 // Launched so that the next kernel of the stream may be put in place while this one drains.
@@ -280,4 +283,8 @@ static cudaError_t attn_launch_pdl(void (*kern)(P...), dim3 grid, dim3 block, in
 int attn_launch_few(jl_ctx *ctx, const AttnArgs &a, int dtype, cudaStream_t s);
 // max_rows: query rows of a sequence and kv head, at most. JL_DECLINED: no tensor map for these strides
 int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &a, int dtype, long long max_rows, cudaStream_t s);
-int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, cudaStream_t s);
+// unit: positions below which no cut divides an item
+int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, int unit, cudaStream_t s);
+static inline int attn_few_grid(const jl_ctx *ctx) {
+    return ctx->sm_count * ATTN_FEW_CTAS < ATTN_FEW_MAX ? ctx->sm_count * ATTN_FEW_CTAS : ATTN_FEW_MAX;
+}

@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     AttnCut first, last;
     attn_share(a, blockIdx.x, gridDim.x, FEW_UNIT_SHIFT, min_units, first, last);
-    AttnMeta meta = {0, 0, 0, 0, 0, 0};
+    AttnMeta meta = {0, 0, 0, 0};
     AttnWalk walk;
     walk.begin(first, last);
     AttnSeg sg, ng;
@@ -294,8 +294,8 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
         if (!whole) {
             const int which = sg.u0 > 0 ? 0 : 1;
             slot = a.part + ((size_t)blockIdx.x * 2 + which) * attn_slot_floats(ATTN_FEW_ROWS, D);
-            if (which == 0) { meta.cont = 1; meta.ends = sg.u1 == sg.units; }
-            else { meta.own = 1; meta.row = sg.q.row + tok0; meta.ntok = ntok; meta.head = sg.head; }
+            if (which == 0) meta.flags |= ATTN_CONT | (sg.u1 == sg.units ? ATTN_ENDS : 0);
+            else { meta.flags |= ATTN_OWN; meta.row = sg.q.row + tok0; meta.ntok = ntok; meta.head = sg.head; }
         }
         for (int x = t; x < 16 * (D / 4); x += 128) {
             const int r = x / (D / 4), c = x % (D / 4);
@@ -330,13 +330,13 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
 
 template <int D, bool BF16>
 static int few_go(jl_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
-    const int smem = FewTile<D>::SMEM, grid = ctx->sm_count * ATTN_FEW_CTAS;
+    const int smem = FewTile<D>::SMEM, grid = attn_few_grid(ctx);
     auto kern = attn_few_kernel<D, BF16>;
     if (smem > 48 * 1024) JL_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const cudaError_t e = attn_launch_pdl(kern, dim3(grid), dim3(128), smem, s, a, FEW_MIN_UNITS);
     JL_CUDA(ctx, e);
     ctx->st.launches++;
-    return attn_launch_merge(ctx, a, ATTN_FEW_ROWS, grid, s);
+    return attn_launch_merge(ctx, a, ATTN_FEW_ROWS, grid, 1 << FEW_UNIT_SHIFT, s);
 }
 
 int attn_launch_few(jl_ctx *ctx, const AttnArgs &args, int dtype, cudaStream_t s) {

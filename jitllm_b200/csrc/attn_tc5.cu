@@ -35,8 +35,9 @@ template <int TILES> struct TaRoles {
 };
 #define TA_STATUS_CODE 7
 // What an item's start and end take against a unit: Q's arrival, the first S, the last product, the rows' way out; 10,000 clocks beside
-// 3250 of two tiles, 6000 beside 2900 of one.
-#define TA_ITEM_COST 4
+// 3250 of two tiles, 6000 beside 2900 of one. 24 prompts of 128 to 512 tokens take 71 us with 1, 64.5 with 2 and 3, 67 with 4; one of
+// 16,384 takes 2250, 2070, 2015 and 2020; shorter ones move by how the cuts happen to fall (1531: 54, 49, 54, 52).
+#define TA_ITEM_COST 3
 #define TA_ITEM_COST_ONE 2
 #define TA_SNAP 2
 // One tile up to as many rows as it has (five tokens of 8 heads: 50 us against 62 with a second tile idle); beyond, two: a 1531-token
@@ -552,7 +553,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         const float c = a.scale_log2;
         uint32_t tiles = 0, parts = 0, segs = 0;
         AttnMeta *const meta = a.meta + blockIdx.x;
-        if (threadIdx.x == 0) meta->cont = meta->ends = meta->own = 0;
+        int flags = 0;                                               // of thread 0
         while (const volatile TaSeg *t = seg_next()) {
             const int E = t->e[i], p_first = t->u0 * TA_KV;
             const int tok = i * tq + r / a.g;                        // of the item
@@ -685,8 +686,8 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 const int which = t->u0 > 0 ? 0 : 1;
                 slot = a.part + ((size_t)blockIdx.x * 2 + which) * attn_slot_floats(R::ROWS, D);
                 if (threadIdx.x == 0) {
-                    if (which == 0) { meta->cont = 1; meta->ends = t->ends; }
-                    else { meta->own = 1; meta->row = t->row + t->tok0; meta->ntok = t->ntok; meta->head = t->head; }
+                    if (which == 0) flags |= ATTN_CONT | (t->ends ? ATTN_ENDS : 0);
+                    else { flags |= ATTN_OWN; meta->row = t->row + t->tok0; meta->ntok = t->ntok; meta->head = t->head; }
                 }
                 if (live) {
                     slot[R::ROWS * D + row] = m * c;
@@ -754,6 +755,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             if (max(t->e[0], t->e[1]) > 0) segs++;
             seg_done();
         }
+        if (threadIdx.x == 0) meta->flags = flags;
     }
     tc5_fence_before();
     __syncthreads();
@@ -780,7 +782,7 @@ static int ta_go(jl_ctx *ctx, const AttnArgs &a, const CUtensorMap &q, const CUt
     const cudaError_t e = attn_launch_pdl(kern, dim3(grid), dim3(R::WARPS * 32), smem, s, a, q, k, v, box_rows, 2);
     JL_CUDA(ctx, e);
     ctx->st.launches++;
-    return attn_launch_merge(ctx, a, R::ROWS, grid, s);
+    return attn_launch_merge(ctx, a, R::ROWS, grid, TA_KV, s);
 }
 
 template <int D, int TILES>
