@@ -17,7 +17,9 @@
 // alone would need 2048. Tried and not kept: exponentials on the FMA pipe by a polynomial (it costs the scheduler what it saves the other
 // unit), rows split over two warps (the exchange of their maxima costs as much), S in halves of 64 positions with columns of their own
 // (the products S = Q K^T then read Q twice as often and take 1.5 times as long), an MMA warp to a tile (their products run side by side
-// and the tiles fall into step). A 16,384-token prompt of 32 heads over 8: 1.99 ms, 1.10 PFLOP/s, at the clock that the power limit leaves.
+// and the tiles fall into step), masked tiles on the short way (a second copy of it: registers spill, every case is 3 to 8 % slower).
+// A 16,384-token prompt of 32 heads over 8: 2.0 ms, 1.10 PFLOP/s, at the clock that the power limit leaves. Short prompts are bound by their
+// items' ends: a 1531-token one spends 2 x 10,000 of a CTA's 70,000 clocks on them (7000 on the rows' way out, the rest on masks).
 #include "attn.cuh"
 #include "tc5.cuh"
 
@@ -35,13 +37,16 @@ template <int TILES> struct TaRoles {
 };
 #define TA_STATUS_CODE 7
 // What an item's start and end take against a unit: Q's arrival, the first S, the last product, the rows' way out; 10,000 clocks beside
-// 3250 of two tiles, 6000 beside 2900 of one. 24 prompts of 128 to 512 tokens take 71 us with 1, 64.5 with 2 and 3, 67 with 4; one of
+// 3250 of two tiles, 6000 beside 2900 of one. 24 prompts of 1 to 1900 tokens take 71 us with 1, 64.5 with 2 and 3, 67 with 4; one of
 // 16,384 takes 2250, 2070, 2015 and 2020; shorter ones move by how the cuts happen to fall (1531: 54, 49, 54, 52).
 #define TA_ITEM_COST 3
 #define TA_ITEM_COST_ONE 2
-#define TA_SNAP 2
+// Two tiles: a cut one unit from an item's end moves onto it. The sliver that it saves costs its CTA 10,000 clocks; a cut further off,
+// moved, would cost the CTA next to it more (a 1531-token prompt 53 us with two units, 48.7 with one, 50 with none; 24 packed prompts 62.5,
+// 60.4, 62). One tile has less to save: 48.3 us with none, 50 to 53 with one for five tokens of 32 sequences.
+#define TA_SNAP 1
 // One tile up to as many rows as it has (five tokens of 8 heads: 50 us against 62 with a second tile idle); beyond, two: a 1531-token
-// prompt takes 52 us so and 60 as single tiles, whose CTAs load K and V each for itself.
+// prompt takes 49 us so and 60 as single tiles, whose CTAs load K and V each for itself.
 #define TA_ONE_TILE_ROWS 128
 #define TA_LIMIT 16384.f                 // of a tile's sum of weights: f16 holds each
 
@@ -797,7 +802,7 @@ int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &args, int dtype, long long max_
     const int tq = 128 / a.g, tiles = max_rows <= TA_ONE_TILE_ROWS ? 1 : 2;
     a.tok_item = tiles * tq;
     a.item_cost = tiles == 1 ? TA_ITEM_COST_ONE : TA_ITEM_COST;
-    a.snap = TA_SNAP;
+    a.snap = tiles == 1 ? 0 : TA_SNAP;
     const bool bf16 = dtype == JL_DT_BF16;
     CUtensorMap q, k, v;
     const cuuint64_t d = a.d;
