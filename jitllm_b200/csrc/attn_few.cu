@@ -18,7 +18,7 @@
 // In units, for 64 sequences of 37 to 8200 positions:
 #define FEW_ITEM_COST 4          // an item's start and end: 1, 2, 3 and 4 take 109, 98, 93 and 93 us
 #define FEW_SNAP 2               // 0, 2 and 6 take 95, 94 and 99 us
-#define FEW_MIN_UNITS 2          // of a share: 1, 2 and 4 take 17.1, 15.7 and 16.5 us for 2049 positions: a part more to join, or a unit more to read
+#define FEW_MIN_UNITS 2          // of a share: 1 and 2 take 17.1 and 15.7 us for 2049 positions: twice the parts to join
 
 template <int D> struct FewTile {
     static constexpr int ROW = 2 * D + 16;            // bytes of a staged row: padded, so that rows start in different banks

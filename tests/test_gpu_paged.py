@@ -232,6 +232,21 @@ def test_many_sequences(dev, new):
     _paged_case(dev, n, lens, 8, 2, 64, 32, _dt("bf16"), _dt("bf16"), 9, max_new=new)
 
 
+@pytest.mark.parametrize("hq,d,new,n", [(4, 128, 1, 70001), (8, 64, 2, 60000), (16, 64, 5, 20011), (16, 128, 20, 20011), (1, 64, 300, 40000)])
+def test_one_item_in_hundreds_of_parts(dev, hq, d, new, n):
+    """One kv head of one sequence: its few items are all the work, and each is divided over as many CTAs as there are."""
+    _paged_case(dev, [new], [n], hq, 1, d, 256, _dt("bf16"), _dt("f32"), n + new)
+    _paged_case(dev, [new, 1], [n, 900], hq, 1, d, 64, _dt("f16"), _dt("f16"), n)
+
+
+@pytest.mark.parametrize("new,lens", [([1] * 9, [48, 1, 33, 2, 16, 17, 47, 5, 40]), ([1] * 300, [1 + 7 * i % 48 for i in range(300)]),
+                                      ([20, 3, 48, 0, 9], [48, 3, 48, 12, 40]), ([100, 1, 112, 64], [100, 50, 112, 112])])
+def test_tables_no_longer_than_a_unit(dev, new, lens):
+    """No sequence can be longer than a unit of positions, so no item is divided and nothing is joined."""
+    _paged_case(dev, new, lens, 8, 2, 64, 16, _dt("f16"), _dt("f32"), len(new))
+    _paged_case(dev, new, lens, 8, 2, 128, 16, _dt("bf16"), _dt("bf16"), len(new) + 1)
+
+
 @pytest.mark.parametrize("max_new", [1, 24, None])
 def test_pages_behind_32_bits_of_elements(dev, max_new):
     """A pool of 2.7e9 elements, its last pages in use: the writer and the attention reach them."""

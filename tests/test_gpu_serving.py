@@ -115,3 +115,27 @@ def test_packed_prompts_are_scored_as_if_alone(dev):
                 _near(logits[s], _alone(dec, rows[at:at + n]))
             at += n
     assert dev.StatusPoll()
+
+
+@pytest.mark.parametrize("real,pad", [([1, 1, 1], 3), ([30, 1, 5], 12)])
+def test_rows_behind_the_last_request_reach_nothing(dev, real, pad):
+    """A step of a fixed number of rows, the last of them nobody's: whatever memory they start from, the requests' logits and the pool are
+    the same to the bit."""
+    import torch
+    dec = _decoder(dev)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rows = torch.randint(0, 2048, (sum(real) + pad,), device="cuda", generator=g)
+    table = torch.arange(12, device="cuda", dtype=torch.int32).view(3, 4)
+    got = []
+    with torch.no_grad():
+        for fill in (0.0, float("nan"), 1e30):
+            dec.open_pool(12, 16)
+            junk = [torch.full((n,), fill, device="cuda") for n in (1 << 10, 1 << 14, 1 << 17, 1 << 20)]      # what the step's tensors get
+            torch.cuda.synchronize()
+            del junk
+            dec.step_paged(rows, _starts(real), _i32(real), table, max(real))
+            got.append((dec.last_logits.clone(), dec.k_pool.clone(), dec.v_pool.clone()))
+        torch.cuda.synchronize()
+    assert bool(got[0][0].isfinite().all())
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
