@@ -62,46 +62,80 @@ __device__ __forceinline__ void attn_merge_load(const float *p, float (&v)[D / 3
 // Bound by the latency of loads that follow one another, 0.7 us each beside parts of a few MB that L2 serves: so everything whose address
 // is known is asked for at once, the maxima, the sums and the first parts' rows, and weighed once it is there.
 
-// Many rows and, as a rule, few parts: block (c, y) takes eight rows, a warp each.
+// Many rows and, as a rule, few parts: block (c, y) takes 16 rows, a warp two of them side by side. One row to a warp needs four waves of
+// blocks (prompts of 1531 tokens 48.9 us in all, of 24 requests 60.4; with two rows 47.4 and 58.9), four take registers from the loads'
+// overlap (49.1, 59.4; a long sequence of 37 parts 275 us instead of 253). More of the parts' rows ahead than two: the same (4: 48.9).
+#define ATTN_MERGE_ROWS 2
+#define ATTN_MERGE_AHEAD 2
 template <int D>
 __global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_constant__ AttnArgs a, int ctas, int slot_rows) {
-    constexpr int V = D / 32, B = 4;
+    constexpr int V = D / 32, B = ATTN_MERGE_AHEAD, R = ATTN_MERGE_ROWS;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int c = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int c = blockIdx.x, lane = threadIdx.x & 31, r0 = (blockIdx.y * 8 + (threadIdx.x >> 5)) * R;
     const AttnItem it = attn_item(a.meta, c, ctas);
-    if (r >= it.ntok * a.g || !it.n) return;
+    const int rows = min(R, it.ntok * a.g - r0);
+    if (!it.n || rows <= 0) return;
     const size_t slot = attn_slot_floats(slot_rows, D);
     auto part_of = [&](int k) { return a.part + ((size_t)(c + k) * 2 + (k == 0)) * slot; };
     auto there = [&](int k) { return k < it.n && (k < 32 ? it.flags : a.meta[c + k].flags & ATTN_CONT) != 0; };      // k % 32 == lane
-    auto top_of = [&](int k) { return there(k) ? __ldcg(part_of(k) + slot_rows * D + r) : -INFINITY; };
-    auto sum_of = [&](int k) { return there(k) ? __ldcg(part_of(k) + slot_rows * D + slot_rows + r) : 0.f; };
-    float v[B][V], m = top_of(lane), l = sum_of(lane), M = m;
+    float v[R][B][V], m[R], l[R], M[R], L[R], acc[R][V];
+    auto heads_of = [&](int k) {                                     // the rows' maxima and sums in part k
+        const bool has = there(k);
+        const float *p = part_of(k) + slot_rows * D + r0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            m[i] = has && i < rows ? __ldcg(p + i) : -INFINITY;
+            l[i] = has && i < rows ? __ldcg(p + slot_rows + i) : 0.f;
+        }
+    };
     auto rows_of = [&](int k0) {
 #pragma unroll
         for (int k = 0; k < B; ++k)
-            if (k0 + k < it.n) attn_merge_load<D>(part_of(k0 + k) + (size_t)r * D + V * lane, v[k]);
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (k0 + k < it.n && i < rows) attn_merge_load<D>(part_of(k0 + k) + (size_t)(r0 + i) * D + V * lane, v[i][k]);
     };
+    heads_of(lane);
     rows_of(0);
-    for (int k = 32 + lane; k < it.n; k += 32) M = fmaxf(M, top_of(k));
 #pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const float mu = M == -INFINITY ? 0.f : M;
-    float L = 0.f, acc[V] = {};
+    for (int i = 0; i < R; ++i) {
+        M[i] = m[i];
+        L[i] = 0.f;
+#pragma unroll
+        for (int x = 0; x < V; ++x) acc[i][x] = 0.f;
+    }
+    for (int k = 32 + lane; k < it.n; k += 32)
+        if (there(k)) {
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (i < rows) M[i] = fmaxf(M[i], __ldcg(part_of(k) + slot_rows * D + r0 + i));
+        }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) M[i] = fmaxf(M[i], __shfl_xor_sync(0xffffffffu, M[i], o));
+        M[i] = M[i] == -INFINITY ? 0.f : M[i];
+    }
     for (int k0 = 0; k0 < it.n; k0 += B) {
-        if (k0 && !(k0 & 31)) { m = top_of(k0 + lane); l = sum_of(k0 + lane); }
+        if (k0 && !(k0 & 31)) heads_of(k0 + lane);
         if (k0) rows_of(k0);
-        const float w = exp2f(m - mu);
 #pragma unroll
-        for (int k = 0; k < B; ++k) {
-            const float wk = __shfl_sync(0xffffffffu, w, (k0 + k) & 31), lk = __shfl_sync(0xffffffffu, l, (k0 + k) & 31);
-            if (k0 + k >= it.n || lk == 0.f) continue;            // the part holds nothing of this row, perhaps not even numbers
-            L = fmaf(wk, lk, L);
+        for (int i = 0; i < R; ++i) {
+            const float w = exp2f(m[i] - M[i]);
 #pragma unroll
-            for (int x = 0; x < V; ++x) acc[x] = fmaf(wk, v[k][x], acc[x]);
+            for (int k = 0; k < B; ++k) {
+                const float wk = __shfl_sync(0xffffffffu, w, (k0 + k) & 31), lk = __shfl_sync(0xffffffffu, l[i], (k0 + k) & 31);
+                if (k0 + k >= it.n || lk == 0.f) continue;        // the part holds nothing of this row, perhaps not even numbers
+                L[i] = fmaf(wk, lk, L[i]);
+#pragma unroll
+                for (int x = 0; x < V; ++x) acc[i][x] = fmaf(wk, v[i][k][x], acc[i][x]);
+            }
         }
     }
-    attn_merge_store<D>(a, it, r, V * lane, acc, L);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+        if (i < rows) attn_merge_store<D>(a, it, r0 + i, V * lane, acc[i], L[i]);
 }
 
 // Few rows: block (c, y) takes rows y, y + 8, ... of the item. A handful of parts: a warp to a row. Hundreds (a long sequence): the eight
@@ -187,7 +221,7 @@ __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_consta
 int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, int unit, cudaStream_t s) {
     // Sequences that can be no longer than a unit leave no parts: 11 us instead of 16 for a prompt of seven tokens.
     if ((a.table ? (long long)a.max_pages << a.page_shift : (long long)a.total) <= unit) return JL_OK;
-    const dim3 few(ctas, ATTN_MERGE_BLOCKS), many(ctas, rows / 8);
+    const dim3 few(ctas, ATTN_MERGE_BLOCKS), many(ctas, rows / (8 * ATTN_MERGE_ROWS));
     const cudaError_t e = rows == ATTN_FEW_ROWS
         ? (a.d == 128 ? attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 128>, few, dim3(256), 0, s, a, ctas)
                       : attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 64>, few, dim3(256), 0, s, a, ctas))
