@@ -77,6 +77,13 @@ def _tensor_code(t) -> int:
     return _dtype_code(t) if code is None else code
 
 
+def _tensor_ptr(t) -> int:
+    """_ptr of what is known to be a torch tensor."""
+    if not t.is_contiguous():
+        raise ValueError("tensor must be contiguous")
+    return t.data_ptr()
+
+
 class Weight:
     """A weight (or expert bank) resident on the device: jl_weight."""
 
@@ -422,8 +429,8 @@ class Device:
         if nseq < 1 or total == 0:
             return
         self._check(self.lib.jl_attn_prompt(self.ctx, out.data_ptr(), _tensor_code(out), q.data_ptr(), qt, qh, k.data_ptr(), v.data_ptr(), kt,
-                                            kh, _tensor_code(q), _ptr(starts), nseq, total, hq, hkv, d, d ** -0.5 if scale is None else scale,
-                                            _ptr(scratch), scratch.numel() * scratch.element_size(), stream))
+                                            kh, _tensor_code(q), _tensor_ptr(starts), nseq, total, hq, hkv, d, d ** -0.5 if scale is None else scale,
+                                            _tensor_ptr(scratch), scratch.numel() * scratch.element_size(), stream))
 
     def AttnPaged(self, out, q, kv: PagedKV, starts, lens, scratch, max_new: int | None = None, scale: float | None = None,
                   stream: int = 0) -> None:
@@ -440,9 +447,9 @@ class Device:
         self._on_device(out, q, kv.k, starts, lens, scratch)
         if kv.n_seq == 0 or total == 0:
             return
-        self._check(self.lib.jl_attn_paged(self.ctx, out.data_ptr(), _tensor_code(out), q.data_ptr(), qt, qh, kv.ref, _ptr(starts), _ptr(lens),
-                                           total, total if max_new is None else max_new, hq, d ** -0.5 if scale is None else scale,
-                                           _ptr(scratch), scratch.numel() * scratch.element_size(), stream))
+        self._check(self.lib.jl_attn_paged(self.ctx, out.data_ptr(), _tensor_code(out), q.data_ptr(), qt, qh, kv.ref, _tensor_ptr(starts),
+                                           _tensor_ptr(lens), total, total if max_new is None else max_new, hq, d ** -0.5 if scale is None else scale,
+                                           _tensor_ptr(scratch), scratch.numel() * scratch.element_size(), stream))
 
     def RopeAppend(self, q_out, qkv, kv: PagedKV, starts, lens, cos, sin, stream: int = 0) -> None:
         """The cache's writer: rows of qkv [total][(hq + 2 n_kv) * d] (f32, f16 or bf16) are the sequences' new rows, at the positions
@@ -453,15 +460,16 @@ class Device:
             raise ValueError("q_out must be contiguous and have the cache's head size and type")
         if qkv.shape != (total, (hq + 2 * kv.n_kv) * d):
             raise ValueError("qkv must be [total][(hq + 2 n_kv) * d]")
-        if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[1] * 2 != d or _tensor_code(cos) or _tensor_code(sin):
+        shape, f32 = cos.shape, _torch().float32
+        if shape != sin.shape or len(shape) != 2 or shape[1] * 2 != d or cos.dtype is not f32 or sin.dtype is not f32:
             raise ValueError("cos and sin must be f32 [positions][d / 2]")
         self._seqs("starts", starts, kv.n_seq + 1)
         self._seqs("lens", lens, kv.n_seq)
         self._on_device(q_out, qkv, kv.k, starts, lens, cos, sin)
         if kv.n_seq == 0 or total == 0:
             return
-        self._check(self.lib.jl_rope_append(self.ctx, q_out.data_ptr(), _ptr(qkv), _tensor_code(qkv), kv.ref, _ptr(starts), _ptr(lens), total, hq,
-                                            _ptr(cos), _ptr(sin), cos.shape[0], stream))
+        self._check(self.lib.jl_rope_append(self.ctx, q_out.data_ptr(), _tensor_ptr(qkv), _tensor_code(qkv), kv.ref, _tensor_ptr(starts),
+                                            _tensor_ptr(lens), total, hq, _tensor_ptr(cos), _tensor_ptr(sin), shape[0], stream))
 
     # The checks below run at every call of a decode step: they ask a tensor for as little as they can.
     @staticmethod
