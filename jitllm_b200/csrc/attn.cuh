@@ -58,7 +58,7 @@ __host__ __device__ static inline int attn_limit(const AttnSeq &q, int t1) {
 // The work is a line of items -- (sequence, block of tok_item tokens, kv head), heads innermost -- and item i is as long on it as
 // the positions that it walks plus item_cost units for its start and end. The line is cut into equal shares, one to a CTA,
 // the cuts rounded to whole units of positions inside an item; an item that a cut divides leaves a partial result in each CTA,
-// and attn_merge_kernel joins them in ascending order of positions. A few long sequences thus fill the GPU as well as many short
+// and the join (attn.cu) adds them up in ascending order of positions. A few long sequences thus fill the GPU as well as many short
 // ones, whatever the lengths, which only the device knows; results depend on the cuts in their rounding and on nothing else.
 
 struct AttnCut { int seq, blk, head, unit; };     // before `unit` of item (seq, blk, head); seq == nseq: the line's end
