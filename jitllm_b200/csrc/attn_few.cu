@@ -11,6 +11,8 @@
 // Measured: 64 sequences of 37 to 8200 positions, 32 heads over 8, 408 MB: 88 us, 4.6 TB/s. The loop itself reads at 6.0 TB/s (long
 // sequences of equal length, 1.3 GB: 5.4 TB/s with everything); the rest is the share's start (4 us: lengths, table, first tiles, one after the
 // other), items' starts and ends, the last CTAs' 8 us and the join (6 us). Few positions are latency: 2049 of one sequence take 15.7 us.
+// Tried and not kept: a ring that runs on into the next item while this one's sums are joined, 16 columns at a time (the join of the warps
+// costs what the loads save, the other CTAs of the SM fill the gap anyway: 89 us).
 #include "attn.cuh"
 
 #define FEW_UNIT_SHIFT 6
