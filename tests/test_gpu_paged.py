@@ -277,6 +277,34 @@ def test_pages_behind_32_bits_of_elements(dev, max_new):
     _check(out, ref, mag, size, torch.bfloat16, 200, d)
 
 
+def test_calls_side_by_side(dev):
+    """Calls on two streams, each with its own scratch, in graphs that are replayed at the same time: the bits of one call alone."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(21)
+    lens = [900, 33, 4000, 1, 257]
+    pool = Pool(lens, 2, 64, 32, _dt("bf16"), 22)
+    work = []
+    for new in ([1] * 5, [40, 3, 300, 1, 9], [5] * 3 + [1, 5], [1] * 5):
+        q = torch.randn(sum(new), 8, 64, generator=g, device="cuda").bfloat16()
+        out = torch.zeros_like(q)
+        args = (out, q, pool.kv, _starts(new), torch.tensor(lens, dtype=torch.int32, device="cuda"), _scratch(dev))
+        dev.AttnPaged(*args, max_new=max(new), stream=torch.cuda.current_stream().cuda_stream)
+        torch.cuda.synchronize()
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            dev.AttnPaged(*args, max_new=max(new), stream=stream.cuda_stream)
+        work.append((out, out.clone(), args, stream, graph))
+    for out, *_ in work:
+        out.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for _, _, _, stream, graph in work:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, alone) for out, alone, *_ in work) and dev.StatusPoll()
+
+
 def test_sequences_may_share_pages(dev):
     import torch
     pool = Pool([200, 200], 2, 64, 32, _dt("f16"), 2)
