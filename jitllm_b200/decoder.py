@@ -39,6 +39,18 @@ def random_q4k(rng: np.random.Generator, nrows: int, k: int) -> np.ndarray:
     return blk.reshape(nrows, (k // 256) * 144)
 
 
+def packed_positions(starts, n: int):
+    """Position of each of n packed rows in its prompt (prompt s is rows starts[s] .. starts[s + 1] - 1), int64 [n]. Rows behind the last
+    prompt are nobody's: 0."""
+    import torch
+    nseq = starts.shape[0] - 1
+    if nseq < 1:
+        raise ValueError("starts must name one prompt at least: [n_seq + 1]")
+    row = torch.arange(n, device=starts.device, dtype=torch.int32)
+    seq = torch.searchsorted(starts[1:].contiguous(), row, right=True)
+    return torch.where(seq < nseq, row - starts[seq.clamp_max(nseq - 1)], torch.zeros_like(row)).long()
+
+
 class Decoder:
     def __init__(self, dev, cfg: Config, max_batch: int, max_len: int, rank: int = 0, world: int = 1, seed: int = 0xB204,
                  group=None, max_prefill: int = 2048, keep_host: bool = False, share_full: bool = False):
@@ -82,9 +94,8 @@ class Decoder:
         self.norm_w = torch.ones(c.hidden, device="cuda")
         self.k_cache = torch.zeros(c.n_layer, max_batch, self.hkv, max_len, d, device="cuda", dtype=torch.bfloat16)
         self.v_cache = torch.zeros_like(self.k_cache)
-        inv = 1.0 / (c.rope_theta ** (torch.arange(0, d, 2, device="cuda").float() / d))
-        ang = torch.arange(max_len, device="cuda").float()[:, None] * inv[None, :]
-        self.cos, self.sin = ang.cos(), ang.sin()
+        self.inv_freq = 1.0 / (c.rope_theta ** (torch.arange(0, d, 2, device="cuda").float() / d))
+        self.cos, self.sin = self._rotation(torch.arange(max_len, device="cuda"))
         dev.Reserve(max(2 * self.ffn_l, self.vocab_l, c.hidden), max(c.hidden, self.ffn_l, self.hq * d), max(max_batch, max_prefill))
         self.weight_bytes = sum(w.nrows * (w.k // 256) * 144 for l in self.layers for w in l.values()) + \
             self.head.nrows * (self.head.k // 256) * 144
@@ -112,22 +123,27 @@ class Decoder:
     def _rms(self, x):
         return x * self.torch.rsqrt((x * x).mean(-1, keepdim=True) + self.cfg.eps) * self.norm_w
 
-    def _rope(self, t, pos):
-        """t [n][heads][d]; pos [n] int64 positions."""
-        cos, sin = self.cos[pos][:, None, :], self.sin[pos][:, None, :]
+    def _rotation(self, pos):
+        """cos and sin [n][d / 2] of positions [n]: what the tables hold for those below max_len, and the same for any other."""
+        ang = pos.float()[:, None] * self.inv_freq[None, :]
+        return ang.cos(), ang.sin()
+
+    def _rope(self, t, rot):
+        """t [n][heads][d]; rot: the rows' cos and sin, [n][d / 2] each."""
+        cos, sin = rot[0][:, None, :], rot[1][:, None, :]
         a, b = t[..., 0::2], t[..., 1::2]
         return self.torch.stack((a * cos - b * sin, a * sin + b * cos), dim=-1).flatten(-2)
 
-    def _layers(self, x, pos, attend):
-        """The layer stack over n rows x [n][hidden] f32. pos [n] int64 gives each row's position (RoPE);
+    def _layers(self, x, rot, attend):
+        """The layer stack over n rows x [n][hidden] f32. rot: the rows' cos and sin (_rope);
         attend(li, q [n][hq][d], k [n][hkv][d], v [n][hkv][d]) -> [n][hq*d] stores k, v and attends."""
         torch, c = self.torch, self.cfg
         import torch.nn.functional as F
         n, d = x.shape[0], c.head_dim
         for li, l in enumerate(self.layers):
             qkv = self.mm(l["qkv"], self._rms(x))
-            q = self._rope(qkv[:, :self.hq * d].view(n, self.hq, d), pos)
-            k = self._rope(qkv[:, self.hq * d:(self.hq + self.hkv) * d].view(n, self.hkv, d), pos)
+            q = self._rope(qkv[:, :self.hq * d].view(n, self.hq, d), rot)
+            k = self._rope(qkv[:, self.hq * d:(self.hq + self.hkv) * d].view(n, self.hkv, d), rot)
             v = qkv[:, (self.hq + self.hkv) * d:].view(n, self.hkv, d)
             att = attend(li, q.to(torch.bfloat16), k.to(torch.bfloat16), v.to(torch.bfloat16))
             x = x + self._allreduce(self.mm(l["o"], att.float()))
@@ -163,7 +179,7 @@ class Decoder:
 
         x = self._prefill_chain(tokens)
         if x is None:
-            x = self._layers(self.emb[tokens].float(), pos, attend)[-1:]
+            x = self._layers(self.emb[tokens].float(), (self.cos[pos], self.sin[pos]), attend)[-1:]
         return self._argmax(x)
 
     def _gemm_operand(self, w, n):
@@ -297,13 +313,12 @@ class Decoder:
 
     def score_packed(self, tokens, starts):
         """The next token after each of several packed prompts, without a cache: tokens [N] int64, prompt s is rows starts[s] ..
-        starts[s + 1] - 1 (int32 device tensor). Returns [n_seq]; that of an empty prompt has no meaning."""
+        starts[s + 1] - 1 (int32 device tensor); rows behind the last prompt are nobody's. Without a cache there is no limit on a
+        prompt's length but N. Returns [n_seq]; that of an empty prompt has no meaning."""
         torch, c = self.torch, self.cfg
         n, d = tokens.shape[0], c.head_dim
         st = torch.cuda.current_stream().cuda_stream
-        row = torch.arange(n, device="cuda", dtype=torch.int32)
-        seq = torch.searchsorted(starts[1:].contiguous(), row, right=True).clamp_max(starts.shape[0] - 2)
-        pos = (row - starts[seq]).long()
+        rot = self._rotation(packed_positions(starts, n))
         out = torch.empty(n, self.hq, d, device="cuda", dtype=torch.bfloat16)
         scratch = self._attn_scratch()
 
@@ -311,7 +326,7 @@ class Decoder:
             self.dev.AttnPrompt(out, q, k, v, starts, scratch, stream=st)
             return out.view(n, -1)
 
-        x = self._layers(self.emb[tokens].float(), pos, attend)
+        x = self._layers(self.emb[tokens].float(), rot, attend)
         return self._argmax(x[(starts[1:] - 1).clamp_min(0).long()])
 
     def decode_step(self, tokens, pos_dev):
@@ -450,5 +465,6 @@ class Decoder:
                                                attn_mask=mask)
             return o.reshape(B, -1)
 
-        x = self._layers(self.emb[tokens].float(), pos_dev.expand(B), attend)
+        pos = pos_dev.expand(B)
+        x = self._layers(self.emb[tokens].float(), (self.cos[pos], self.sin[pos]), attend)
         return self._argmax(x)

@@ -1,0 +1,44 @@
+"""The decoder's serving calls at the edges of what they allow: rows that are nobody's, prompts and contexts longer than the tables."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _decoder(dev, max_len=256, max_prefill=512):
+    from jitllm_b200.decoder import Config, Decoder
+    cfg = Config(n_layer=2, hidden=512, n_head=4, n_kv=2, head_dim=128, ffn=1024, vocab=2048)
+    return Decoder(dev, cfg, max_batch=3, max_len=max_len, max_prefill=max_prefill, seed=11)
+
+
+def _i32(x):
+    import torch
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _starts(new):
+    at = [0]
+    for n in new:
+        at.append(at[-1] + n)
+    return _i32(at)
+
+
+def _tokens(n, seed):
+    import torch
+    return torch.randint(0, 2048, (n,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+
+
+@pytest.mark.parametrize("new,rows", [([100], 512), ([30, 0, 7], 300), ([300], 300), ([10, 400], 500)])
+def test_packed_scores_do_not_depend_on_the_tables(dev, new, rows):
+    """Rows behind the last prompt and prompts longer than max_len: the bits of a decoder whose tables hold every position."""
+    import torch
+    tokens, starts, got = _tokens(rows, 5), _starts(new), []
+    with torch.no_grad():
+        for max_len in (64, 512):
+            dec = _decoder(dev, max_len)
+            nxt = dec.score_packed(tokens, starts)
+            got.append((nxt, dec.last_logits.clone()))
+        torch.cuda.synchronize()
+    live = [s for s, n in enumerate(new) if n]
+    assert bool(got[0][1][live].isfinite().all())
+    assert torch.equal(got[0][1][live], got[1][1][live]) and torch.equal(got[0][0][live], got[1][0][live])
+    assert dev.StatusPoll()
