@@ -167,6 +167,8 @@ class Decoder:
         torch = self.torch
         import torch.nn.functional as F
         T = tokens.shape[0]
+        if not 1 <= T <= self.max_len:
+            raise ValueError(f"a prompt of {T} tokens: 1 to max_len = {self.max_len} fit the caches")
         pos = torch.arange(T, device="cuda")
         g = self.hq // self.hkv
 

@@ -34,3 +34,12 @@ def test_rotation_is_that_of_the_tables_and_goes_on_behind_them():
             assert torch.equal(c[i], cos[p]) and torch.equal(s[i], sin[p])
     ang = 500.0 * dec.inv_freq.double()
     assert float((c[3] - ang.cos()).abs().max()) < 500 * 2.0 ** -23 and float((s[3] - ang.sin()).abs().max()) < 500 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("n", [0, 65, 4000])
+def test_a_prompt_that_does_not_fit_the_caches_is_refused(n):
+    """On the host, before the positions index a table."""
+    dec = decoder.Decoder.__new__(decoder.Decoder)
+    dec.torch, dec.max_len = torch, 64
+    with pytest.raises(ValueError, match="max_len"):
+        dec.prefill(torch.zeros(n, dtype=torch.int64))
