@@ -51,6 +51,12 @@ def packed_positions(starts, n: int):
     return torch.where(seq < nseq, row - starts[seq.clamp_max(nseq - 1)], torch.zeros_like(row)).long()
 
 
+def last_rows(starts, n: int):
+    """Row of each sequence's last new token among n rows, int64 [n_seq]. Whatever starts holds, an index of n rows: a sequence without
+    rows, or one whose rows were cut off at n, gets a row that is not its own."""
+    return (starts[1:] - 1).clamp(0, n - 1).long()
+
+
 class Decoder:
     def __init__(self, dev, cfg: Config, max_batch: int, max_len: int, rank: int = 0, world: int = 1, seed: int = 0xB204,
                  group=None, max_prefill: int = 2048, keep_host: bool = False, share_full: bool = False):
@@ -310,8 +316,7 @@ class Decoder:
             return out.view(n, -1)
 
         x, delta = self._chain(tokens, op, attend)
-        last = (starts[1:] - 1).clamp_min(0).long()
-        return self._argmax((x + delta)[last])
+        return self._argmax((x + delta)[last_rows(starts, n)])
 
     def score_packed(self, tokens, starts):
         """The next token after each of several packed prompts, without a cache: tokens [N] int64, prompt s is rows starts[s] ..
@@ -329,7 +334,7 @@ class Decoder:
             return out.view(n, -1)
 
         x = self._layers(self.emb[tokens].float(), rot, attend)
-        return self._argmax(x[(starts[1:] - 1).clamp_min(0).long()])
+        return self._argmax(x[last_rows(starts, n)])
 
     def decode_step(self, tokens, pos_dev):
         """tokens [B] int64, one per sequence, all at position pos_dev (a 1-element int64 DEVICE tensor,

@@ -18,6 +18,12 @@ def test_positions_of_packed_rows(starts, n):
     assert decoder.packed_positions(_i32(starts), n).tolist() == want
 
 
+@pytest.mark.parametrize("starts,n,want", [([0, 3, 3, 10], 12, [2, 2, 9]), ([0, 0, 5], 5, [0, 4]), ([0, 4, 900], 8, [3, 7]), ([0, -7, 8], 8, [0, 7])])
+def test_last_rows_are_rows(starts, n, want):
+    """Starts that pass the rows or fall below zero index none outside them."""
+    assert decoder.last_rows(_i32(starts), n).tolist() == want
+
+
 def test_starts_without_a_prompt_are_refused():
     with pytest.raises(ValueError):
         decoder.packed_positions(_i32([0]), 4)

@@ -42,3 +42,23 @@ def test_packed_scores_do_not_depend_on_the_tables(dev, new, rows):
     assert bool(got[0][1][live].isfinite().all())
     assert torch.equal(got[0][1][live], got[1][1][live]) and torch.equal(got[0][0][live], got[1][0][live])
     assert dev.StatusPoll()
+
+
+def test_starts_behind_the_rows_index_none(dev):
+    """A last sequence that claims more rows than there are: the others' results, and no index out of range."""
+    import torch
+    dec = _decoder(dev)
+    dec.open_pool(40, 16)
+    table = torch.arange(40, device="cuda", dtype=torch.int32).view(2, 20)
+    tokens = _tokens(40, 6)
+    with torch.no_grad():
+        dec.score_packed(tokens, _starts([20, 20]))
+        want = dec.last_logits[0].clone()
+        dec.score_packed(tokens, _i32([0, 20, 900]))
+        assert torch.equal(dec.last_logits[0], want)
+        dec.step_paged(tokens, _starts([20, 20]), _i32([20, 20]), table, 20)
+        want = dec.last_logits[0].clone()
+        dec.step_paged(tokens, _i32([0, 20, 900]), _i32([20, 20]), table, 20)
+        assert torch.equal(dec.last_logits[0], want)
+        torch.cuda.synchronize()
+    assert dev.StatusPoll()
