@@ -282,23 +282,24 @@ class Decoder:
     # -- several requests at once ---------------------------------------------------
     def open_pool(self, n_pages: int, page_len: int) -> None:
         """A pool of cache pages for step_paged, beside the per-sequence caches: every layer has its own pages under the same numbers,
-        so that one page table serves the whole stack. Pages hold a power of two from 16 to 1024 positions."""
+        so that one page table serves the whole stack. Pages hold a power of two from 16 to 1024 positions. Opening it again replaces the pages:
+        steps captured over the old ones must not be replayed."""
         torch, c = self.torch, self.cfg
         self.k_pool = torch.zeros(c.n_layer, n_pages, self.hkv, page_len, c.head_dim, device="cuda", dtype=torch.bfloat16)
         self.v_pool = torch.zeros_like(self.k_pool)
-        self._paged_scratch = torch.empty(self.dev.AttnScratchBytes(), device="cuda", dtype=torch.uint8)
 
     def _attn_scratch(self):
-        if getattr(self, "_paged_scratch", None) is None:
-            self._paged_scratch = self.torch.empty(self.dev.AttnScratchBytes(), device="cuda", dtype=self.torch.uint8)
-        return self._paged_scratch
+        """Scratch of one step's attention calls, which follow one another. Every step has its own, as it has its other tensors: an eager
+        one from its stream's memory, a captured one from its graph's, which lives as long as the graph does."""
+        return self.torch.empty(self.dev.AttnScratchBytes(), device="cuda", dtype=self.torch.uint8)
 
     def step_paged(self, tokens, starts, lens, table, max_new: int):
         """One step of several requests over the pool: prompts, chunks of prompts and single tokens in any mixture. tokens [N] int64:
         rows starts[s] .. starts[s + 1] - 1 are sequence s's new tokens; lens[s] its positions with them; table [n_seq][max_pages] its
         pages (int32 device tensors; the caller hands out pages for the new positions beforehand). max_new: the most new tokens of any
         sequence. Returns the next token of every sequence [n_seq]; that of a sequence without new tokens has no meaning. Allocates
-        nothing but tensors, so that a step of fixed N can be captured and replayed on other lengths and tables."""
+        nothing but tensors, so that a step of fixed N can be captured and replayed on other lengths and tables. Steps of one Decoder, on
+        whatever streams or in whatever graphs, must not overlap: their matmuls share the Device's one operand (jl_gemm_operand)."""
         from .device import PagedKV
         torch, c = self.torch, self.cfg
         n, d = tokens.shape[0], c.head_dim

@@ -62,3 +62,57 @@ def test_starts_behind_the_rows_index_none(dev):
         assert torch.equal(dec.last_logits[0], want)
         torch.cuda.synchronize()
     assert dev.StatusPoll()
+
+
+def test_a_captured_step_keeps_its_scratch(dev):
+    """Scores captured before the pool is opened (again), replayed after it while other tensors come and go: the same bits, and nobody
+    else's memory is written."""
+    import torch
+    dec = _decoder(dev)
+    rows, starts = _tokens(300, 7), _starts([200, 100])
+    with torch.no_grad():
+        dec.score_packed(rows, starts)
+        want = dec.last_logits.clone()
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            dec.score_packed(rows, starts)
+            logits = dec.last_logits
+        for _ in range(2):
+            dec.open_pool(40, 16)
+            guard = [torch.full((dev.AttnScratchBytes(),), 7, device="cuda", dtype=torch.uint8) for _ in range(3)]
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(logits, want) and all(bool((g == 7).all()) for g in guard)
+    assert dev.StatusPoll()
+    graph.reset()
+
+
+def test_no_two_steps_have_one_scratch(dev):
+    """Two captured steps, an eager one on another stream and one on this: none has the scratch of another that is still to run."""
+    import torch
+    dec = _decoder(dev)
+    dec.open_pool(40, 16)
+    at, real = [], dec._attn_scratch
+
+    def watched():
+        at.append(real())
+        return at[-1]
+    dec._attn_scratch = watched
+    table = torch.arange(40, device="cuda", dtype=torch.int32).view(2, 20)
+    args = (_tokens(2, 8), _starts([1, 1]), _i32([1, 1]), table, 1)
+    graphs = []
+    with torch.no_grad():
+        dec.step_paged(*args)
+        for _ in range(2):
+            graphs.append(torch.cuda.CUDAGraph())
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graphs[-1]):
+                dec.step_paged(*args)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            dec.step_paged(*args)
+        torch.cuda.synchronize()
+    assert len({t.data_ptr() for t in at}) == 4
+    for g in graphs:
+        g.reset()
