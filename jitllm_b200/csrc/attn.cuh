@@ -42,7 +42,11 @@ __host__ __device__ static inline AttnSeq attn_seq(const AttnArgs &a, int s) {
     q.over = 0;
     if (a.table) {
         const long long cap = (long long)a.max_pages << a.page_shift;
-        if (len > cap) { len = (int)cap; q.over = 1; }
+        if (len > cap) {                          // its rows walk the table (and come out NaN); neither pos0 nor a weight passes it
+            len = (int)cap;
+            q.pos0 = q.pos0 < len ? q.pos0 : len;
+            q.over = 1;
+        }
     }
     q.len = len;
     const long long rows = (long long)q.n * a.g;
@@ -74,7 +78,7 @@ __host__ __device__ static inline long long attn_item_weight(const AttnSeq &q, i
 // Sum of the weights of blocks [0, i) of a sequence, i <= ceil(n / T); for one head.
 __host__ __device__ static inline long long attn_blocks_weight(const AttnSeq &q, int i, int T, int cost) {
     if (i <= 0) return 0;
-    const long long base = (long long)i * (cost + (q.pos0 > 0 ? q.pos0 : 0));
+    const long long base = (long long)i * ((long long)cost + (q.pos0 > 0 ? q.pos0 : 0));
     const long long whole = (long long)T * i * (i + 1) / 2;
     const long long over = (long long)i * T - q.n;           // of the last block, if it is the ragged one
     return base + whole - (over > 0 ? over : 0);

@@ -129,3 +129,15 @@ def test_entry_points_refuse_without_a_context():
     assert L.jl_rope_append(None, 16, 16, 0, C.byref(kv), 16, 16, 1, 1, 16, 16, 1, None) == _lib.EINVAL
     s = np.zeros(2, np.int32)
     assert L.jl_test_attn_share(s.ctypes.data, None, 0, 1, 1, 1, 6, 1, 6, 0, 1, 0, s.ctypes.data, 0) == _lib.EINVAL
+
+
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 257, 2 ** 30 + 1, 5000])
+def test_a_length_beyond_its_table_takes_no_more_than_the_table(length):
+    """One sequence claims more positions than its table holds: it weighs what the table holds, and the others get their shares of the
+    grid. (The claimed length would take all of it; near 2^31 its sum with an item's cost left 32 bits.)"""
+    starts, lens = [0, 1, 2, 3], [1280, length, 1280]                    # tables of 20 pages of 64
+    shares = _shares(starts, lens, 3, 8, 4, 6, 2, 6, 20, 100)
+    work = [sum(u1 - u0 for _, _, _, u0, u1, _ in segs) for segs in shares]
+    assert sum(work) == 3 * 8 * 20 and max(work) <= 1.15 * sum(work) / len(work) + 2
+    for s in (0, 1, 2):
+        assert len([c for c, segs in enumerate(shares) if any(g[0] == s for g in segs)]) >= 20
