@@ -297,7 +297,9 @@ class Decoder:
         """One step of several requests over the pool: prompts, chunks of prompts and single tokens in any mixture. tokens [N] int64:
         rows starts[s] .. starts[s + 1] - 1 are sequence s's new tokens; lens[s] its positions with them; table [n_seq][max_pages] its
         pages (int32 device tensors; the caller hands out pages for the new positions beforehand). max_new: the most new tokens of any
-        sequence. Returns the next token of every sequence [n_seq]; that of a sequence without new tokens has no meaning. Allocates
+        sequence. Returns the next token of every sequence [n_seq]; that of a sequence without new tokens has no meaning. Positions from
+        max_len on are not served, whatever the table holds: a sequence whose last row sits there has NaN logits and the next token -1, as
+        has one with a page number outside the pool or a length beyond its table. Allocates
         nothing but tensors, so that a step of fixed N can be captured and replayed on other lengths and tables. Steps of one Decoder, on
         whatever streams or in whatever graphs, must not overlap: their matmuls share the Device's one operand (jl_gemm_operand)."""
         from .device import PagedKV
@@ -306,7 +308,7 @@ class Decoder:
         st = torch.cuda.current_stream().cuda_stream
         operands = self._gemm_operands(n)
         op = operands if n >= 9 and self.ffn_l <= 50 * 1024 else lambda w: None
-        q = torch.empty(n, self.hq, d, device="cuda", dtype=torch.bfloat16)
+        q = torch.full((n, self.hq, d), float("nan"), device="cuda", dtype=torch.bfloat16)      # and so it stays where RopeAppend leaves a row out
         out = torch.empty(n, self.hq, d, device="cuda", dtype=torch.bfloat16 if n >= 9 else torch.float32)
         scratch = self._attn_scratch()
 
@@ -317,7 +319,13 @@ class Decoder:
             return out.view(n, -1)
 
         x, delta = self._chain(tokens, op, attend)
-        return self._argmax((x + delta)[last_rows(starts, n)])
+        last = last_rows(starts, n)
+        nxt = self._argmax((x + delta)[last])
+        # The attention's row of a sequence that has no result is NaN, in the last layer as in the first; the matmuls' operands are made of
+        # integers and do not pass that on.
+        bad = out[last, 0, 0].isnan()
+        self.last_logits.masked_fill_(bad[:, None], float("nan"))
+        return torch.where(bad, -1, nxt)
 
     def score_packed(self, tokens, starts):
         """The next token after each of several packed prompts, without a cache: tokens [N] int64, prompt s is rows starts[s] ..

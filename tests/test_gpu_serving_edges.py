@@ -116,3 +116,48 @@ def test_no_two_steps_have_one_scratch(dev):
     assert len({t.data_ptr() for t in at}) == 4
     for g in graphs:
         g.reset()
+
+
+@pytest.mark.parametrize("new,lens", [([1], [65]), ([1, 1, 1], [64, 65, 30]), ([2, 1, 2], [66, 90, 64]), ([12, 3, 1], [70, 40, 64]), ([40, 1, 20], [100, 10, 20])])
+def test_positions_behind_the_tables_are_not_numbers(dev, new, lens):
+    """A request that grows past max_len while its pages go on: NaN logits and the token -1 instead of a plausible one; the requests beside it
+    have the bits of a decoder whose tables go on, too."""
+    import torch
+    got = []
+    full = [_tokens(n, 20 + i) for i, n in enumerate(lens)]
+    with torch.no_grad():
+        for max_len in (64, 512):
+            dec = _decoder(dev, max_len)
+            dec.open_pool(24, 16)
+            table = torch.arange(24, device="cuda", dtype=torch.int32).view(3, 8)[:len(lens)].contiguous()
+            dec.k_pool.normal_(generator=torch.Generator(device="cuda").manual_seed(1))      # what an earlier owner of the pages left
+            dec.v_pool.normal_(generator=torch.Generator(device="cuda").manual_seed(2))
+            if any(n > m for n, m in zip(lens, new)):
+                rest = [n - m for n, m in zip(lens, new)]
+                dec.step_paged(torch.cat([f[:r] for f, r in zip(full, rest)]), _starts(rest), _i32(rest), table, max(rest))
+            junk = [torch.randn(1 << k, device="cuda") for k in (10, 14, 17, 20)]            # what the step's tensors get
+            torch.cuda.synchronize()
+            del junk
+            nxt = dec.step_paged(torch.cat([f[n - m:] for f, n, m in zip(full, lens, new)]), _starts(new), _i32(lens), table, max(new))
+            got.append((nxt.tolist(), dec.last_logits.clone()))
+        torch.cuda.synchronize()
+    for s, n in enumerate(lens):
+        if n > 64:
+            assert bool(got[0][1][s].isnan().all()) and got[0][0][s] == -1
+        else:
+            assert torch.equal(got[0][1][s], got[1][1][s]) and got[0][0][s] == got[1][0][s] >= 0
+        assert bool(got[1][1][s].isfinite().all())
+    assert dev.StatusPoll()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 12])
+def test_a_bad_page_has_no_next_token(dev, rows):
+    import torch
+    dec = _decoder(dev)
+    dec.open_pool(8, 16)
+    table = torch.tensor([[0, 1], [2, 99]], device="cuda", dtype=torch.int32)
+    tokens = _tokens(2 * rows, 30)
+    with torch.no_grad():
+        nxt = dec.step_paged(tokens, _starts([rows, rows]), _i32([20, 20]), table, rows)
+        torch.cuda.synchronize()
+    assert nxt[0].item() >= 0 and nxt[1].item() == -1 and bool(dec.last_logits[0].isfinite().all())
