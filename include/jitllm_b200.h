@@ -440,7 +440,8 @@ typedef struct jl_paged_kv {
     const int32_t *page_table;           /* device [n_seq][max_pages] */
 } jl_paged_kv;
 /* lens[s] positions of sequence s are in the cache (int32, device), the last of them its new rows': new row i of n sits at position
- * lens[s] - n + i and sees the positions up to its own. A row before position 0 sees nothing: its result is zero. A page number outside
+ * lens[s] - n + i and sees the positions up to its own. A row before position 0 sees nothing: its result is zero; that of a row whose
+ * scores are all -inf is NaN (0 / 0). A page number outside
  * the pool, or a length beyond the table, is never followed: the results of the rows that read there are NaN, and so may be the
  * sequence's other rows. max_new: the most new rows that any sequence has, as far as the host knows; it picks the kernel, not the
  * result. */

@@ -80,6 +80,7 @@ __global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_const
     auto part_of = [&](int k) { return a.part + ((size_t)(c + k) * 2 + (k == 0)) * slot; };
     auto there = [&](int k) { return k < it.n && (k < 32 ? it.flags : a.meta[c + k].flags & ATTN_CONT) != 0; };      // k % 32 == lane
     float v[R][B][V], m[R], l[R], M[R], L[R], acc[R][V];
+    bool dark[R];
     auto heads_of = [&](int k) {                                     // the rows' maxima and sums in part k
         const bool has = there(k);
         const float *p = part_of(k) + slot_rows * D + r0;
@@ -102,6 +103,7 @@ __global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_const
     for (int i = 0; i < R; ++i) {
         M[i] = m[i];
         L[i] = 0.f;
+        dark[i] = __shfl_sync(0xffffffffu, l[i], 0) < 0.f;           // said by the first part, which every row that sees anything sees
 #pragma unroll
         for (int x = 0; x < V; ++x) acc[i][x] = 0.f;
     }
@@ -126,7 +128,7 @@ __global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_const
 #pragma unroll
             for (int k = 0; k < B; ++k) {
                 const float wk = __shfl_sync(0xffffffffu, w, (k0 + k) & 31), lk = __shfl_sync(0xffffffffu, l[i], (k0 + k) & 31);
-                if (k0 + k >= it.n || lk == 0.f) continue;        // the part holds nothing of this row, perhaps not even numbers
+                if (k0 + k >= it.n || lk <= 0.f) continue;        // the part holds nothing of this row, perhaps not even numbers
                 L[i] = fmaf(wk, lk, L[i]);
 #pragma unroll
                 for (int x = 0; x < V; ++x) acc[i][x] = fmaf(wk, v[i][k][x], acc[i][x]);
@@ -135,7 +137,7 @@ __global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_const
     }
 #pragma unroll
     for (int i = 0; i < R; ++i)
-        if (i < rows) attn_merge_store<D>(a, it, r0 + i, V * lane, acc[i], L[i]);
+        if (i < rows) attn_merge_store<D>(a, it, r0 + i, V * lane, acc[i], dark[i] && L[i] == 0.f ? __int_as_float(0x7fffffff) : L[i]);
 }
 
 // Few rows: block (c, y) takes rows y, y + 8, ... of the item. A handful of parts: a warp to a row. Hundreds (a long sequence): the eight
@@ -184,6 +186,7 @@ __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_consta
 #pragma unroll
             for (int i = 0; i < 8; ++i) M = fmaxf(M, tops[i]);
         }
+        const bool dark = lo == 0 && __shfl_sync(0xffffffffu, l[0], 0) < 0.f;        // of the first part: every row that sees anything sees it
         const float mu = M == -INFINITY ? 0.f : M;
         const float w0 = exp2f(m[0] - mu), w1 = exp2f(m[1] - mu);
         float L = 0.f, acc[V] = {};
@@ -193,7 +196,7 @@ __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_consta
             for (int k = 0; k < B; ++k) {
                 const float wk = __shfl_sync(0xffffffffu, k0 < 32 ? w0 : w1, (k0 + k) & 31);
                 const float lk = __shfl_sync(0xffffffffu, k0 < 32 ? l[0] : l[1], (k0 + k) & 31);
-                if (lo + k0 + k >= hi || lk == 0.f) continue;     // the part holds nothing of the row, perhaps not even numbers
+                if (lo + k0 + k >= hi || lk <= 0.f) continue;     // the part holds nothing of the row, perhaps not even numbers
                 L = fmaf(wk, lk, L);
 #pragma unroll
                 for (int x = 0; x < V; ++x) acc[x] = fmaf(wk, v[k][x], acc[x]);
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_consta
                 }
             }
         }
-        if (!together || warp == 0) attn_merge_store<D>(a, it, r, V * lane, acc, L);
+        if (!together || warp == 0) attn_merge_store<D>(a, it, r, V * lane, acc, dark && L == 0.f ? __int_as_float(0x7fffffff) : L);
         if (together) __syncthreads();                            // sums and tops are read
     }
 }

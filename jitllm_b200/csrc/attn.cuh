@@ -265,7 +265,10 @@ __device__ __forceinline__ void attn_store4(void *out, int dtype, size_t at, flo
 }
 #endif
 
-// A partial result in scratch: [rows][d] weighted sums of V, then [rows] maxima (base 2, scaled), then [rows] sums, all f32.
+// A partial result in scratch: [rows][d] weighted sums of V, then [rows] maxima (base 2, scaled), then [rows] sums, all f32. A row that sees
+// nothing has the maximum -inf and the sum 0, and its result is zero. One that sees positions whose scores are all -inf has the maximum
+// -inf too, but no result (0 / 0): its sum is ATTN_DARK, which no part's weight multiplies, and if no part has more, its result is NaN.
+#define ATTN_DARK (-1.f)
 __host__ __device__ static inline size_t attn_slot_floats(int rows, int d) { return (size_t)rows * (d + 2); }
 #define ATTN_FEW_ROWS 16
 #define ATTN_FEW_CTAS 3          // to an SM

@@ -316,9 +316,11 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
                 const float4 v = *reinterpret_cast<const float4 *>(&red[w][r][4 * c]);
                 s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
             }
+            const int tk = r / a.g;
+            if (L == 0.f && tk < ntok && attn_limit(sg.q, tok0 + tk + 1) > 0)       // sees positions, and each of its scores is -inf
+                L = whole ? __int_as_float(0x7fffffff) : ATTN_DARK;
             if (bad || sg.q.over) L = __int_as_float(0x7fffffff);   // a page outside the pool, positions outside the table: NaN
             if (whole) {
-                const int tk = r / a.g;
                 if (tk < ntok) {
                     const float inv = L == 0.f ? 0.f : 1.f / L;     // a row that sees nothing is zero
                     if (L == 0.f) s = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -674,8 +674,9 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 if (lane == 0) mbar_arrive(p_full + 8 * i);
             }
             if (!ok) break;
-            if (m == -INFINITY) l = 0.f;                             // sees nothing
             const bool whole = t->whole;
+            // sees nothing; or sees positions, and each of its scores is -inf
+            if (m == -INFINITY) l = seen + p_first <= 0 ? 0.f : (whole ? __int_as_float(0x7fffffff) : ATTN_DARK);
             bool odd = false;
             if (E > 0) {
                 ok = __all_sync(0xffffffffu, ta_wait(o_full + 8 * i, parts & 1, abort_flag));
