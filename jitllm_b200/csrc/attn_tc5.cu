@@ -48,7 +48,13 @@ template <int TILES> struct TaRoles {
 // One tile up to as many rows as it has (five tokens of 8 heads: 50 us against 62 with a second tile idle); beyond, two: a 1531-token
 // prompt takes 49 us so and 60 as single tiles, whose CTAs load K and V each for itself.
 #define TA_ONE_TILE_ROWS 128
-#define TA_LIMIT 16384.f                 // of a tile's sum of weights: f16 holds each
+// log2 of a weight at the reference, and the limit of a tile's sum of weights. f16 ends at 2^-24 and at 65504: with weights of one at the
+// reference a long flat tail below 2^-25 of it would leave the products but not the sum (131,071 positions: 0.4 % of a result). At 2^6 a
+// weight is held to 2^-31 and may still grow by 2^10 over the reference; at 2^8 more tiles pass the limit (f16, 24 packed prompts 63.2 us
+// against 60.3, one of 1531 tokens 52.4 against 48.7). f32 results take the weights to a maximum that is exact, and so to 2^14.
+template <bool BF16, bool HILO> struct TaWeights {
+    static constexpr float LOG_TOP = BF16 ? 0.f : HILO ? 14.f : 6.f, LIMIT = BF16 ? 16384.f : 65504.f;
+};
 
 // The bounded wait of this kernel's roles. A try that may sleep for up to 20 us: the warps that wait are many, and their polling would take
 // the issue slots of those that work.
@@ -269,6 +275,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 const __grid_constant__ CUtensorMap vmap, int box_rows, int min_units) {
     using L = TaSmem<D, TILES>;
     using R = TaRoles<TILES>;
+    using W = TaWeights<BF16, HILO>;
     constexpr int TM_O = TILES * 128;                       // O's columns in TMEM, behind S's
     extern __shared__ uint8_t raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -548,10 +555,10 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         // ------------------------------------------------ softmax: warpgroup i owns tile i, a thread one of its rows
         // The weights of a tile are taken to a reference of the tiles before it, without looking for the tile's own maximum first (250
         // clocks): nothing is lost as long as they stay in range, and their sum, which is taken anyway, says whether they do. A row's
-        // first reference is the largest of its first 16 scores. Where the sum passes TA_LIMIT (or is NaN), and in masked tiles, S is
-        // read for its maximum, O rescaled -- S's arrival tells that the product before it is complete -- and the weights taken to that:
-        // S stays whole until P is written over it. The sums and products are f32, so scaled by up to TA_LIMIT they lose nothing. The two
-        // ways are kept apart: a loop around one of them, or masks in it, cost 100 to 470 clocks a tile.
+        // first reference is the largest of its first 16 scores (f16: of its first tile's). Where the sum passes the limit (or is NaN), in masked tiles, and for f32
+        // results of f16, S is read for its maximum, O rescaled -- S's arrival tells that the product before it is complete -- and the weights
+        // taken to that: S stays whole until P is written over it. The sums and products are f32, so scaled by up to the limit they lose
+        // nothing. The two ways are kept apart: a loop around one of them, or masks in it, cost 100 to 470 clocks a tile.
         const int i = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // 32 lanes a warp, in bits 16 and up of a TMEM address
         const uint32_t S = tmem + i * 128 + lanes, O = tmem + TM_O + i * 128 + lanes;
@@ -585,6 +592,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                         tc5_fma2(u, w, __uint_as_float(v[2 * y]), __uint_as_float(v[2 * y + 1]), c, mc);
                         u = ta_exp2(u);
                         w = ta_exp2(w);
+                        if constexpr (!BF16 && HILO) { u *= 16384.f; w *= 16384.f; }       // 2^LOG_TOP, exact; else mc holds it
                         ta_add2(sum[y & 1], u, w);
                         hi[y] = ta_pack<BF16>(u, w);
                         if constexpr (HILO) {
@@ -593,8 +601,10 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                         }
                     }
                 };
-                bool slow = masked;
-                if (j == 0 && !masked) {                             // any of a row's scores may be the first reference
+                // what the scores' exponents start from
+                auto minus = [&](float ref) { return ref == -INFINITY ? 0.f : BF16 || HILO ? -ref * c : fmaf(-ref, c, W::LOG_TOP); };
+                bool slow = masked || (HILO && !BF16);
+                if (BF16 && j == 0 && !masked) {                             // any of a row's scores may be the first reference
                     uint32_t v[16];
                     tc5_ld16(S, v);
                     ta_wait_ld(v);
@@ -611,11 +621,22 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     for (int x = 0; x < 4; ++x) tc5_ld32(S + 32 * x, s[x]);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) ta_wait_ld(s[x]);
-                    const float mc = m == -INFINITY ? 0.f : -m * c;
+                    if (!BF16 && j == 0) {                           // f16 has less room over the reference: the largest of the tile
+                        float top[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            top[x] = __uint_as_float(s[x][0]);
+#pragma unroll
+                            for (int y = 1; y < 32; ++y) top[x] = fmaxf(top[x], __uint_as_float(s[x][y]));
+                        }
+                        m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                        if (!(m < INFINITY)) m = 0.f;
+                    }
+                    const float mc = minus(m);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) weights(s[x], mc, sum, hi[x], lo[HILO ? x : 0]);
                     const float total = (sum[0][0] + sum[1][0]) + (sum[0][1] + sum[1][1]);
-                    slow = __any_sync(0xffffffffu, live && m == m && (!(total <= TA_LIMIT) || (m == -INFINITY && total > 0.f)));
+                    slow = __any_sync(0xffffffffu, live && m == m && (!(total <= W::LIMIT) || (m == -INFINITY && total > 0.f)));
                     if (!slow) {
                         l += total;
 #pragma unroll
@@ -657,7 +678,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                             ta_st16(O + 16 * x, o);
                         }
                     }
-                    const float mc = m == -INFINITY ? 0.f : -m * c;
+                    const float mc = minus(m);
                     float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {

@@ -68,3 +68,46 @@ def test_scores_that_are_all_minus_infinity_have_no_result(dev, dt, d, out, new,
             first = max(0, m + new - n)                                    # rows that see infinite keys alone
             assert first == 0 or bool(got[:first].isnan().all())
             _check(got[first:], ref[first:], mag[first:], size[first:], _dt(dt), n, d)
+
+
+@pytest.mark.parametrize("out", ["f32", "f16"])
+@pytest.mark.parametrize("hq,hkv,d,new,n,exponent", [(8, 2, 128, 1, 131072, 18.1), (8, 8, 64, [1] * 70, 2500, 17.4), (8, 1, 64, 2, 70001, 17.4), (4, 2, 128, 40, 60000, 17.4),
+                                                     (8, 4, 64, 300, 40000, 17.4), (16, 1, 128, 1, 5000, 15.3), (8, 2, 64, 33, 3000, 15.3)])
+def test_a_long_flat_tail_keeps_its_weight(dev, out, hq, hkv, d, new, n, exponent):
+    """f16, one position far above all others (by e^exponent, 2^22 to 2^26): together the others weigh up to a part in 500, each of them
+    less than half of f16's smallest step beside one. The large position's value is zero, so that the tail is the result.
+    A weight is held to 2^-39 of the largest, or to 2^-31 where many rows have 16-bit results: n times that of the largest value beside
+    the tolerance of the other tests (without its allowance of n 2^-25 for this)."""
+    import torch
+    from jitllm_b200 import PagedKV
+    each = new if isinstance(new, list) else [new]                          # one sequence whose parts are joined, or many whole ones
+    new = sum(each)
+    pool = Pool([n], hkv, d, 64, torch.float16, 5)
+    k, v = pool.rows[0]
+    k.zero_()
+    k[3, :, 0] = 1.0
+    v.abs_().add_(0.25)
+    v[3] = 0
+    p = torch.arange(n, device="cuda")
+    page = pool.table[0].long()[p // 64]
+    pool.k[page, :, p % 64], pool.v[page, :, p % 64] = k, v
+    kv = PagedKV(pool.k, pool.v, pool.table.expand(len(each), -1).contiguous())
+    q = torch.randn(new, hq, d, device="cuda").half()
+    q[..., 0] = exponent
+    res = torch.full((new, hq, d), 7.0, device="cuda", dtype=_dt(out))
+    dev.AttnPaged(res, q, kv, _starts(each), _i32([n] * len(each)), _scratch(dev), max_new=max(each), scale=1.0, stream=_stream())
+    torch.cuda.synchronize()
+    assert dev.StatusPoll()
+    if len(each) > 1:
+        ref, mag, size = (torch.cat(x) for x in zip(*(_reference(q[i:i + 1], k, v, n - 1, 1.0) for i in range(new))))
+    else:
+        ref, mag, size = _reference(q, k, v, n - new, 1.0)
+    few = max(each) * hq // hkv <= 16
+    w = 2.0 ** -22 if few or out == "f32" else 2.0 ** -11
+    floor = 2.0 ** -39 if few or out == "f32" else 2.0 ** -31
+    e = size * (d * 2.0 ** -23 + 2.0 ** -22) + 2.0 ** -22
+    tol = mag * (w + 2 * e + (128 + n / 128) * 2.0 ** -23) + n * floor * float(v.max())
+    h = torch.finfo(_dt(out))
+    tol = tol + ref.abs() * h.eps / 2 + h.smallest_normal * h.eps / 2
+    bad = (res.double() - ref).abs() > tol
+    assert not bool(bad.any()), float(((res.double() - ref).abs() / tol).max())
