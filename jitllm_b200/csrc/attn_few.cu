@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
     walk.begin(first, last);
     AttnSeg sg, ng;
     if (t == 0) bad = 0;
+    const bool third = a.out_dtype == JL_DT_F32;       // of a weight's bf16 parts
     const uint16_t *kp = static_cast<const uint16_t *>(a.k), *vp = static_cast<const uint16_t *>(a.v);
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(tiles) + warp * FEW_STAGES * TILE;
     // the page of the warp's tile i: 16 positions lie in one (pages are 16 positions at least, cut at multiples of their length)
@@ -213,9 +214,9 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
                         l[e] += s;
                     }
             }
-            // A fragments of the weights, as value + remainder (16 significant bits of bf16, 22 of f16): the products with V lose
-            // nothing that an f32 result shows
-            uint32_t ph[4], pl[4];
+            // A fragments of the weights, as value + remainder (16 significant bits of bf16, 22 of f16), and for f32 results of bf16
+            // the remainder's remainder (24): the products with V lose nothing that the result shows
+            uint32_t ph[4], pl[4], pt[4];
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
@@ -223,6 +224,7 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
                     float rx, ry, z0, z1;
                     ph[2 * nt + e] = few_pack<BF16>(sv[nt][2 * e], sv[nt][2 * e + 1], rx, ry);
                     pl[2 * nt + e] = few_pack<BF16>(rx, ry, z0, z1);
+                    if constexpr (BF16) { float y0, y1; pt[2 * nt + e] = few_pack<BF16>(z0, z1, y0, y1); }
                 }
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
@@ -255,6 +257,10 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
                     few_mma<BF16>(oacc[2 * jp], pl, b0, b1);
                     few_mma<BF16>(oacc[2 * jp + 1], ph, b2, b3);
                     few_mma<BF16>(oacc[2 * jp + 1], pl, b2, b3);
+                    if (BF16 && third) {
+                        few_mma<BF16>(oacc[2 * jp], pt, b0, b1);
+                        few_mma<BF16>(oacc[2 * jp + 1], pt, b2, b3);
+                    }
                 }
             } else {
 #pragma unroll 1

@@ -111,3 +111,45 @@ def test_a_long_flat_tail_keeps_its_weight(dev, out, hq, hkv, d, new, n, exponen
     tol = tol + ref.abs() * h.eps / 2 + h.smallest_normal * h.eps / 2
     bad = (res.double() - ref).abs() > tol
     assert not bool(bad.any()), float(((res.double() - ref).abs() / tol).max())
+
+
+def _exact_scores(rows, hq, hkv, d, n, dt, seed):
+    """q, k, v whose scores, at a scale of log 2, are multiples of 1/32 up to 4 that no product or sum rounds."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def steps(k, *shape):
+        return torch.randint(0, k + 1, shape, generator=g, device="cuda")
+    q, k = torch.zeros(rows, hq, d, device="cuda", dtype=dt), torch.zeros(n, hkv, d, device="cuda", dtype=dt)
+    q[..., 0] = (steps(16, rows, hq) / 8).to(dt)                           # up to 2, in eighths
+    k[..., 0] = (steps(8, n, hkv) / 4).to(dt)                              # up to 2, in quarters
+    v = torch.randn(n, hkv, d, generator=g, device="cuda").to(dt)
+    return q, k, v
+
+
+def _weights_of_24_bits(got, ref, mag, n):
+    """f32 results of exact scores. Of A = sum p|v| / sum p: 2^-22 for a weight as 16-bit parts; its exponent, twice (in the sum and in the
+    product): 2^-22 of the exponential, 4 * 2^-24 of the scale's two roundings at exponents up to 4, 2^-23 of their product's; n + 8 additions
+    in f32 that may truncate, 2^-23 each; 3 * 2^-24 for the quotient."""
+    tol = mag * (2.0 ** -22 + 2 * (2.0 ** -22 + 4 * 2.0 ** -24 + 2.0 ** -23) + (n + 8) * 2.0 ** -23 + 3 * 2.0 ** -24) + 1e-30
+    bad = (got.double() - ref).abs() > tol
+    assert not bool(bad.any()), float(((got.double() - ref).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 8, 128), (12, 4, 64), (16, 1, 128)])
+def test_f32_results_of_few_rows_carry_f32_weights(dev, dt, hq, hkv, d):
+    """A weight in two bf16 values would be off by up to 2^-16."""
+    import torch
+    from jitllm_b200 import PagedKV
+    lens, scale = [8, 7, 5, 2, 1, 8, 6, 3] * 8, float(torch.tensor(2.0).log())
+    q, k, v = _exact_scores(len(lens), hq, hkv, d, 8 * len(lens), _dt(dt), 3)
+    pk, pv = (torch.zeros(len(lens), hkv, 16, d, device="cuda", dtype=_dt(dt)) for _ in range(2))
+    pk[:, :, :8], pv[:, :, :8] = (x.view(len(lens), 8, hkv, d).transpose(1, 2) for x in (k, v))
+    table = torch.arange(len(lens), device="cuda", dtype=torch.int32)[:, None].contiguous()
+    out = torch.empty(len(lens), hq, d, device="cuda")
+    dev.AttnPaged(out, q, PagedKV(pk, pv, table), _starts([1] * len(lens)), _i32(lens), _scratch(dev), max_new=1, scale=scale, stream=_stream())
+    torch.cuda.synchronize()
+    for s, n in enumerate(lens):
+        ref, mag, _ = _reference(q[s:s + 1], k[8 * s:8 * s + n], v[8 * s:8 * s + n], n - 1, scale)
+        _weights_of_24_bits(out[s:s + 1], ref, mag, n)
