@@ -410,7 +410,10 @@ int jl_matmul_dev_prepared(jl_ctx *ctx, void *out_dev, int out_dtype, const jl_w
  * Attention of grouped query heads (query head h reads kv head h / (hq / n_kv)), causal within each sequence:
  *   out[r][h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale q[r][h] . k_j - max),   j = 0 .. r's own position
  * q, k and v are f16 or bf16 (one type), sums and softmax f32. out [total][hq][d] is f32, f16 or bf16; for an f32 result the softmax
- * weights enter the product with V as two 16-bit values, for a 16-bit one as one (half a unit of that type at most on each).
+ * weights enter the product with V with 22 bits (f16) or 24 (bf16), as two or three 16-bit values; for a 16-bit result of more than sixteen
+ * query rows to a kv head as one (half a unit of the type of q at most on each), of fewer as two. Beside this, a weight of f16 is held to
+ * 2^-39 of the row's largest (where it is one value, 2^-31). The sums over many positions are those of the tensor cores' f32 accumulators, which
+ * truncate: results of one sign come out low by 7e-7 of themselves at 2048 positions, 4e-6 to 7e-6 at 8192.
  * Served: d of 64 and 128, hq / n_kv up to 16.
  *
  * The sequences are described on the device, so that a captured graph can be replayed on other lengths: new rows of sequence s are rows
@@ -443,8 +446,8 @@ typedef struct jl_paged_kv {
  * lens[s] - n + i and sees the positions up to its own. A row before position 0 sees nothing: its result is zero; that of a row whose
  * scores are all -inf is NaN (0 / 0). A page number outside
  * the pool, or a length beyond the table, is never followed: the results of the rows that read there are NaN, and so may be the
- * sequence's other rows. max_new: the most new rows that any sequence has, as far as the host knows; it picks the kernel, not the
- * result. */
+ * sequence's other rows. max_new: the most new rows that any sequence has, as far as the host knows; it picks the kernel, and whatever it
+ * says every row has its result: to the roundings above, which are the kernel's. */
 int jl_attn_paged(jl_ctx *ctx, void *out_dev, int out_dtype, const void *q_dev, long long q_tok_stride, long long q_head_stride,
                   const jl_paged_kv *kv, const int32_t *starts_dev, const int32_t *lens_dev, int total, int max_new, int hq, float scale,
                   void *scratch_dev, size_t scratch_bytes, void *stream);

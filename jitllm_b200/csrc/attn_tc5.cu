@@ -12,6 +12,11 @@
 // a warp each that issues the products, that loads (K and V tiles of 128 positions through one ring by TMA, a box to a page and 64
 // columns; Q once an item), that looks over the V tiles at a sequence's edge, and that walks the CTA's share.
 //
+// An f32 result takes a weight as two f16 values or three bf16 values (S's columns hold two: the third goes over the first once the product
+// with that is done, while the product with the second runs), to a maximum that is looked for. A third more products: bf16, five tokens of
+// 32 sequences 72 us (two parts: 60), a prompt of 1531 tokens 71 (67), of 16,384 3750 (2635); errors 1e-7 to 8e-7 of relative rms up to
+// 1500 positions, 8e-7 to 2e-6 with two. Both tiles' first parts in front of both thirds: 4430 us, the tiles fall into step.
+//
 // What bounds it: a tile's round of 128 positions, 1450 clocks of softmax (1290 of a loop of nothing else, of them 1024 exponentials), 300
 // for S, P and the barriers to change hands, 1024 of products: 3250 clocks as counted with two tiles at work, where the tensor core
 // alone would need 2048. Tried and not kept: exponentials on the FMA pipe by a polynomial (it costs the scheduler what it saves the other
@@ -51,9 +56,10 @@ template <int TILES> struct TaRoles {
 // log2 of a weight at the reference, and the limit of a tile's sum of weights. f16 ends at 2^-24 and at 65504: with weights of one at the
 // reference a long flat tail below 2^-25 of it would leave the products but not the sum (131,071 positions: 0.4 % of a result). At 2^6 a
 // weight is held to 2^-31 and may still grow by 2^10 over the reference; at 2^8 more tiles pass the limit (f16, 24 packed prompts 63.2 us
-// against 60.3, one of 1531 tokens 52.4 against 48.7). f32 results take the weights to a maximum that is exact, and so to 2^14.
+// against 60.3, one of 1531 tokens 52.4 against 48.7). f32 results take the weights to a maximum that is known, and so to 2^14.
 template <bool BF16, bool HILO> struct TaWeights {
     static constexpr float LOG_TOP = BF16 ? 0.f : HILO ? 14.f : 6.f, LIMIT = BF16 ? 16384.f : 65504.f;
+    static constexpr float ROOM = BF16 ? 14.f : 1.f;         // log2 of what a weight of an f32 result may pass 2^LOG_TOP by
 };
 
 // The bounded wait of this kernel's roles. A try that may sleep for up to 20 us: the warps that wait are many, and their polling would take
@@ -227,9 +233,9 @@ template <int D, int TILES> struct TaSmem {
     static constexpr int STAGES = (D == 128 ? 2 : 4) * TILES;
     static constexpr int PASS = D == 128 && TILES == 1 ? 64 : 128;       // bytes of a row that leave at a time
     static constexpr int Q = 0, KV = TILES * TILE, OUT = KV + STAGES * TILE, BARS = OUT + 4 * TILES * 32 * PASS;     // OUT: 32 rows of PASS bytes to a softmax warp
-    // barriers: kv_full[STAGES], kv_empty[STAGES], q_full, q_empty, s_full[2], p_full[2], o_full[2], drain, v_ok[OKS], e_full[OKS], g_full[TA_SEGS], g_empty[TA_SEGS]
+    // barriers: kv_full[STAGES], kv_empty[STAGES], q_full, q_empty, s_full[2], p_full[2], o_full[2], drain, v_ok[OKS], e_full[OKS], g_full[TA_SEGS], g_empty[TA_SEGS], h_used[2]
     static constexpr int OKS = D == 128 ? 4 : 8;              // more than the V tiles that the ring can hold
-    static constexpr int NBARS = 2 * STAGES + 9 + 2 * OKS + 2 * TA_SEGS;
+    static constexpr int NBARS = 2 * STAGES + 11 + 2 * OKS + 2 * TA_SEGS;
     static constexpr int SEGS = (BARS + NBARS * 8 + 15) & ~15;
     static constexpr int MISC = SEGS + TA_SEGS * (int)sizeof(TaSeg);      // tmem address, abort flag and limit, seg_bad[4], seg_odd[4]
     static constexpr int TOTAL = MISC + 64 + 1024;           // 1024: the tiles start on a swizzle atom
@@ -276,13 +282,14 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     using L = TaSmem<D, TILES>;
     using R = TaRoles<TILES>;
     using W = TaWeights<BF16, HILO>;
+    constexpr bool THIRD = BF16 && HILO;                    // a weight has three parts; the third goes over the first once that is used
     constexpr int TM_O = TILES * 128;                       // O's columns in TMEM, behind S's
     extern __shared__ uint8_t raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sbase = smem_u32(smem), bars = sbase + L::BARS;
     const uint32_t kv_full = bars, kv_empty = bars + 8 * L::STAGES, q_full = bars + 16 * L::STAGES, q_empty = q_full + 8, s_full = q_full + 16,
                    p_full = q_full + 32, o_full = q_full + 48, drain = q_full + 64, v_ok = q_full + 72, e_full = v_ok + 8 * L::OKS, g_full = e_full + 8 * L::OKS,
-                   g_empty = g_full + 8 * TA_SEGS;
+                   g_empty = g_full + 8 * TA_SEGS, h_used = g_empty + 8 * TA_SEGS;
     volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(smem + L::MISC);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::MISC + 4);        // [0] flag, [1] limit
     volatile int *seg_bad = reinterpret_cast<volatile int *>(smem + L::MISC + 16), *seg_odd = seg_bad + 4;
@@ -296,6 +303,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             mbar_init(s_full + 8 * i, 1);
             mbar_init(p_full + 8 * i, 4);                   // one arrival a softmax warp
             mbar_init(o_full + 8 * i, 1);
+            mbar_init(h_used + 8 * i, 1);
         }
         for (int i = 0; i < 2 * L::OKS; ++i) mbar_init(v_ok + 8 * i, 1);       // and e_full
         for (int i = 0; i < TA_SEGS; ++i) { mbar_init(g_full + 8 * i, 1); mbar_init(g_empty + 8 * i, R::SOFT + 3); }     // all but the walk
@@ -444,25 +452,38 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     ok = __all_sync(0xffffffffu, ta_wait(kv_full + 8 * sv, (it / L::STAGES) & 1, abort_flag));
                 }
                 if (ok && j + 1 < E) ok = __all_sync(0xffffffffu, ta_wait(kv_full + 8 * sk, ((it + 1) / L::STAGES) & 1, abort_flag));
-#pragma unroll
-                for (int i = 0; i < TILES; ++i) {
+                const uint64_t v = vd + sv * (L::TILE >> 4);
+                // O of tile i += P V, P's first part and (HILO) second, or its third; with the last part S of the next unit, or the segment's end
+                auto product = [&](int i, bool first, bool last) {
                     const int e = i ? e1 : e0;
-                    if (!ok || j >= e) continue;
+                    if (!ok || j >= e) return;
                     ok = __all_sync(0xffffffffu, ta_wait(p_full + 8 * i, done[i] & 1, abort_flag));
-                    if (!ok) continue;
+                    if (!ok) return;
                     tc5_fence_after();
                     if (leader) {
-                        const uint64_t v = vd + sv * (L::TILE >> 4);
                         const uint32_t p = tm + i * 128, o = tm + TM_O + i * 128;
+                        auto part = [&](int x, int at, bool fresh) {         // 16 positions of the part in columns `at`
+                            ta_mma_ts(o, p + 32 * (x >> 1) + at + 8 * (x & 1), v + x * (2048 >> 4), id_o, !fresh);
+                        };
 #pragma unroll
                         for (int x = 0; x < TA_KV / 16; ++x) {
-                            ta_mma_ts(o, p + 32 * (x >> 1) + 8 * (x & 1), v + x * (2048 >> 4), id_o, j != 0 || x != 0);
-                            if constexpr (HILO) ta_mma_ts(o, p + 32 * (x >> 1) + 16 + 8 * (x & 1), v + x * (2048 >> 4), id_o, 1);
+                            part(x, 0, first && j == 0 && x == 0);
+                            if constexpr (HILO && !THIRD) part(x, 16, false);
                         }
-                        if (j + 1 < e) scores(i, sk);
+                        if (!last) {                                         // the third part comes while the product with the second runs
+                            tc5_commit(h_used + 8 * i);
+#pragma unroll
+                            for (int x = 0; x < TA_KV / 16; ++x) part(x, 16, false);
+                        }
+                        else if (j + 1 < e) scores(i, sk);
                         else tc5_commit(o_full + 8 * i);
                     }
                     done[i]++;
+                };
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) {                    // a tile's parts follow one another, the other tile's softmax beside them
+                    product(i, true, !THIRD);
+                    if constexpr (THIRD) product(i, false, true);
                 }
                 if (ok && leader) {
                     tc5_commit(kv_empty + 8 * sv);
@@ -556,7 +577,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         // The weights of a tile are taken to a reference of the tiles before it, without looking for the tile's own maximum first (250
         // clocks): nothing is lost as long as they stay in range, and their sum, which is taken anyway, says whether they do. A row's
         // first reference is the largest of its first 16 scores (f16: of its first tile's). Where the sum passes the limit (or is NaN), in masked tiles, and for f32
-        // results of f16, S is read for its maximum, O rescaled -- S's arrival tells that the product before it is complete -- and the weights
+        // results, S is read for its maximum, O rescaled -- S's arrival tells that the product before it is complete -- and the weights
         // taken to that: S stays whole until P is written over it. The sums and products are f32, so scaled by up to the limit they lose
         // nothing. The two ways are kept apart: a loop around one of them, or masks in it, cost 100 to 470 clocks a tile.
         const int i = warp >> 2, r = threadIdx.x & 127;
@@ -579,13 +600,18 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 if (!ok) break;
                 if (idle) {
                     if (lane == 0) mbar_arrive(p_full + 8 * i);
+                    if constexpr (THIRD) {
+                        ok = __all_sync(0xffffffffu, ta_wait(h_used + 8 * i, tiles & 1, abort_flag));
+                        if (!ok) break;
+                        if (lane == 0) mbar_arrive(p_full + 8 * i);
+                    }
                     continue;
                 }
                 tc5_fence_after();
                 const int n = seen - j * TA_KV;                      // positions of the tile that the row sees
                 const bool masked = (j + 1) * TA_KV > all_seen;
-                // 32 positions' weights, packed, and (HILO) what the packing left; their sum
-                auto weights = [&](const uint32_t (&v)[32], float mc, float (&sum)[2][2], uint32_t (&hi)[16], uint32_t (&lo)[16]) {
+                // 32 positions' weights, packed, (HILO) what the packing left, and (THIRD) what that one's left; their sum
+                auto weights = [&](const uint32_t (&v)[32], float mc, float (&sum)[2][2], uint32_t (&hi)[16], uint32_t (&lo)[16], uint32_t (&th)[16]) {
 #pragma unroll
                     for (int y = 0; y < 16; ++y) {
                         float u, w;
@@ -597,14 +623,19 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                         hi[y] = ta_pack<BF16>(u, w);
                         if constexpr (HILO) {
                             const float2 b = ta_unpack<BF16>(hi[y]);
-                            lo[y] = ta_pack<BF16>(u - b.x, w - b.y);
+                            u -= b.x; w -= b.y;
+                            lo[y] = ta_pack<BF16>(u, w);
+                            if constexpr (THIRD) {
+                                const float2 d = ta_unpack<BF16>(lo[y]);
+                                th[y] = ta_pack<BF16>(u - d.x, w - d.y);
+                            }
                         }
                     }
                 };
                 // what the scores' exponents start from
                 auto minus = [&](float ref) { return ref == -INFINITY ? 0.f : BF16 || HILO ? -ref * c : fmaf(-ref, c, W::LOG_TOP); };
-                bool slow = masked || (HILO && !BF16);
-                if (BF16 && j == 0 && !masked) {                             // any of a row's scores may be the first reference
+                bool slow = masked || HILO;
+                if (BF16 && j == 0 && !slow) {                             // any of a row's scores may be the first reference
                     uint32_t v[16];
                     tc5_ld16(S, v);
                     ta_wait_ld(v);
@@ -615,7 +646,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     if (!(m < INFINITY)) m = 0.f;                    // the sum tells of NaN and +inf
                 }
                 if (!slow) {
-                    uint32_t s[4][32], hi[4][16], lo[HILO ? 4 : 1][16];
+                    uint32_t s[4][32], hi[4][16], none[16];
                     float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
                     for (int x = 0; x < 4; ++x) tc5_ld32(S + 32 * x, s[x]);
@@ -634,36 +665,40 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                     }
                     const float mc = minus(m);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) weights(s[x], mc, sum, hi[x], lo[HILO ? x : 0]);
+                    for (int x = 0; x < 4; ++x) weights(s[x], mc, sum, hi[x], none, none);
                     const float total = (sum[0][0] + sum[1][0]) + (sum[0][1] + sum[1][1]);
                     slow = __any_sync(0xffffffffu, live && m == m && (!(total <= W::LIMIT) || (m == -INFINITY && total > 0.f)));
                     if (!slow) {
                         l += total;
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {                // over the positions' own columns
-                            ta_st16(S + 32 * x, hi[x]);
-                            if constexpr (HILO) ta_st16(S + 32 * x + 16, lo[x]);
-                        }
+                        for (int x = 0; x < 4; ++x) ta_st16(S + 32 * x, hi[x]);      // over the positions' own columns
                     }
                 }
+                uint32_t third[THIRD ? 4 : 1][16];
                 if (slow) {
                     uint32_t s[4][32];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) tc5_ld32(S + 32 * x, s[x]);
 #pragma unroll
                     for (int x = 0; x < 4; ++x) ta_wait_ld(s[x]);
+                    if (!HILO || masked) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+#pragma unroll
+                            for (int y = 0; y < 32; ++y)
+                                if (32 * x + y >= n) s[x][y] = 0xFF800000u;
+                    }
                     float tops[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-#pragma unroll
-                        for (int y = 0; y < 32; ++y)
-                            if (32 * x + y >= n) s[x][y] = 0xFF800000u;
                         tops[x] = __uint_as_float(s[x][0]);
 #pragma unroll
                         for (int y = 1; y < 32; ++y) tops[x] = ta_max(tops[x], __uint_as_float(s[x][y]));
                     }
-                    const float top = ta_max(ta_max(tops[0], tops[1]), ta_max(tops[2], tops[3]));      // of the row; m, l and O go up to it
-                    const float next = ta_max(m, top);               // NaN stays
+                    const float top = ta_max(ta_max(tops[0], tops[1]), ta_max(tops[2], tops[3]));      // of the row; m, l and O go up to it,
+                    // or (f32 results) stay where they are while the weights have room
+                    const bool stay = HILO && !__any_sync(0xffffffffu, live && !((top - m) * c <= W::ROOM));
+                    const float next = stay ? m : ta_max(m, top);    // NaN stays
                     const float f = next == m || next == -INFINITY ? 1.f : ta_exp2((m - next) * c);
                     m = next < INFINITY ? next : __int_as_float(0x7fffffff);      // a score of NaN or +inf: so is every weight of the row
                     l *= f;
@@ -683,7 +718,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         uint32_t hi[16], lo[16];
-                        weights(s[x], mc, sum, hi, lo);
+                        weights(s[x], mc, sum, hi, lo, third[THIRD ? x : 0]);
                         ta_st16(S + 32 * x, hi);
                         if constexpr (HILO) ta_st16(S + 32 * x + 16, lo);
                     }
@@ -693,6 +728,17 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 tc5_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(p_full + 8 * i);
+                if constexpr (THIRD) {
+                    ok = __all_sync(0xffffffffu, ta_wait(h_used + 8 * i, tiles & 1, abort_flag));
+                    if (!ok) break;
+                    tc5_fence_after();
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) ta_st16(S + 32 * x, third[x]);
+                    ta_wait_st();
+                    tc5_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full + 8 * i);
+                }
             }
             if (!ok) break;
             const bool whole = t->whole;

@@ -437,7 +437,7 @@ class Device:
         """Attention of each sequence's new rows over its pages, causal: new row i of the n that sequence s has sits at position
         lens[s] - n + i (its key and value are in the cache already: RopeAppend). starts int32 [n_seq + 1] and lens int32 [n_seq] are
         device tensors; q, out, scratch and scale as in AttnPrompt. max_new: the most new rows of any sequence, as far as the caller
-        knows; it picks the kernel, not the result (None: all rows may be one sequence's)."""
+        knows; it picks the kernel, and so the result's rounding, not what is computed (None: all rows may be one sequence's)."""
         total, hq, d, qt, qh = self._heads("q", q)
         if d != kv.head_dim or q.dtype != kv.k.dtype:
             raise ValueError("q must have the cache's head size and type")

@@ -153,3 +153,22 @@ def test_f32_results_of_few_rows_carry_f32_weights(dev, dt, hq, hkv, d):
     for s, n in enumerate(lens):
         ref, mag, _ = _reference(q[s:s + 1], k[8 * s:8 * s + n], v[8 * s:8 * s + n], n - 1, scale)
         _weights_of_24_bits(out[s:s + 1], ref, mag, n)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hkv,d,nseq", [(8, 8, 128, 40), (12, 4, 64, 9), (16, 1, 128, 30), (16, 1, 64, 1)])
+def test_f32_results_of_many_rows_carry_f32_weights(dev, dt, hq, hkv, d, nseq):
+    """Prompts of up to eight tokens, packed: the tensor core's kernel with one tile and with two."""
+    import torch
+    new = [8, 7, 5, 2, 1, 8, 6, 3][:nseq] * (nseq // 8) + [8] * (nseq % 8)
+    scale = float(torch.tensor(2.0).log())
+    q, k, v = _exact_scores(sum(new), hq, hkv, d, sum(new), _dt(dt), 4)
+    out = torch.empty(sum(new), hq, d, device="cuda")
+    dev.AttnPrompt(out, q, k, v, _starts(new), _scratch(dev), scale=scale, stream=_stream())
+    torch.cuda.synchronize()
+    assert dev.StatusPoll()
+    at = 0
+    for n in new:
+        ref, mag, _ = _reference(q[at:at + n], k[at:at + n], v[at:at + n], 0, scale)
+        _weights_of_24_bits(out[at:at + n], ref, mag, 8)
+        at += n
