@@ -226,10 +226,10 @@ int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, int un
     if ((a.table ? (long long)a.max_pages << a.page_shift : (long long)a.total) <= unit) return JL_OK;
     const dim3 few(ctas, ATTN_MERGE_BLOCKS), many(ctas, rows / (8 * ATTN_MERGE_ROWS));
     const cudaError_t e = rows == ATTN_FEW_ROWS
-        ? (a.d == 128 ? attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 128>, few, dim3(256), 0, s, a, ctas)
-                      : attn_launch_pdl(attn_merge_few_kernel<ATTN_FEW_ROWS, 64>, few, dim3(256), 0, s, a, ctas))
-        : (a.d == 128 ? attn_launch_pdl(attn_merge_many_kernel<128>, many, dim3(256), 0, s, a, ctas, rows)
-                      : attn_launch_pdl(attn_merge_many_kernel<64>, many, dim3(256), 0, s, a, ctas, rows));
+        ? (a.d == 128 ? attn_launch_pdl(ctx, attn_merge_few_kernel<ATTN_FEW_ROWS, 128>, few, dim3(256), 0, s, a, ctas)
+                      : attn_launch_pdl(ctx, attn_merge_few_kernel<ATTN_FEW_ROWS, 64>, few, dim3(256), 0, s, a, ctas))
+        : (a.d == 128 ? attn_launch_pdl(ctx, attn_merge_many_kernel<128>, many, dim3(256), 0, s, a, ctas, rows)
+                      : attn_launch_pdl(ctx, attn_merge_many_kernel<64>, many, dim3(256), 0, s, a, ctas, rows));
     JL_CUDA(ctx, e);
     ctx->st.launches++;
     return JL_OK;
@@ -460,7 +460,7 @@ JL_EXPORT int jl_rope_append(jl_ctx *ctx, void *q_out, const void *qkv, int x_dt
     a.kv_tok = c.head_dim; a.kv_head = (long long)c.page_len * c.head_dim; a.kv_page = a.kv_head * c.n_kv;
     a.nseq = c.n_seq; a.total = total; a.hq = hq; a.hkv = c.n_kv; a.d = c.head_dim; a.page_shift = shift; a.n_pages = c.n_pages;
     a.max_pages = c.max_pages; a.max_pos = max_pos; a.x_dtype = x_dtype; a.dtype = c.dtype;
-    const cudaError_t e = attn_launch_pdl(attn_append_kernel, dim3(total, 1), dim3(256), 0, (cudaStream_t)stream, a);
+    const cudaError_t e = attn_launch_pdl(ctx, attn_append_kernel, dim3(total, 1), dim3(256), 0, (cudaStream_t)stream, a);
     JL_CUDA(ctx, e);
     ctx->st.launches++;
     ctx->st.served++;

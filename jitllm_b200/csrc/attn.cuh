@@ -275,14 +275,15 @@ __host__ __device__ static inline size_t attn_slot_floats(int rows, int d) { ret
 #define ATTN_FEW_MAX 512         // in all: the join keeps 64 parts to each of eight warps
 #define ATTN_TC_ROWS 256         // or 128, and twice the CTAs
 
-// Launched so that the next kernel of the stream may be put in place while this one drains.
+// Launched so that the kernel may be put in place while the one in front of it in the stream drains (unless the context is to do without).
 template <typename... P, typename... Args>
-static cudaError_t attn_launch_pdl(void (*kern)(P...), dim3 grid, dim3 block, int smem, cudaStream_t s, Args... args) {
+static cudaError_t attn_launch_pdl(const jl_ctx *ctx, void (*kern)(P...), dim3 grid, dim3 block, int smem, cudaStream_t s, Args... args) {
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = s; cfg.attrs = at; cfg.numAttrs = 1;
+    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = s; cfg.attrs = at;
+    cfg.numAttrs = (ctx->opts.flags & JL_FLAG_NO_PDL) ? 0 : 1;
     return cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);
 }
 

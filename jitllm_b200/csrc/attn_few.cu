@@ -352,7 +352,7 @@ static int few_go(jl_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
     const int smem = FewTile<D>::SMEM, grid = attn_few_grid(ctx);
     auto kern = attn_few_kernel<D, BF16>;
     if (smem > 48 * 1024) JL_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const cudaError_t e = attn_launch_pdl(kern, dim3(grid), dim3(128), smem, s, a, FEW_MIN_UNITS);
+    const cudaError_t e = attn_launch_pdl(ctx, kern, dim3(grid), dim3(128), smem, s, a, FEW_MIN_UNITS);
     JL_CUDA(ctx, e);
     ctx->st.launches++;
     return attn_launch_merge(ctx, a, ATTN_FEW_ROWS, grid, 1 << FEW_UNIT_SHIFT, s);

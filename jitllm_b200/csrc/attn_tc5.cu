@@ -852,7 +852,7 @@ static int ta_go(jl_ctx *ctx, const AttnArgs &a, const CUtensorMap &q, const CUt
     auto kern = attn_tc5_kernel<D, TILES, BF16, HILO>;
     const int smem = TaSmem<D, TILES>::TOTAL, grid = ctx->sm_count * R::CTAS;
     JL_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    const cudaError_t e = attn_launch_pdl(kern, dim3(grid), dim3(R::WARPS * 32), smem, s, a, q, k, v, box_rows, 2);
+    const cudaError_t e = attn_launch_pdl(ctx, kern, dim3(grid), dim3(R::WARPS * 32), smem, s, a, q, k, v, box_rows, 2);
     JL_CUDA(ctx, e);
     ctx->st.launches++;
     return attn_launch_merge(ctx, a, R::ROWS, grid, TA_KV, s);

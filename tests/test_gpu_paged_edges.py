@@ -172,3 +172,40 @@ def test_f32_results_of_many_rows_carry_f32_weights(dev, dt, hq, hkv, d, nseq):
         ref, mag, _ = _reference(q[at:at + n], k[at:at + n], v[at:at + n], 0, scale)
         _weights_of_24_bits(out[at:at + n], ref, mag, 8)
         at += n
+
+
+def _programmatic_edges(graph):
+    """Of a captured graph's edges, those along which a kernel may start before the one in front of it is done."""
+    import ctypes as C
+    cu = C.CDLL("libcuda.so.1")
+    h, n = C.c_void_p(graph.raw_cuda_graph()), C.c_size_t(0)
+    assert cu.cuGraphGetEdges_v2(h, None, None, None, C.byref(n)) == 0
+    a, b, data = (C.c_void_p * n.value)(), (C.c_void_p * n.value)(), (C.c_uint8 * (8 * n.value))()      # from, to; ports, type, reserved
+    assert cu.cuGraphGetEdges_v2(h, a, b, data, C.byref(n)) == 0
+    return sum(data[8 * i + 2] == 1 for i in range(n.value))
+
+
+def test_no_dependent_launches_where_the_context_forbids_them():
+    import torch
+    from jitllm_b200 import Device, PagedKV, _lib
+    cos, q = torch.zeros(64, 32, device="cuda"), torch.zeros(40, 8, 64, device="cuda", dtype=torch.bfloat16)
+    qkv, lens, table = torch.randn(40, 12 * 64, device="cuda"), _i32([40, 50]), torch.arange(8, device="cuda", dtype=torch.int32).view(2, 4)
+    kv = PagedKV(torch.zeros(8, 2, 128, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(8, 2, 128, 64, device="cuda", dtype=torch.bfloat16), table)
+    found, results = [], []
+    for flags in (0, _lib.FLAG_NO_PDL):
+        with Device(0, flags=flags) as d:
+            out, starts, scratch = torch.zeros(40, 8, 64, device="cuda"), _starts([1, 39]), _scratch(d)
+
+            def calls(stream):
+                d.RopeAppend(q, qkv, kv, starts, lens, cos + 1, cos, stream=stream)
+                d.AttnPaged(out, q, kv, starts, lens, scratch, max_new=39, stream=stream)        # few rows, many rows, a join of each
+                d.AttnPrompt(out, q, q[:, :2], q[:, 2:4], starts, scratch, stream=stream)
+            calls(_stream())
+            torch.cuda.synchronize()
+            results.append(out.clone())
+            graph = torch.cuda.CUDAGraph(keep_graph=True)
+            with torch.cuda.graph(graph):
+                calls(_stream())
+            found.append(_programmatic_edges(graph))
+            graph.reset()
+    assert found[0] >= 5 and found[1] == 0 and torch.equal(*results)
