@@ -64,9 +64,13 @@ template <bool BF16, bool HILO> struct TaWeights {
 
 // The bounded wait of this kernel's roles. A try that may sleep for up to 20 us: the warps that wait are many, and their polling would take
 // the issue slots of those that work.
-// patience: by how much the limit is longer for a role whose wait spans others' whole work (they give up first, and end it).
-#define TA_PATIENCE 4096u
-__device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, uint32_t patience = 1) {
+// A patient role's wait spans others' whole work -- all of a segment, or the walk over the sequences -- and so has 4096 times the limit, up to
+// ten seconds more than it. Those others give up first where something is lost, and end it.
+#define TA_PATIENCE 4096ull
+#define TA_PATIENCE_NS 10000000000ull
+// What is waited for at a CTA's end, whatever the limit is: copies and products that are on their way end by themselves.
+#define TA_DRAIN_NS 1000000000ull
+__device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, bool patient = false) {
     uint64_t t0 = 0;
     for (;;) {
         uint32_t done;
@@ -81,7 +85,10 @@ __device__ __forceinline__ bool ta_wait(uint32_t bar, uint32_t parity, volatile 
         if (*abort_flag) return false;
         const uint64_t t = jl_gtime_ns();
         if (!t0) t0 = t;
-        else if (t - t0 > tc5_limit_ns(abort_flag) * patience) break;
+        else {
+            const uint64_t limit = tc5_limit_ns(abort_flag);
+            if (t - t0 > limit + (patient ? min((unsigned long long)limit * (TA_PATIENCE - 1), TA_PATIENCE_NS) : 0ull)) break;
+        }
     }
     *abort_flag = 1;
     return false;
@@ -325,7 +332,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
     uint32_t gi = 0;                                        // segments seen
     // the next segment, or NULL at the end of the share
     auto seg_next = [&]() -> const volatile TaSeg * {
-        ok = ok && __all_sync(0xffffffffu, ta_wait(g_full + 8 * (gi % TA_SEGS), (gi / TA_SEGS) & 1, abort_flag));
+        ok = ok && __all_sync(0xffffffffu, ta_wait(g_full + 8 * (gi % TA_SEGS), (gi / TA_SEGS) & 1, abort_flag, true));
         const volatile TaSeg *t = ring + gi % TA_SEGS;
         return ok && t->seq >= 0 ? t : nullptr;
     };
@@ -401,15 +408,13 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             segs++;
             seg_done();
         }
-        // a copy must not outlive its CTA: after a failed wait elsewhere those in flight are waited for here
-        if (*abort_flag) {
-            const uint64_t limit = tc5_limit_ns(abort_flag);
-            if (segs) mbar_wait_ns(q_full, (segs - 1) & 1, limit);
-            for (uint32_t i = it > (uint32_t)L::STAGES ? it - L::STAGES : 0; i < it; ++i)
-                mbar_wait_ns(kv_full + 8 * (i % L::STAGES), (i / L::STAGES) & 1, limit);
-            for (uint32_t i = edges > (uint32_t)L::OKS ? edges - L::OKS : 0; i < edges; ++i)
-                mbar_wait_ns(e_full + 8 * (i % L::OKS), (i / L::OKS) & 1, limit);
-        }
+        // A copy must not outlive its CTA: the last on each barrier are waited for here. Where all went well they have landed or are about to;
+        // where a role gives up, perhaps after this one is done, nobody else waits for them.
+        if (segs) mbar_wait_ns(q_full, (segs - 1) & 1, TA_DRAIN_NS);
+        for (uint32_t i = it > (uint32_t)L::STAGES ? it - L::STAGES : 0; i < it; ++i)
+            mbar_wait_ns(kv_full + 8 * (i % L::STAGES), (i / L::STAGES) & 1, TA_DRAIN_NS);
+        for (uint32_t i = edges > (uint32_t)L::OKS ? edges - L::OKS : 0; i < edges; ++i)
+            mbar_wait_ns(e_full + 8 * (i % L::OKS), (i / L::OKS) & 1, TA_DRAIN_NS);
     } else if (warp == R::MMA) {
         TA_REGS("dec", R::REGS_OTHER);
         // ------------------------------------------------ products
@@ -497,7 +502,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         }
         if (leader) tc5_commit(drain);                               // nothing of the tensor core's is left when TMEM is given back
         __syncwarp();
-        if (!mbar_wait_ns(drain, 0, tc5_limit_ns(abort_flag))) *abort_flag = 1;
+        if (!mbar_wait_ns(drain, 0, TA_DRAIN_NS)) *abort_flag = 1;
     } else if (warp == R::EDGES) {
         TA_REGS("dec", R::REGS_OTHER);
         // ------------------------------------------------ edges
@@ -514,7 +519,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             for (int j = 0; j < E && ok; ++j, it += 2) {
                 if (j < edge) continue;
                 const uint32_t s = (it + 1) % L::STAGES;
-                ok = __all_sync(0xffffffffu, ta_wait(e_full + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag, TA_PATIENCE));
+                ok = __all_sync(0xffffffffu, ta_wait(e_full + 8 * (edges % L::OKS), (edges / L::OKS) & 1, abort_flag, true));
                 if (!ok) break;
                 const int rows = left - j * TA_KV;       // of the sequence
                 const uint32_t v = sbase + L::KV + s * L::TILE;
@@ -562,7 +567,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         walk.begin(first, last);
         AttnSeg g;
         for (bool more = true; more && ok; ++gi) {
-            if (gi >= TA_SEGS) ok = __all_sync(0xffffffffu, ta_wait(g_empty + 8 * (gi % TA_SEGS), (gi / TA_SEGS + 1) & 1, abort_flag, TA_PATIENCE));
+            if (gi >= TA_SEGS) ok = __all_sync(0xffffffffu, ta_wait(g_empty + 8 * (gi % TA_SEGS), (gi / TA_SEGS + 1) & 1, abort_flag, true));
             if (!ok) break;
             more = walk.next(a, TA_UNIT_SHIFT, g);
             if (lane == 0) {

@@ -209,3 +209,58 @@ def test_no_dependent_launches_where_the_context_forbids_them():
             found.append(_programmatic_edges(graph))
             graph.reset()
     assert found[0] >= 5 and found[1] == 0 and torch.equal(*results)
+
+
+def _last_of_a_million(d, rows):
+    """A prompt behind 2^20 - 1 sequences without rows: each CTA goes over all of them before it knows its share. (out, check)"""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q, k, v = (torch.randn(rows, h, 128, generator=g, device="cuda").bfloat16() for h in (8, 2, 2))
+    starts = torch.zeros((1 << 20) + 1, dtype=torch.int32, device="cuda")
+    starts[-1] = rows
+    out = torch.full((rows, 8, 128), 7.0, device="cuda")
+    d.AttnPrompt(out, q, k, v, starts, _scratch(d), stream=_stream())
+    torch.cuda.synchronize()
+    return out, lambda o: _check(o, *_reference(q, k, v, 0, 128 ** -0.5), _dt("bf16"), rows, 128)
+
+
+def test_a_wait_that_runs_out_is_reported_and_the_context_goes_on():
+    """With a limit of a microsecond the roles that wait for a share give up (after 4 ms: they are patient) before a walk over a million
+    sequences has found one: the kernel returns, the status says so, and the next call is right."""
+    import torch
+    from jitllm_b200 import Device
+    with Device(0, wait_limit_us=1) as d:
+        _last_of_a_million(d, 300)
+        assert not d.StatusPoll() and "attention" in d.Err()
+        assert d.StatusPoll()
+        q = torch.randn(4, 8, 128, device="cuda").bfloat16()                # sixteen query rows: a kernel that waits for nothing
+        out = torch.empty_like(q)
+        d.AttnPrompt(out, q, q[:, :2], q[:, 2:4], _starts([4]), _scratch(d), stream=_stream())
+        torch.cuda.synchronize()
+        _check(out, *_reference(q, q[:, :2], q[:, 2:4], 0, 128 ** -0.5), _dt("bf16"), 4, 128)
+        assert d.StatusPoll()
+    with Device(0) as d:
+        out, check = _last_of_a_million(d, 300)
+        assert d.StatusPoll()
+        check(out)
+
+
+@pytest.mark.parametrize("new,lens", [([20] * 200, [9000] * 200), ([60] * 100, [9000] * 100)])
+def test_a_short_limit_does_not_end_long_work(new, lens):
+    """Two tiles to an item, the second one idle: its roles wait through all of the first one's work, many times the limit."""
+    import torch
+    from jitllm_b200 import Device, PagedKV
+    g = torch.Generator(device="cuda").manual_seed(6)
+    pages = torch.randn(160, 2, 64, 128, generator=g, device="cuda").bfloat16()
+    table = torch.stack([torch.randperm(160, generator=g, device="cuda")[:lens[0] // 64 + 1] for _ in new]).to(torch.int32)
+    q = torch.randn(sum(new), 2, 128, generator=g, device="cuda").bfloat16()
+    kv, st = PagedKV(pages, pages.flip(0).contiguous(), table), _stream()
+    got = []
+    for limit in (0, 60):
+        with Device(0, wait_limit_us=limit) as d:
+            out = torch.zeros_like(q)
+            d.AttnPaged(out, q, kv, _starts(new), _i32(lens), _scratch(d), stream=st)
+            torch.cuda.synchronize()
+            assert d.StatusPoll()
+            got.append(out)
+    assert torch.equal(*got)
