@@ -78,7 +78,7 @@ __host__ __device__ static inline long long attn_item_weight(const AttnSeq &q, i
 // Sum of the weights of blocks [0, i) of a sequence, i <= ceil(n / T); for one head.
 __host__ __device__ static inline long long attn_blocks_weight(const AttnSeq &q, int i, int T, int cost) {
     if (i <= 0) return 0;
-    const long long base = (long long)i * ((long long)cost + (q.pos0 > 0 ? q.pos0 : 0));
+    const long long base = (long long)i * (cost + (q.pos0 > 0 ? q.pos0 : 0));        // no more than a table's 2^30 positions and a cost
     const long long whole = (long long)T * i * (i + 1) / 2;
     const long long over = (long long)i * T - q.n;           // of the last block, if it is the ragged one
     return base + whole - (over > 0 ? over : 0);

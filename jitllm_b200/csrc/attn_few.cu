@@ -74,7 +74,7 @@ __device__ __forceinline__ bool few_odd(uint32_t w) {
     return (w & E) == E || (w & (E << 16)) == (E << 16);
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool THIRD>
 __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant__ AttnArgs a, int min_units) {
     constexpr int ROW = FewTile<D>::ROW, TILE = FewTile<D>::BYTES, NJ = D / 8, CH = D / 8;   // CH: 16-byte pieces of a row
     extern __shared__ __align__(16) uint8_t tiles[];   // the warps' rings; the cross-warp sum red[4][16][D] reuses them
@@ -91,7 +91,6 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
     walk.begin(first, last);
     AttnSeg sg, ng;
     if (t == 0) bad = 0;
-    const bool third = a.out_dtype == JL_DT_F32;       // of a weight's bf16 parts
     const uint16_t *kp = static_cast<const uint16_t *>(a.k), *vp = static_cast<const uint16_t *>(a.v);
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(tiles) + warp * FEW_STAGES * TILE;
     // the page of the warp's tile i: 16 positions lie in one (pages are 16 positions at least, cut at multiples of their length)
@@ -215,7 +214,8 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
                     }
             }
             // A fragments of the weights, as value + remainder (16 significant bits of bf16, 22 of f16), and for f32 results of bf16
-            // the remainder's remainder (24): the products with V lose nothing that the result shows
+            // the remainder's remainder (24): the products with V lose nothing that the result shows. (An instance of its own: for 16-bit
+            // results the third part would cost 0.8 of 88 us, 64 sequences.)
             uint32_t ph[4], pl[4], pt[4];
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt)
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
                     float rx, ry, z0, z1;
                     ph[2 * nt + e] = few_pack<BF16>(sv[nt][2 * e], sv[nt][2 * e + 1], rx, ry);
                     pl[2 * nt + e] = few_pack<BF16>(rx, ry, z0, z1);
-                    if constexpr (BF16) { float y0, y1; pt[2 * nt + e] = few_pack<BF16>(z0, z1, y0, y1); }
+                    if constexpr (THIRD) { float y0, y1; pt[2 * nt + e] = few_pack<BF16>(z0, z1, y0, y1); }
                 }
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
                     few_mma<BF16>(oacc[2 * jp], pl, b0, b1);
                     few_mma<BF16>(oacc[2 * jp + 1], ph, b2, b3);
                     few_mma<BF16>(oacc[2 * jp + 1], pl, b2, b3);
-                    if (BF16 && third) {
+                    if constexpr (THIRD) {
                         few_mma<BF16>(oacc[2 * jp], pt, b0, b1);
                         few_mma<BF16>(oacc[2 * jp + 1], pt, b2, b3);
                     }
@@ -347,10 +347,10 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
     if (t == 0) a.meta[blockIdx.x] = meta;
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool THIRD>
 static int few_go(jl_ctx *ctx, const AttnArgs &a, cudaStream_t s) {
     const int smem = FewTile<D>::SMEM, grid = attn_few_grid(ctx);
-    auto kern = attn_few_kernel<D, BF16>;
+    auto kern = attn_few_kernel<D, BF16, THIRD>;
     if (smem > 48 * 1024) JL_CUDA(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     const cudaError_t e = attn_launch_pdl(ctx, kern, dim3(grid), dim3(128), smem, s, a, FEW_MIN_UNITS);
     JL_CUDA(ctx, e);
@@ -363,6 +363,8 @@ int attn_launch_few(jl_ctx *ctx, const AttnArgs &args, int dtype, cudaStream_t s
     a.tok_item = ATTN_FEW_ROWS / a.g;
     a.item_cost = FEW_ITEM_COST;
     a.snap = FEW_SNAP;
-    if (a.d == 128) return dtype == JL_DT_BF16 ? few_go<128, true>(ctx, a, s) : few_go<128, false>(ctx, a, s);
-    return dtype == JL_DT_BF16 ? few_go<64, true>(ctx, a, s) : few_go<64, false>(ctx, a, s);
+    const bool third = a.out_dtype == JL_DT_F32;
+    if (dtype != JL_DT_BF16) return a.d == 128 ? few_go<128, false, false>(ctx, a, s) : few_go<64, false, false>(ctx, a, s);
+    if (a.d == 128) return third ? few_go<128, true, true>(ctx, a, s) : few_go<128, true, false>(ctx, a, s);
+    return third ? few_go<64, true, true>(ctx, a, s) : few_go<64, true, false>(ctx, a, s);
 }
