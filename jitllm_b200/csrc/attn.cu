@@ -288,8 +288,8 @@ __global__ void __launch_bounds__(256) attn_append_kernel(const __grid_constant_
         const int hd = i / quads, j = i - hd * quads;
         float4 v = attn_load4(a.qkv, a.x_dtype, ((size_t)row * heads + hd) * a.d + 4 * j);
         if (hd < a.hq + a.hkv) {
-            const float2 c = __ldg(reinterpret_cast<const float2 *>(a.cos_t + (size_t)pos * (a.d / 2)) + j);
-            const float2 s = __ldg(reinterpret_cast<const float2 *>(a.sin_t + (size_t)pos * (a.d / 2)) + j);
+            const float2 c = reinterpret_cast<const float2 *>(a.cos_t + (size_t)pos * (a.d / 2))[j];
+            const float2 s = reinterpret_cast<const float2 *>(a.sin_t + (size_t)pos * (a.d / 2))[j];
             v = make_float4(v.x * c.x - v.y * s.x, v.x * s.x + v.y * c.x, v.z * c.y - v.w * s.y, v.z * s.y + v.w * c.y);
         }
         if (hd < a.hq) {

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
     auto page_of = [&](const AttnSeg &g, int i) -> int {
         const int p = (g.u0 + i) * 64 + warp * 16;
         if (!a.table || i >= g.u1 - g.u0 || p >= g.q.len) return 0;
-        return __ldg(a.table + (long long)g.seq * a.max_pages + (p >> a.page_shift));
+        return a.table[(long long)g.seq * a.max_pages + (p >> a.page_shift)];
     };
     bool more = walk.next(a, FEW_UNIT_SHIFT, ng);
     int page0 = more ? page_of(ng, 0) : 0, page1 = more ? page_of(ng, 1) : 0;
@@ -141,6 +141,8 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
             seen[e] = tk < ntok ? attn_limit(sg.q, tok0 + tk + 1) : 0;
         }
         const int few_seen = attn_limit(sg.q, tok0 + 1);            // of the item's first token: below it every row sees everything
+        // q (and the table) by plain loads: the kernel in front, which may still have run when this one was put in place, can have written
+        // it, and the read-only path is for what nothing writes while the kernel is there
         uint32_t qa[D / 16][4];
         {
             const uint16_t *qp = static_cast<const uint16_t *>(a.q);
@@ -153,8 +155,8 @@ __global__ void __launch_bounds__(128, 3) attn_few_kernel(const __grid_constant_
             }
 #pragma unroll
             for (int ks = 0; ks < D / 16; ++ks) {
-                qa[ks][0] = __ldg(row[0] + ks * 8 + tq); qa[ks][1] = __ldg(row[1] + ks * 8 + tq);
-                qa[ks][2] = __ldg(row[0] + ks * 8 + 4 + tq); qa[ks][3] = __ldg(row[1] + ks * 8 + 4 + tq);
+                qa[ks][0] = row[0][ks * 8 + tq]; qa[ks][1] = row[1][ks * 8 + tq];
+                qa[ks][2] = row[0][ks * 8 + 4 + tq]; qa[ks][3] = row[1][ks * 8 + 4 + tq];
             }
         }
         more = walk.next(a, FEW_UNIT_SHIFT, ng);

@@ -254,7 +254,7 @@ __device__ __noinline__ void ta_odd(const AttnArgs *a, int seq, int head, int ro
     for (int p = p0; p < p1; ++p) {
         long long at;
         if (a->table) {
-            const int page = __ldg(a->table + (long long)seq * a->max_pages + (p >> a->page_shift));
+            const int page = a->table[(long long)seq * a->max_pages + (p >> a->page_shift)];
             if ((unsigned)page >= (unsigned)a->n_pages) continue;
             at = page * a->kv_page + head * a->kv_head + (p & ((1 << a->page_shift) - 1)) * a->kv_tok;
         } else {
@@ -263,7 +263,7 @@ __device__ __noinline__ void ta_odd(const AttnArgs *a, int seq, int head, int ro
         const uint32_t *v = reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(a->v) + at);
 #pragma unroll 1
         for (int y = 0; y < a->d / 2; ++y) {
-            const uint32_t w = __ldg(v + y);
+            const uint32_t w = v[y];                         // a plain load: the kernel in front may have written it (attn_few.cu)
             if (ta_finite<BF16>(w) == w) continue;
             float2 f = ta_unpack<BF16>(w);                   // what is finite of the pair is in the sum already
             f.x = isfinite(f.x) ? 0.f : f.x;
@@ -369,7 +369,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
             const int nbox = TA_KV / box_rows;               // a page, or the part of it in a unit; lane b looks up the page of box b
             auto page_of = [&](int u) -> int {
                 const int p = u * TA_KV + lane * box_rows;
-                return table && lane < nbox && u < u1 && p < len ? __ldg(table + (p >> a.page_shift)) : 0;
+                return table && lane < nbox && u < u1 && p < len ? table[p >> a.page_shift] : 0;
             };
             int page = page_of(u0);
             for (int u = u0; u < u1 && ok; ++u) {

@@ -141,3 +141,13 @@ def test_a_length_beyond_its_table_takes_no_more_than_the_table(length):
     assert sum(work) == 3 * 8 * 20 and max(work) <= 1.15 * sum(work) / len(work) + 2
     for s in (0, 1, 2):
         assert len([c for c, segs in enumerate(shares) if any(g[0] == s for g in segs)]) >= 20
+
+
+@pytest.mark.parametrize("name", ["attn.cu", "attn.cuh", "attn_few.cu", "attn_tc5.cu"])
+def test_no_read_only_loads_behind_a_dependent_launch(name):
+    """These kernels are put in place while the one in front of them still runs, and what they read that one may have written: the read-only
+    load is for memory that nothing writes while a kernel is there."""
+    import os
+    from jitllm_b200 import build
+    text = open(os.path.join(build.CSRC, name)).read()
+    assert "__ldg(" not in text and "global.nc" not in text and "__restrict__" not in text
