@@ -191,7 +191,7 @@ class PagedKV:
     def __init__(self, k, v, table):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("k and v must be alike: [n_pages][n_kv][page_len][head_dim]")
-        if table.dim() != 2 or not str(table.dtype).endswith("int32"):
+        if table.dim() != 2 or table.dtype != _torch().int32:
             raise ValueError("the page table must be int32 [n_seq][max_pages]")
         if not (k.device == v.device == table.device) or k.device.type != "cuda":
             raise ValueError("the cache and its table must lie on one GPU")

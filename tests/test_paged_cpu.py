@@ -151,3 +151,12 @@ def test_no_read_only_loads_behind_a_dependent_launch(name):
     from jitllm_b200 import build
     text = open(os.path.join(build.CSRC, name)).read()
     assert "__ldg(" not in text and "global.nc" not in text and "__restrict__" not in text
+
+
+@pytest.mark.parametrize("dtype", ["uint32", "int64", "int16", "float32"])
+def test_a_page_table_is_int32(dtype):
+    import torch
+    from jitllm_b200 import PagedKV
+    k = torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="int32"):
+        PagedKV(k, k.clone(), torch.zeros(1, 2, dtype=getattr(torch, dtype)))
