@@ -461,6 +461,11 @@ int jl_rope_append(jl_ctx *ctx, void *q_out_dev, const void *qkv_dev, int x_dtyp
  * end unit, units of the item. Returns n. max_pages 0: no table. */
 int jl_test_attn_share(const int32_t *starts, const int32_t *lens, int nseq, int total, int hkv, int tok_item, int unit_shift, int min_units,
                        int page_shift, int max_pages, int grid, int cta, int32_t *segs, int cap);
+/* The same for a launch's own settings: query heads to a kv head, the sequences it takes (row_lo < new rows * g <= row_hi), units that an
+ * item's start and end cost, units from an item's end within which a cut moves onto it. */
+int jl_test_attn_share_as(const int32_t *starts, const int32_t *lens, int nseq, int total, int hkv, int g, int row_lo, int row_hi, int tok_item,
+                          int item_cost, int snap, int unit_shift, int min_units, int page_shift, int max_pages, int grid, int cta, int32_t *segs,
+                          int cap);
 
 /* ---- whole blocks in one submission: nn.LayerDevice (engine/nn/device.go:1096-1176) ------------
  * PrepLayer hands a block's weights to the device, Layers runs blocks [lo, hi) for the positions of one

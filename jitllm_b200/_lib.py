@@ -161,6 +161,7 @@ SYMBOLS = {
     "jl_attn_paged": (_I, [_VP, _VP, _I, _VP, _LL, _LL, C.POINTER(PagedKVDesc), _VP, _VP, _I, _I, _I, C.c_float, _VP, _SZ, _VP]),
     "jl_rope_append": (_I, [_VP, _VP, _VP, _I, C.POINTER(PagedKVDesc), _VP, _VP, _I, _I, _VP, _VP, _I, _VP]),
     "jl_test_attn_share": (_I, [_VP, _VP] + [_I] * 10 + [_VP, _I]),
+    "jl_test_attn_share_as": (_I, [_VP, _VP] + [_I] * 15 + [_VP, _I]),
     "jl_decode_operand": (_VP, [_VP, _VP, _I]),
     "jl_matvec_dev_prepared": (_I, [_VP, _VP, _VP, _I, _VP]),
 }

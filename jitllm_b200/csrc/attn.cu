@@ -467,26 +467,35 @@ JL_EXPORT int jl_rope_append(jl_ctx *ctx, void *q_out, const void *qkv, int x_dt
     return JL_OK;
 }
 
-// The division of the work as attn_share and AttnWalk make it, on the host: the segments of CTA `cta` as (sequence, block, head,
-// first unit, end unit, units of the item). Test-only.
-JL_EXPORT int jl_test_attn_share(const int32_t *starts, const int32_t *lens, int nseq, int total, int hkv, int tok_item, int unit_shift,
-                                 int min_units, int page_shift, int max_pages, int grid, int cta, int32_t *segs, int cap) {
-    if (!starts || !segs || nseq < 1 || hkv < 1 || tok_item < 1 || unit_shift < 1 || grid < 1 || cta < 0 || cta >= grid) return JL_EINVAL;
+// How a launch divides the work, on the host: the segments of CTA `cta` as (sequence, block, head, first unit, end unit, units of the
+// item). The items, the cuts and the walk are the device's own functions (attn.cuh); only the search for the sequences that the cuts
+// fall into is the host's, one sequence after the other where a warp looks at 32 (attn_share). Test-only.
+JL_EXPORT int jl_test_attn_share_as(const int32_t *starts, const int32_t *lens, int nseq, int total, int hkv, int g, int row_lo, int row_hi,
+                                    int tok_item, int item_cost, int snap, int unit_shift, int min_units, int page_shift, int max_pages,
+                                    int grid, int cta, int32_t *segs, int cap) {
+    if (!starts || !segs || nseq < 1 || hkv < 1 || g < 1 || tok_item < 1 || item_cost < 0 || snap < 0 || unit_shift < 1 || unit_shift > 16 ||
+        min_units < 1 || page_shift < 0 || page_shift > 16 || grid < 1 || cta < 0 || cta >= grid)
+        return JL_EINVAL;
     AttnArgs a = {};
     a.starts = starts; a.lens = lens; a.nseq = nseq; a.total = total; a.hkv = hkv; a.tok_item = tok_item;
     a.table = max_pages > 0 ? starts : nullptr;       // only its presence matters here
     a.page_shift = page_shift; a.max_pages = max_pages;
-    a.g = 1; a.row_hi = INT_MAX; a.item_cost = 1; a.snap = 2;
+    a.g = g; a.row_lo = row_lo; a.row_hi = row_hi; a.item_cost = item_cost; a.snap = snap;
     AttnCut first, last;
     attn_share_host(a, cta, grid, unit_shift, min_units, first, last);
     AttnWalk w;
     w.begin(first, last);
-    AttnSeg g;
+    AttnSeg sg;
     int n = 0;
-    while (w.next(a, unit_shift, g)) {
+    while (w.next(a, unit_shift, sg)) {
         if (n == cap) return -100;
         int32_t *o = segs + 6 * n++;
-        o[0] = g.seq; o[1] = g.blk; o[2] = g.head; o[3] = g.u0; o[4] = g.u1; o[5] = g.units;
+        o[0] = sg.seq; o[1] = sg.blk; o[2] = sg.head; o[3] = sg.u0; o[4] = sg.u1; o[5] = sg.units;
     }
     return n;
+}
+JL_EXPORT int jl_test_attn_share(const int32_t *starts, const int32_t *lens, int nseq, int total, int hkv, int tok_item, int unit_shift,
+                                 int min_units, int page_shift, int max_pages, int grid, int cta, int32_t *segs, int cap) {
+    return jl_test_attn_share_as(starts, lens, nseq, total, hkv, 1, 0, INT_MAX, tok_item, 1, 2, unit_shift, min_units, page_shift, max_pages,
+                                 grid, cta, segs, cap);
 }

@@ -160,3 +160,85 @@ def test_a_page_table_is_int32(dtype):
     k = torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="int32"):
         PagedKV(k, k.clone(), torch.zeros(1, 2, dtype=getattr(torch, dtype)))
+
+
+# what the kernels are launched with: unit, an item's cost, snap, tokens of an item, CTAs
+LAUNCHED = {"few": (6, 4, 2, lambda g: 16 // g, 444), "two tiles": (7, 3, 1, lambda g: 2 * (128 // g), 148), "one tile": (7, 2, 0, lambda g: 128 // g, 296)}
+TAKES = {"all": (0, 2 ** 31 - 1), "up to sixteen rows": (0, 16), "more": (16, 2 ** 31 - 1)}
+
+
+@pytest.mark.parametrize("which", LAUNCHED)
+@pytest.mark.parametrize("takes", TAKES)
+def test_the_launches_own_divisions(which, takes):
+    """Lengths, groups and idle sequences at random: of the sequences that a launch takes every unit of every item falls to one CTA, and the
+    parts of an item that a join would follow from the CTA that began it are all of them, in ascending order."""
+    shift, cost, snap, tokens, grid = LAUNCHED[which]
+    lo, hi = TAKES[takes]
+    rng = np.random.default_rng(11)
+    segs = np.zeros((1 << 14, 6), np.int32)
+    for trial in range(25):
+        n, g, hkv = int(rng.integers(1, 200)), int(rng.choice([1, 2, 3, 4, 8, 16])), int(rng.integers(1, 9))
+        new = np.where(rng.random(n) < 0.3, 0, np.where(rng.random(n) < 0.6, 1, rng.integers(1, 200, n)))
+        lens = np.maximum(0, new + rng.integers(-3, rng.choice([40, 3000, 9000]), n)).astype(np.int32)
+        starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        if trial % 5 == 0:
+            lens[rng.integers(0, n)] = 2 ** 31 - 1
+        total, T, max_pages = int(starts[-1]), tokens(g), 130
+        if total == 0:
+            continue
+        items = {}
+        for s in range(n):
+            if not lo < new[s] * g <= hi:
+                continue
+            pos0, ln = int(lens[s]) - int(new[s]), min(int(lens[s]), max_pages << 6)
+            for b in range(-(-int(new[s]) // T)):
+                limit = min(max(pos0 + min((b + 1) * T, int(new[s])), 0), ln)
+                for h in range(hkv):
+                    items[(s, b, h)] = -(-limit // (1 << shift))
+        shares = []
+        for c in range(grid):
+            k = L.jl_test_attn_share_as(starts.ctypes.data, lens.ctypes.data, n, total, hkv, g, lo, hi, T, cost, snap, shift, 2, 6, max_pages, grid,
+                                        c, segs.ctypes.data, len(segs))
+            assert k >= 0
+            shares.append(segs[:k].tolist())
+        whole, own, cont = [], {}, {}
+        for c, share in enumerate(shares):
+            for i, (s, b, h, u0, u1, units) in enumerate(share):
+                assert units == items[(s, b, h)] and (0 <= u0 < u1 <= units or u0 == u1 == units == 0)
+                if u0 == 0 and u1 == units:
+                    whole.append((s, b, h))
+                elif u0 > 0:
+                    assert i == 0 and c not in cont              # slot 0
+                    cont[c] = ((s, b, h), u0, u1, u1 == units)
+                else:
+                    assert i == len(share) - 1 and c not in own  # slot 1
+                    own[c] = ((s, b, h), u1)
+        for c, (item, at) in own.items():                        # as the join goes on from there
+            d = c + 1
+            while True:
+                assert d < grid
+                if d in cont:
+                    assert cont[d][0] == item and cont[d][1] == at
+                    at = cont[d][2]
+                    if cont.pop(d)[3]:
+                        break
+                else:
+                    assert not shares[d]
+                d += 1
+            assert at == items[item]
+            whole.append(item)
+        assert not cont and sorted(whole) == sorted(items)
+
+
+def test_shares_of_nothing_are_refused():
+    """Settings that would divide by zero or shift out of range come back as an error."""
+    s = np.zeros(6, np.int32)
+    good = dict(nseq=1, total=1, hkv=1, g=1, row_lo=0, row_hi=9, tok_item=1, item_cost=1, snap=0, unit_shift=6, min_units=1, page_shift=6, max_pages=0, grid=1, cta=0)
+
+    def call(**kw):
+        return L.jl_test_attn_share_as(s.ctypes.data, None, *{**good, **kw}.values(), s.ctypes.data, 1)
+    assert call() >= 0
+    for bad in (dict(min_units=0), dict(g=0), dict(tok_item=0), dict(unit_shift=0), dict(unit_shift=40), dict(page_shift=-1), dict(page_shift=40), dict(grid=0),
+                dict(cta=1), dict(cta=-1), dict(nseq=0), dict(hkv=0), dict(item_cost=-1), dict(snap=-1)):
+        assert call(**bad) == _lib.EINVAL, bad
+    assert L.jl_test_attn_share(s.ctypes.data, None, 1, 1, 1, 1, 6, 0, 6, 0, 1, 0, s.ctypes.data, 1) == _lib.EINVAL
