@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(256) attn_append_kernel(const __grid_constant_
     if (pos < 0) return;
     const int heads = a.hq + 2 * a.hkv, quads = a.d / 4;
     const long long at = page * a.kv_page + (pos & ((1 << a.page_shift) - 1)) * a.kv_tok;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < heads * quads; i += gridDim.y * 256) {
+    for (int i = threadIdx.x; i < heads * quads; i += 256) {
         const int hd = i / quads, j = i - hd * quads;
         float4 v = attn_load4(a.qkv, a.x_dtype, ((size_t)row * heads + hd) * a.d + 4 * j);
         if (hd < a.hq + a.hkv) {
@@ -351,8 +351,7 @@ int attn_launch(jl_ctx *ctx, AttnArgs a, int dtype, long long max_new, bool mixe
         a.row_lo = a.row_hi;
         a.row_hi = INT_MAX;
     }
-    const int rc = attn_launch_tc5(ctx, a, dtype, max_new * a.g, s);
-    return rc == JL_DECLINED ? attn_launch_few(ctx, a, dtype, s) : rc;
+    return attn_launch_tc5(ctx, a, dtype, max_new * a.g, s);
 }
 
 // A cache in pages: JL_OK, or the status with its reason. *shift: log2 of the page length.
@@ -460,7 +459,7 @@ JL_EXPORT int jl_rope_append(jl_ctx *ctx, void *q_out, const void *qkv, int x_dt
     a.kv_tok = c.head_dim; a.kv_head = (long long)c.page_len * c.head_dim; a.kv_page = a.kv_head * c.n_kv;
     a.nseq = c.n_seq; a.total = total; a.hq = hq; a.hkv = c.n_kv; a.d = c.head_dim; a.page_shift = shift; a.n_pages = c.n_pages;
     a.max_pages = c.max_pages; a.max_pos = max_pos; a.x_dtype = x_dtype; a.dtype = c.dtype;
-    const cudaError_t e = attn_launch_pdl(ctx, attn_append_kernel, dim3(total, 1), dim3(256), 0, (cudaStream_t)stream, a);
+    const cudaError_t e = attn_launch_pdl(ctx, attn_append_kernel, dim3(total), dim3(256), 0, (cudaStream_t)stream, a);
     JL_CUDA(ctx, e);
     ctx->st.launches++;
     ctx->st.served++;

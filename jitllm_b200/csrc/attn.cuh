@@ -289,7 +289,7 @@ static cudaError_t attn_launch_pdl(const jl_ctx *ctx, void (*kern)(P...), dim3 g
 
 // attn_few.cu, attn_tc5.cu, attn.cu
 int attn_launch_few(jl_ctx *ctx, const AttnArgs &a, int dtype, cudaStream_t s);
-// max_rows: query rows of a sequence and kv head, at most. JL_DECLINED: no tensor map for these strides
+// max_rows: query rows of a sequence and kv head, at most
 int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &a, int dtype, long long max_rows, cudaStream_t s);
 // unit: positions below which no cut divides an item
 int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, int unit, cudaStream_t s);

@@ -887,7 +887,7 @@ int attn_launch_tc5(jl_ctx *ctx, const AttnArgs &args, int dtype, long long max_
     const cuuint64_t ks[3] = {(cuuint64_t)a.kv_tok * 2, (cuuint64_t)a.kv_head * 2, a.table ? (cuuint64_t)a.kv_page * 2 : (cuuint64_t)a.kv_tok * 2};
     const cuuint32_t kb[4] = {64, (cuuint32_t)box_rows, 1, 1};
     if (!ta_map(&q, a.q, bf16, 3, qd, qs, qb) || !ta_map(&k, a.k, bf16, 4, kd, ks, kb) || !ta_map(&v, a.v, bf16, 4, kd, ks, kb))
-        return JL_DECLINED;
+        return jl_set_err(ctx, JL_ENOTSUP, "attention: the driver makes no tensor map of these strides");       // it does of all that are let through
     if (tiles == 1) return a.d == 128 ? ta_type<128, 1>(ctx, a, bf16, q, k, v, box_rows, s) : ta_type<64, 1>(ctx, a, bf16, q, k, v, box_rows, s);
     return a.d == 128 ? ta_type<128, 2>(ctx, a, bf16, q, k, v, box_rows, s) : ta_type<64, 2>(ctx, a, bf16, q, k, v, box_rows, s);
 }

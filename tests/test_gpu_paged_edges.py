@@ -264,3 +264,35 @@ def test_a_short_limit_does_not_end_long_work(new, lens):
             assert d.StatusPoll()
             got.append(out)
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("rows", [3, 12, 200])
+@pytest.mark.parametrize("what", ["kv heads", "kv rows", "q heads", "q rows", "overlapping rows", "far rows"])
+def test_strides_that_repeat_overlap_or_leap(dev, rows, what):
+    """Views whose strides are zero, smaller than a row or large: on the kernel for few rows and on the tensor core's."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(12)
+    hq, hkv, d = 8, 4, 64
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").bfloat16()
+    q, k, v = randn(rows, hq, d), randn(rows, hkv, d), randn(rows, hkv, d)
+    if what == "kv heads":
+        k, v = k[:, :1].expand(-1, hkv, -1), v[:, :1].expand(-1, hkv, -1)
+    elif what == "kv rows":
+        k, v = k[:1].expand(rows, -1, -1), v[:1].expand(rows, -1, -1)
+    elif what == "q heads":
+        q = q[:, :1].expand(-1, hq, -1)
+    elif what == "q rows":
+        q = q[:1].expand(rows, -1, -1)
+    elif what == "overlapping rows":
+        q, k, v = (randn(8 * rows + h * d).as_strided((rows, h, d), (8, d, 1)) for h in (hq, hkv, hkv))
+    else:
+        q, k, v = (randn(h * 8192 + rows * d).as_strided((rows, h, d), (d, 8192, 1)) if rows * d <= 8192 else
+                   randn(rows * 8192).as_strided((rows, h, d), (8192, d, 1)) for h in (hq, hkv, hkv))
+    for dt in ("f32", "bf16"):
+        out = torch.full((rows, hq, d), 7.0, device="cuda", dtype=_dt(dt))
+        dev.AttnPrompt(out, q, k, v, _starts([rows]), _scratch(dev), stream=_stream())
+        torch.cuda.synchronize()
+        assert dev.StatusPoll()
+        _check(out, *_reference(q, k, v, 0, d ** -0.5), torch.bfloat16, rows, d)
