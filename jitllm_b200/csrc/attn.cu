@@ -63,8 +63,9 @@ __device__ __forceinline__ void attn_merge_load(const float *p, float (&v)[D / 3
 // is known is asked for at once, the maxima, the sums and the first parts' rows, and weighed once it is there.
 
 // Many rows and, as a rule, few parts: block (c, y) takes 16 rows, a warp two of them side by side. One row to a warp needs four waves of
-// blocks (prompts of 1531 tokens 48.9 us in all, of 24 requests 60.4; with two rows 47.4 and 58.9), four take registers from the loads'
-// overlap (49.1, 59.4; a long sequence of 37 parts 275 us instead of 253). More of the parts' rows ahead than two: the same (4: 48.9).
+// blocks (five tokens of 32 sequences 50 us in all, 24 prompts 61.7; with two rows 48.5 and 60.8), four take registers from the loads'
+// overlap (50, 61.4, 1531 tokens 52.7 instead of 50.5; a mixed step 142 instead of 138). Four of the parts' rows ahead instead of two: 1531 tokens
+// 52.4, the step 140.
 #define ATTN_MERGE_ROWS 2
 #define ATTN_MERGE_AHEAD 2
 template <int D>
@@ -141,8 +142,8 @@ __global__ void __launch_bounds__(256) attn_merge_many_kernel(const __grid_const
 }
 
 // Few rows: block (c, y) takes rows y, y + 8, ... of the item. A handful of parts: a warp to a row. Hundreds (a long sequence): the eight
-// warps share a row, each a run of its parts, the runs added in order (131,071 positions of two kv heads, 222 parts to a row: 150 us with
-// one warp and one part at a time; 52.9 in all with four blocks to an item, 48.4 with eight).
+// warps share a row, each a run of its parts, the runs added in order (131,071 positions of two kv heads, 222 parts to a row: the join
+// alone 150 us with one warp and one part at a time; 46.8 in all with four blocks to an item, 45 with eight; 64 sequences 87.6 and 89.3).
 #define ATTN_MERGE_BLOCKS 8
 template <int ROWS, int D>
 __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_constant__ AttnArgs a, int ctas) {
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(256) attn_merge_few_kernel(const __grid_consta
 }
 
 int attn_launch_merge(jl_ctx *ctx, const AttnArgs &a, int rows, int ctas, int unit, cudaStream_t s) {
-    // Sequences that can be no longer than a unit leave no parts: 11 us instead of 16 for a prompt of seven tokens.
+    // Sequences that can be no longer than a unit leave no parts: 10.7 us instead of 16 for a prompt of seven tokens.
     if ((a.table ? (long long)a.max_pages << a.page_shift : (long long)a.total) <= unit) return JL_OK;
     const dim3 few(ctas, ATTN_MERGE_BLOCKS), many(ctas, rows / (8 * ATTN_MERGE_ROWS));
     const cudaError_t e = rows == ATTN_FEW_ROWS

@@ -3,24 +3,24 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale log2(e) q.k_j - m),  m the largest exponent so far
 //
-// Per position and kv head 4 d bytes are read for 64 d multiply-adds: bound by the cache's bytes. A CTA is four warps; a unit is 64
+// Per position and kv head 4 d bytes are read for 48 d multiply-adds (64 d for f32 results of bf16): bound by the cache's bytes. A CTA is four warps; a unit is 64
 // positions, 16 of them a warp's, and each warp runs its own cp.async ring, running maximum, sum and accumulators: no warp waits
 // for another before the end of the CTA's positions. mma.sync, not tcgen05: the products are a few percent of the tensor cores' time, and an
 // accumulator in registers needs no barrier between a tile's softmax and its product with V.
 //
-// Measured: 64 sequences of 37 to 8200 positions, 32 heads over 8, 408 MB: 88 us, 4.6 TB/s. The loop itself reads at 6.0 TB/s (long
+// Measured: 64 sequences of 37 to 8200 positions, 32 heads over 8, 408 MB: 89 us, 4.6 TB/s. The loop itself reads at 6.0 TB/s (long
 // sequences of equal length, 1.3 GB: 5.4 TB/s with everything); the rest is the share's start (4 us: lengths, table, first tiles, one after the
-// other), items' starts and ends, the last CTAs' 8 us and the join (6 us). Few positions are latency: 2049 of one sequence take 15.7 us.
+// other), items' starts and ends, the last CTAs' 8 us and the join (6 us). Few positions are latency: 2049 of one sequence take 16 us.
 // Tried and not kept: a ring that runs on into the next item while this one's sums are joined, 16 columns at a time (the join of the warps
-// costs what the loads save, the other CTAs of the SM fill the gap anyway: 89 us).
+// costs what the loads save, the other CTAs of the SM fill the gap anyway: a microsecond slower).
 #include "attn.cuh"
 
 #define FEW_UNIT_SHIFT 6
 #define FEW_STAGES 2
 // In units, for 64 sequences of 37 to 8200 positions:
-#define FEW_ITEM_COST 4          // an item's start and end: 1, 2, 3 and 4 take 109, 98, 93 and 93 us
-#define FEW_SNAP 2               // 0, 2 and 6 take 95, 94 and 99 us
-#define FEW_MIN_UNITS 2          // of a share: 1 and 2 take 17.1 and 15.7 us for 2049 positions: twice the parts to join
+#define FEW_ITEM_COST 4          // an item's start and end: 1, 2, 3 and 4 take 105, 96, 89 and 89 us
+#define FEW_SNAP 2               // 0, 2 and 6 take 90, 89 and 96 us
+#define FEW_MIN_UNITS 2          // of a share: 1 and 2 take 16.2 and 16.0 us for 2049 positions: twice the parts to join
 
 template <int D> struct FewTile {
     static constexpr int ROW = 2 * D + 16;            // bytes of a staged row: padded, so that rows start in different banks

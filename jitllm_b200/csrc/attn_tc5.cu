@@ -23,7 +23,8 @@
 // unit), rows split over two warps (the exchange of their maxima costs as much), S in halves of 64 positions with columns of their own
 // (the products S = Q K^T then read Q twice as often and take 1.5 times as long), an MMA warp to a tile (their products run side by side
 // and the tiles fall into step), masked tiles on the short way (a second copy of it: registers spill, every case is 3 to 8 % slower).
-// A 16,384-token prompt of 32 heads over 8: 2.0 ms, 1.10 PFLOP/s, at the clock that the power limit leaves. Short prompts are bound by their
+// A 16,384-token prompt of 32 heads over 8: 2.05 to 2.1 ms, 1.05 to 1.08 PFLOP/s, at the clock that the power limit leaves (1.8 ms in the
+// first moments of a cool GPU). Short prompts are bound by their
 // items' ends: a 1531-token one spends 2 x 10,000 of a CTA's 70,000 clocks on them (7000 on the rows' way out, the rest on masks).
 #include "attn.cuh"
 #include "tc5.cuh"
@@ -42,16 +43,17 @@ template <int TILES> struct TaRoles {
 };
 #define TA_STATUS_CODE 7
 // What an item's start and end take against a unit: Q's arrival, the first S, the last product, the rows' way out; 10,000 clocks beside
-// 3250 of two tiles, 6000 beside 2900 of one. 24 prompts of 1 to 1900 tokens take 71 us with 1, 64.5 with 2 and 3, 67 with 4; one of
-// 16,384 takes 2250, 2070, 2015 and 2020; shorter ones move by how the cuts happen to fall (1531: 54, 49, 54, 52).
+// 3250 of two tiles, 6000 beside 2900 of one. With 1, 2, 3 and 4 a prompt of 16,384 tokens takes 2270, 2020, 1875 and 1865 us, 24 prompts of 1
+// to 1900 tokens 72, 61.5, 60.8 and 65, one of 1531 52, 48.5, 50.5 and 49 (how the cuts happen to fall). One tile, 1, 2 and 3: 49.5, 48
+// and 47.5 us for five tokens of 32 sequences.
 #define TA_ITEM_COST 3
 #define TA_ITEM_COST_ONE 2
 // Two tiles: a cut one unit from an item's end moves onto it. The sliver that it saves costs its CTA 10,000 clocks; a cut further off,
-// moved, would cost the CTA next to it more (a 1531-token prompt 53 us with two units, 48.7 with one, 50 with none; 24 packed prompts 62.5,
-// 60.4, 62). One tile has less to save: 48.3 us with none, 50 to 53 with one for five tokens of 32 sequences.
+// moved, would cost the CTA next to it more (24 packed prompts 61.1 us with none, 60.8 with one unit, 62.6 with two; 1531 tokens 49.8, 50.5,
+// 50.2). One tile has less to save: the same with none and with one.
 #define TA_SNAP 1
-// One tile up to as many rows as it has (five tokens of 8 heads: 50 us against 62 with a second tile idle); beyond, two: a 1531-token
-// prompt takes 49 us so and 60 as single tiles, whose CTAs load K and V each for itself.
+// One tile up to as many rows as it has (five tokens of 8 heads: 48 us against 55 with a second tile idle); beyond, two: a 1531-token
+// prompt takes 50.5 us so and 58 as single tiles, whose CTAs load K and V each for itself.
 #define TA_ONE_TILE_ROWS 128
 // log2 of a weight at the reference, and the limit of a tile's sum of weights. f16 ends at 2^-24 and at 65504: with weights of one at the
 // reference a long flat tail below 2^-25 of it would leave the products but not the sum (131,071 positions: 0.4 % of a result). At 2^6 a
