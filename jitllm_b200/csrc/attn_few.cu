@@ -3,10 +3,10 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(scale log2(e) q.k_j - m),  m the largest exponent so far
 //
-// Per position and kv head 4 d bytes are read for 48 d multiply-adds (64 d for f32 results of bf16): bound by the cache's bytes. A CTA is four warps; a unit is 64
-// positions, 16 of them a warp's, and each warp runs its own cp.async ring, running maximum, sum and accumulators: no warp waits
-// for another before the end of the CTA's positions. mma.sync, not tcgen05: the products are a few percent of the tensor cores' time, and an
-// accumulator in registers needs no barrier between a tile's softmax and its product with V.
+// Per position and kv head 4 d bytes are read for 48 d multiply-adds (64 d for f32 results of bf16): bound by the cache's bytes. A CTA is
+// four warps; a unit is 64 positions, 16 of them a warp's, and each warp runs its own cp.async ring, running maximum, sum and accumulators:
+// no warp waits for another before the end of the CTA's positions. mma.sync, not tcgen05: the products are a few percent of the tensor
+// cores' time, and an accumulator in registers needs no barrier between a tile's softmax and its product with V.
 //
 // Measured: 64 sequences of 37 to 8200 positions, 32 heads over 8, 408 MB: 89 us, 4.6 TB/s. The loop itself reads at 6.0 TB/s (long
 // sequences of equal length, 1.3 GB: 5.4 TB/s with everything); the rest is the share's start (4 us: lengths, table, first tiles, one after the

@@ -481,9 +481,11 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                             tc5_commit(h_used + 8 * i);
 #pragma unroll
                             for (int x = 0; x < TA_KV / 16; ++x) part(x, 16, false);
+                        } else if (j + 1 < e) {
+                            scores(i, sk);
+                        } else {
+                            tc5_commit(o_full + 8 * i);
                         }
-                        else if (j + 1 < e) scores(i, sk);
-                        else tc5_commit(o_full + 8 * i);
                     }
                     done[i]++;
                 };
@@ -583,10 +585,11 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
         // ------------------------------------------------ softmax: warpgroup i owns tile i, a thread one of its rows
         // The weights of a tile are taken to a reference of the tiles before it, without looking for the tile's own maximum first (250
         // clocks): nothing is lost as long as they stay in range, and their sum, which is taken anyway, says whether they do. A row's
-        // first reference is the largest of its first 16 scores (f16: of its first tile's). Where the sum passes the limit (or is NaN), in masked tiles, and for f32
-        // results, S is read for its maximum, O rescaled -- S's arrival tells that the product before it is complete -- and the weights
-        // taken to that: S stays whole until P is written over it. The sums and products are f32, so scaled by up to the limit they lose
-        // nothing. The two ways are kept apart: a loop around one of them, or masks in it, cost 100 to 470 clocks a tile.
+        // first reference is the largest of its first 16 scores (f16, whose weights have less room: of its first tile's). Where the sum
+        // passes the limit (or is NaN), in masked tiles, and for f32 results, S is read for its maximum, O rescaled -- S's arrival tells
+        // that the product before it is complete -- and the weights taken to that: S stays whole until P is written over it. The sums and
+        // products are f32, so scaled by up to the limit they lose nothing. The two ways are kept apart: a loop around one of them, or
+        // masks in it, cost 100 to 470 clocks a tile.
         const int i = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;           // 32 lanes a warp, in bits 16 and up of a TMEM address
         const uint32_t S = tmem + i * 128 + lanes, O = tmem + TM_O + i * 128 + lanes;
@@ -642,7 +645,7 @@ attn_tc5_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUte
                 // what the scores' exponents start from
                 auto minus = [&](float ref) { return ref == -INFINITY ? 0.f : BF16 || HILO ? -ref * c : fmaf(-ref, c, W::LOG_TOP); };
                 bool slow = masked || HILO;
-                if (BF16 && j == 0 && !slow) {                             // any of a row's scores may be the first reference
+                if (BF16 && j == 0 && !slow) {                       // any of a row's scores may be the first reference
                     uint32_t v[16];
                     tc5_ld16(S, v);
                     ta_wait_ld(v);

@@ -296,3 +296,53 @@ def test_strides_that_repeat_overlap_or_leap(dev, rows, what):
         torch.cuda.synchronize()
         assert dev.StatusPoll()
         _check(out, *_reference(q, k, v, 0, d ** -0.5), torch.bfloat16, rows, d)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(1024, 64, 64), (300, 300, 128), (1000, 125, 64)])
+@pytest.mark.parametrize("new,max_new", [([1, 0, 2], 2), ([1, 70, 20], None)])
+def test_hundreds_of_heads(dev, hq, hkv, d, new, max_new):
+    import torch
+    lens = [33, 80, 150]
+    pool = Pool(lens, hkv, d, 16, _dt("bf16"), 2)
+    q = torch.randn(sum(new), hq, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).bfloat16()
+    out = torch.full((sum(new), hq, d), 7.0, device="cuda", dtype=torch.bfloat16)
+    dev.AttnPaged(out, q, pool.kv, _starts(new), _i32(lens), _scratch(dev), max_new=max_new, stream=_stream())
+    torch.cuda.synchronize()
+    assert dev.StatusPoll()
+    at = 0
+    for s, n in enumerate(new):
+        _check(out[at:at + n], *_reference(q[at:at + n], *pool.rows[s], lens[s] - n, d ** -0.5), _dt("bf16"), lens[s], d)
+        at += n
+
+
+@pytest.mark.parametrize("x", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hq,hkv,d", [(3, 2, 4), (5, 1, 12), (2, 2, 96), (4, 1, 256), (2, 1, 1024), (1, 600, 8)])
+def test_the_writer_takes_any_multiple_of_four(dev, x, hq, hkv, d):
+    """Head sizes that the attention does not serve. One rounding to the cache's type of a result that is off by 2^-24 for each of two
+    products and their sum."""
+    import torch
+    from jitllm_b200 import PagedKV
+    new, lens, p = [3, 1, 20], [3, 17, 45], 16
+    table = torch.arange(9, device="cuda", dtype=torch.int32).flip(0).view(3, 3)
+    k = torch.full((9, hkv, p, d), 7.0, device="cuda", dtype=torch.bfloat16)
+    v = torch.full_like(k, 7.0)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    qkv = torch.randn(25, (hq + 2 * hkv) * d, device="cuda", generator=g).to(_dt(x))
+    ang = torch.arange(64, device="cuda")[:, None] * 0.7 ** torch.arange(d // 2, device="cuda")[None, :]
+    cos, sin = ang.cos(), ang.sin()
+    q = torch.full((25, hq, d), 7.0, device="cuda", dtype=torch.bfloat16)
+    dev.RopeAppend(q, qkv, PagedKV(k, v, table), _starts(new), _i32(lens), cos, sin, stream=_stream())
+    torch.cuda.synchronize()
+    pos = torch.cat([torch.arange(n - m, n, device="cuda") for n, m in zip(lens, new)])
+    seq = torch.cat([torch.full((m,), s, device="cuda") for s, m in enumerate(new)])
+    rows = qkv[:24].double().view(24, hq + 2 * hkv, d)
+    a, b = rows[:, :hq + hkv, 0::2], rows[:, :hq + hkv, 1::2]
+    c, s = cos[pos].double()[:, None], sin[pos].double()[:, None]
+    rot, size = torch.stack((a * c - b * s, a * s + b * c), -1).flatten(-2), (a.abs() + b.abs()).repeat_interleave(2, -1)
+    page, slot = table[seq, pos // p].long(), pos % p
+    tol = rot.abs() * 2.0 ** -8 + size * 3 * 2.0 ** -24 * (1 + 2.0 ** -8)
+    assert not bool(((q[:24].double() - rot[:, :hq]).abs() > tol[:, :hq]).any()) and bool((q[24] == 7.0).all())
+    assert not bool(((k[page, :, slot].double() - rot[:, hq:]).abs() > tol[:, hq:]).any())
+    assert torch.equal(v[page, :, slot], rows[:, hq + hkv:].to(torch.bfloat16))
+    k[page, :, slot], v[page, :, slot] = 7.0, 7.0
+    assert bool((k == 7.0).all()) and bool((v == 7.0).all())               # nothing else was written
