@@ -328,7 +328,7 @@ int check_common(jl_ctx *ctx, const char *name, const void *out, int out_dtype, 
     if (nseq < 1 || total < 1 || hq < 1 || hkv < 1) return jl_set_err(ctx, JL_EINVAL, "%s: sizes below one", name);
     if (hq % hkv || hq / hkv > 16) return jl_set_err(ctx, JL_ENOTSUP, "%s: %d query heads over %d kv heads (a multiple, up to 16)", name, hq, hkv);
     if (d != 64 && d != 128) return jl_set_err(ctx, JL_ENOTSUP, "%s: head size %d (64 and 128 are served)", name, d);
-    if (!(scale > 0.f) || !(scale < INFINITY)) return jl_set_err(ctx, JL_EINVAL, "%s: the scale must be positive and finite", name);
+    if (!(scale > 0.f) || !(scale * 1.4426950408889634f < INFINITY)) return jl_set_err(ctx, JL_EINVAL, "%s: the scale must be positive and finite", name);
     if (total > (1 << 26) || hq > 1024 || nseq > (1 << 20)) return jl_set_err(ctx, JL_ENOTSUP, "%s: too many rows, heads or sequences", name);
     if (off16(out) || off16(q) || off16(k) || off16(v) || off16(scratch) || ((uintptr_t)starts & 3))
         return jl_set_err(ctx, JL_EINVAL, "%s: pointers must be 16-byte aligned (4 for the sequences' tables)", name);

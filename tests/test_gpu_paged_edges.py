@@ -346,3 +346,14 @@ def test_the_writer_takes_any_multiple_of_four(dev, x, hq, hkv, d):
     assert torch.equal(v[page, :, slot], rows[:, hq + hkv:].to(torch.bfloat16))
     k[page, :, slot], v[page, :, slot] = 7.0, 7.0
     assert bool((k == 7.0).all()) and bool((v == 7.0).all())               # nothing else was written
+
+
+@pytest.mark.parametrize("scale", [3.0e38, float("inf"), float("nan"), 0.0, -1.0])
+def test_a_scale_that_leaves_f32_is_refused(dev, scale):
+    """To the base 2 a scale is 1.44 times as large: past 2.35e38 it would be infinite, and a score of zero not a number."""
+    import torch
+    from jitllm_b200 import DeviceError, _lib
+    q = torch.zeros(4, 2, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(DeviceError) as e:
+        dev.AttnPrompt(torch.empty_like(q), q, q, q, _starts([4]), _scratch(dev), scale=scale)
+    assert e.value.status == _lib.EINVAL
